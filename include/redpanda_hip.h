@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define RP_ABI_VERSION 14
+#define RP_ABI_VERSION 15
 
 /* element type codes of the streamed scan inputs (delta, u, Bc, Cc); each
  * tensor carries its own code, as autocast hands over mixed dtypes */
@@ -372,6 +372,128 @@ int rp_ply_gather_check(const rp_ply_gather_args* a);
 
 /* The legal moves' logits of every rollout of a ply. */
 int rp_ply_gather(const rp_ply_gather_args* a, void* stream);
+
+/*
+ * Dropout whose mask is never stored: out = [res +] keep * x * 65536 / (65536 -
+ * t), t = round(65536 p).  The mask comes from Philox4x32-10 with the seed as
+ * its key and (column / 8, low word of the row, stream, high word of the row)
+ * as its counter; column 8 b + 2 j + i takes the low (i = 0) or high half of
+ * output word j, and is kept where that half is at least t.  The same seed and
+ * stream give the same mask for any dtype, stride and device, so the backward
+ * pass is this call on the output's gradient, without res.
+ * x: (rows, d) in dtype_x with row stride x_sr; res: NULL or (rows, d) in
+ * dtype_res with row stride res_sr; out: (rows, d) contiguous in dtype_out
+ * (any of the three), the sum in fp32 rounded once.  seed_ptr: NULL (the value
+ * `seed` is used) or a device word that holds the seed when the kernel runs.
+ * Rows need only their elements' alignment.  out must not overlap x or res.
+ */
+typedef struct rp_dropout_args {
+  int64_t rows, d;
+  int32_t dtype_x, dtype_res, dtype_out;
+  uint32_t stream;
+  double p;
+  uint64_t seed;
+  const uint64_t* seed_ptr;
+  const void* x;    int64_t x_sr;
+  const void* res;  int64_t res_sr;
+  void* out;
+} rp_dropout_args;
+
+/* Validate dropout arguments on the host without launching anything. */
+int rp_dropout_check(const rp_dropout_args* a);
+int rp_dropout(const rp_dropout_args* a, void* stream);
+
+/*
+ * Layer norm over the last dimension, with GELU (the exact one) on its input
+ * and dropout on its output folded in: the middle of a search model's head
+ * (engine/search_mamba.py:52-72: Linear, GELU, LayerNorm, Linear).
+ *     h = gelu ? GELU(x) : x;  out = drop((h - mean) rstd w + b)
+ * per row, rstd = 1 / sqrt(mean((h - mean)^2) + eps); the dropout (p > 0) is
+ * rp_dropout's with the same seed, stream and rows.  x: (rows, d) in dtype_x
+ * with row stride x_sr; w, b: (d,) fp32, or NULL (1 and 0); out: (rows, d)
+ * contiguous in dtype_out, which must not overlap x; stats: (rows, 2) fp32, each
+ * row's mean and rstd (rp_layernorm_fwd writes them unless NULL;
+ * rp_layernorm_bwd reads them).  All arithmetic in fp32.
+ */
+typedef struct rp_layernorm_args {
+  int64_t rows, d;
+  int32_t dtype_x, dtype_out, gelu;
+  uint32_t stream;
+  double p;
+  uint64_t seed;
+  const uint64_t* seed_ptr;
+  const void* x;   int64_t x_sr;
+  const float* w;
+  const float* b;
+  void* out;
+  float* stats;
+  float eps;
+  int32_t reserved;
+} rp_layernorm_args;
+
+/*
+ * Layer norm backward.  dout: (rows, d) in dtype_out with row stride dout_sr;
+ * dx: NULL or (rows, d) contiguous in dtype_x; dw, db: (d,) fp32 each, or both
+ * NULL (their sums over the rows are taken in a fixed order).  The forward's
+ * `out` is not read.  work: rp_layernorm_work_bytes() of scratch, 256-byte
+ * aligned (unused without dw and db).
+ */
+typedef struct rp_layernorm_grad {
+  const void* dout; int64_t dout_sr;
+  void* dx;
+  float* dw;
+  float* db;
+  void* work;
+  int64_t work_bytes;
+} rp_layernorm_grad;
+
+/* Validate layer norm arguments on the host without launching anything. */
+int rp_layernorm_check(const rp_layernorm_args* a);
+
+/* Bytes of scratch rp_layernorm_bwd needs. */
+int64_t rp_layernorm_work_bytes(const rp_layernorm_args* a);
+int rp_layernorm_fwd(const rp_layernorm_args* a, void* stream);
+int rp_layernorm_bwd(const rp_layernorm_args* a, const rp_layernorm_grad* g, void* stream);
+
+/*
+ * One token a row, drawn from logits with given uniform numbers.  A row's
+ * candidates are its logits above -inf, over the vocabulary or over a list of
+ * ids (ids outside [0, V) are padding; an id listed twice is two candidates).
+ * In order of value, then of place in the row, those are kept that are
+ *   - among the first top_k (<= 0: all),
+ *   - and have less weight before them than top_p of the weight of those
+ *     (top_p >= 1: all),
+ *   - and a weight of at least min_p,
+ * weights exp((l - largest) / temperature); the first is always kept, and is
+ * the only one where temperature <= 0.  The token is the first kept one, in
+ * order of its place, at which the running weight exceeds u times the kept
+ * ones' total (u in [0, 1); from 1 on: the last kept one).
+ * logits: (R, V) in dtype_logits with row stride logits_sr; u: (R,) fp32;
+ * tokens: NULL or (R, M) int32 with row stride tokens_sr.  temperature, top_p,
+ * min_p, top_k: one value, or where the *_row pointer is given (R,) values.
+ * ids: (R,) int64, -1 for a row without candidates; logp: NULL or (R,) fp32, the
+ * logarithm of the token's share of the kept weights (-inf without candidates).
+ * Weights are summed as 64-bit integers, so results do not depend on order.
+ */
+typedef struct rp_sample_args {
+  int64_t R, V, M;
+  int32_t dtype_logits, reserved;
+  const void* logits;     int64_t logits_sr;
+  const float* u;
+  const int32_t* tokens;  int64_t tokens_sr;
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const float* temperature_row;
+  const float* top_p_row;
+  const float* min_p_row;
+  const int32_t* top_k_row;
+  int64_t* ids;
+  float* logp;
+} rp_sample_args;
+
+/* Validate rp_sample arguments on the host without launching anything. */
+int rp_sample_check(const rp_sample_args* a);
+int rp_sample(const rp_sample_args* a, void* stream);
 
 /* ABI version this library was built with (RP_ABI_VERSION). */
 int rp_abi_version(void);

@@ -13,13 +13,16 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libredpanda_hip.so")
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 RP_F32, RP_BF16, RP_F16 = 0, 1, 2
 DTYPE_CODES = {torch.float32: RP_F32, torch.bfloat16: RP_BF16, torch.float16: RP_F16}
 MAX_STATE = 128
 
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
+_u32 = ctypes.c_uint32
+_u64 = ctypes.c_uint64
+_f64 = ctypes.c_double
 _vp = ctypes.c_void_p
 
 
@@ -134,6 +137,40 @@ class PlyGatherArgs(ctypes.Structure):
     ]
 
 
+class DropoutArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("d", _i64), ("dtype_x", _i32), ("dtype_res", _i32), ("dtype_out", _i32),
+        ("stream", _u32), ("p", _f64), ("seed", _u64), ("seed_ptr", _vp),
+        ("x", _vp), ("x_sr", _i64), ("res", _vp), ("res_sr", _i64), ("out", _vp),
+    ]
+
+
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("d", _i64), ("dtype_x", _i32), ("dtype_out", _i32), ("gelu", _i32),
+        ("stream", _u32), ("p", _f64), ("seed", _u64), ("seed_ptr", _vp),
+        ("x", _vp), ("x_sr", _i64), ("w", _vp), ("b", _vp), ("out", _vp), ("stats", _vp),
+        ("eps", ctypes.c_float), ("reserved", _i32),
+    ]
+
+
+class LayerNormGrad(ctypes.Structure):
+    _fields_ = [
+        ("dout", _vp), ("dout_sr", _i64), ("dx", _vp), ("dw", _vp), ("db", _vp),
+        ("work", _vp), ("work_bytes", _i64),
+    ]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [
+        ("R", _i64), ("V", _i64), ("M", _i64), ("dtype_logits", _i32), ("reserved", _i32),
+        ("logits", _vp), ("logits_sr", _i64), ("u", _vp), ("tokens", _vp), ("tokens_sr", _i64),
+        ("temperature", _f64), ("top_p", _f64), ("min_p", _f64), ("top_k", _i64),
+        ("temperature_row", _vp), ("top_p_row", _vp), ("min_p_row", _vp), ("top_k_row", _vp),
+        ("ids", _vp), ("logp", _vp),
+    ]
+
+
 # Every symbol include/redpanda_hip.h declares, with its ctypes signature.
 SIGNATURES = {
     "rp_abi_version": (ctypes.c_int, []),
@@ -162,6 +199,15 @@ SIGNATURES = {
     "rp_ply_topk": (ctypes.c_int, [ctypes.POINTER(PlyTopkArgs), _vp]),
     "rp_ply_gather_check": (ctypes.c_int, [ctypes.POINTER(PlyGatherArgs)]),
     "rp_ply_gather": (ctypes.c_int, [ctypes.POINTER(PlyGatherArgs), _vp]),
+    "rp_dropout_check": (ctypes.c_int, [ctypes.POINTER(DropoutArgs)]),
+    "rp_dropout": (ctypes.c_int, [ctypes.POINTER(DropoutArgs), _vp]),
+    "rp_layernorm_check": (ctypes.c_int, [ctypes.POINTER(LayerNormArgs)]),
+    "rp_layernorm_work_bytes": (_i64, [ctypes.POINTER(LayerNormArgs)]),
+    "rp_layernorm_fwd": (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), _vp]),
+    "rp_layernorm_bwd": (ctypes.c_int, [ctypes.POINTER(LayerNormArgs),
+                                        ctypes.POINTER(LayerNormGrad), _vp]),
+    "rp_sample_check": (ctypes.c_int, [ctypes.POINTER(SampleArgs)]),
+    "rp_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), _vp]),
     "rp_mixer_out_check": (ctypes.c_int, [ctypes.POINTER(MixerOutArgs)]),
     "rp_mixer_out_work_bytes": (_i64, [ctypes.POINTER(MixerOutArgs)]),
     "rp_mixer_out_fwd": (ctypes.c_int, [ctypes.POINTER(MixerOutArgs), _vp]),

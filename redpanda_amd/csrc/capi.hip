@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <math.h>
 #include <mutex>
 #include <stdarg.h>
 #include <stdio.h>
@@ -12,6 +13,7 @@
 #include <string.h>
 
 #include "redpanda_hip.h"
+#include "rp_heads.h"
 #include "rp_launch.h"
 
 namespace {
@@ -1220,6 +1222,281 @@ int rp_softplus(const float* x, float* out, int64_t n, void* stream) {
     return fail(RP_ERR_INVALID, "softplus: misaligned buffer");
   hipError_t e = rp::launch_softplus(x, out, n, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "softplus launch");
+  return RP_OK;
+}
+
+namespace {
+
+bool known_dtype(int dt) { return dt == RP_F32 || dt == RP_BF16 || dt == RP_F16; }
+
+// Bytes from the first to past the last element of (rows, d) with row stride sr.
+int64_t rows_bytes(int64_t rows, int64_t d, int64_t sr, int64_t es) {
+  return ((rows - 1) * sr + d) * es;
+}
+
+// Sizes the head operators index with: element offsets stay in int64, a row's
+// blocks of eight columns in int32.
+int check_rows(int64_t rows, int64_t d, int64_t sr, const char* what) {
+  if (rows < 0 || d < 0) return fail(RP_ERR_INVALID, "%s args: negative size", what);
+  if (d > kI32Max) return fail(RP_ERR_UNSUPPORTED, "%s args: d must fit in int32", what);
+  if (rows > 0 && sr < d) return fail(RP_ERR_INVALID, "%s args: x row stride shorter than d", what);
+  if (rows > ((int64_t)1 << 40) || (rows > 0 && sr > 0 && rows > ((int64_t)1 << 60) / sr))
+    return fail(RP_ERR_UNSUPPORTED, "%s args: too many elements", what);
+  return RP_OK;
+}
+
+int drop_params(double p, uint32_t stream, uint64_t seed, const uint64_t* seed_ptr,
+                const char* what, rp::DropParams* out) {
+  if (!(p >= 0.0 && p <= 1.0)) return fail(RP_ERR_INVALID, "%s args: p must be in [0, 1]", what);
+  if (!aligned(seed_ptr, 8)) return fail(RP_ERR_INVALID, "%s args: misaligned seed", what);
+  out->t = (uint32_t)nearbyint(65536.0 * p);
+  out->scale = out->t < 65536 ? (float)(65536.0 / (65536 - out->t)) : 0.f;
+  out->stream = stream;
+  out->seed = seed;
+  out->seed_ptr = seed_ptr;
+  return RP_OK;
+}
+
+}  // namespace
+
+int rp_dropout_check(const rp_dropout_args* a) {
+  if (a == nullptr) return fail(RP_ERR_INVALID, "dropout args: NULL");
+  int st = check_rows(a->rows, a->d, a->x_sr, "dropout");
+  if (st != RP_OK) return st;
+  if (!known_dtype(a->dtype_x) || !known_dtype(a->dtype_out) ||
+      (a->res && !known_dtype(a->dtype_res)))
+    return fail(RP_ERR_INVALID, "dropout args: unknown dtype code");
+  rp::DropParams dp;
+  st = drop_params(a->p, a->stream, a->seed, a->seed_ptr, "dropout", &dp);
+  if (st != RP_OK) return st;
+  if (a->rows == 0 || a->d == 0) return RP_OK;
+  if (!a->x || !a->out) return fail(RP_ERR_INVALID, "dropout args: NULL x / out");
+  const int64_t ex = elem_size(a->dtype_x), eo = elem_size(a->dtype_out);
+  if (!aligned(a->x, ex) || !aligned(a->out, eo))
+    return fail(RP_ERR_INVALID, "dropout args: misaligned pointer");
+  const int64_t ob = a->rows * a->d * eo;
+  if (overlaps(a->out, ob, a->x, rows_bytes(a->rows, a->d, a->x_sr, ex)))
+    return fail(RP_ERR_INVALID, "dropout args: out overlaps x");
+  if (a->res) {
+    const int64_t er = elem_size(a->dtype_res);
+    if (a->res_sr < a->d || a->res_sr > ((int64_t)1 << 60) / a->rows || !aligned(a->res, er))
+      return fail(RP_ERR_INVALID, "dropout args: res row stride shorter than d or misaligned");
+    if (overlaps(a->out, ob, a->res, rows_bytes(a->rows, a->d, a->res_sr, er)))
+      return fail(RP_ERR_INVALID, "dropout args: out overlaps res");
+  }
+  return RP_OK;
+}
+
+int rp_dropout(const rp_dropout_args* a, void* stream) {
+  int st = rp_dropout_check(a);
+  if (st != RP_OK || a->rows == 0 || a->d == 0) return st;
+  rp::DropoutParams p{};
+  drop_params(a->p, a->stream, a->seed, a->seed_ptr, "dropout", &p.drop);
+  p.rows = a->rows;
+  p.d = a->d;
+  p.dt_x = a->dtype_x;
+  p.dt_res = a->res ? a->dtype_res : RP_F32;
+  p.dt_out = a->dtype_out;
+  p.es_x = (int)elem_size(p.dt_x);
+  p.es_res = (int)elem_size(p.dt_res);
+  p.es_out = (int)elem_size(p.dt_out);
+  p.x = a->x;
+  p.xsr = a->x_sr;
+  p.res = a->res;
+  p.rsr = a->res_sr;
+  p.out = a->out;
+  hipError_t e = rp::launch_dropout(p, (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "dropout launch");
+  return RP_OK;
+}
+
+int rp_layernorm_check(const rp_layernorm_args* a) {
+  if (a == nullptr) return fail(RP_ERR_INVALID, "layernorm args: NULL");
+  int st = check_rows(a->rows, a->d, a->x_sr, "layernorm");
+  if (st != RP_OK) return st;
+  if (a->d == 0) return fail(RP_ERR_INVALID, "layernorm args: rows of no elements have no mean");
+  if (!known_dtype(a->dtype_x) || !known_dtype(a->dtype_out))
+    return fail(RP_ERR_INVALID, "layernorm args: unknown dtype code");
+  if (a->gelu != 0 && a->gelu != 1) return fail(RP_ERR_INVALID, "layernorm args: gelu must be 0 or 1");
+  if (!(a->eps >= 0.f)) return fail(RP_ERR_INVALID, "layernorm args: eps must be >= 0");
+  rp::DropParams dp;
+  st = drop_params(a->p, a->stream, a->seed, a->seed_ptr, "layernorm", &dp);
+  if (st != RP_OK) return st;
+  if (!aligned(a->w, 4) || !aligned(a->b, 4) || !aligned(a->stats, 4))
+    return fail(RP_ERR_INVALID, "layernorm args: misaligned pointer");
+  if (a->rows == 0) return RP_OK;
+  if (!a->x) return fail(RP_ERR_INVALID, "layernorm args: NULL x");
+  if (!aligned(a->x, elem_size(a->dtype_x)))
+    return fail(RP_ERR_INVALID, "layernorm args: misaligned pointer");
+  return RP_OK;
+}
+
+namespace {
+
+rp::LayerNormParams layernorm_params(const rp_layernorm_args* a) {
+  rp::LayerNormParams p{};
+  drop_params(a->p, a->stream, a->seed, a->seed_ptr, "layernorm", &p.drop);
+  p.rows = a->rows;
+  p.d = a->d;
+  p.dt_x = a->dtype_x;
+  p.dt_out = a->dtype_out;
+  p.es_x = (int)elem_size(p.dt_x);
+  p.es_out = (int)elem_size(p.dt_out);
+  p.gelu = a->gelu;
+  p.eps = a->eps;
+  p.x = a->x;
+  p.xsr = a->x_sr;
+  p.w = a->w;
+  p.b = a->b;
+  p.out = a->out;
+  p.stats = a->stats;
+  return p;
+}
+
+}  // namespace
+
+int64_t rp_layernorm_work_bytes(const rp_layernorm_args* a) {
+  if (rp_layernorm_check(a) != RP_OK) return -1;
+  return round_up((int64_t)rp::layernorm_parts(a->rows, a->d) * 2 * a->d * 4, 256);
+}
+
+int rp_layernorm_fwd(const rp_layernorm_args* a, void* stream) {
+  int st = rp_layernorm_check(a);
+  if (st != RP_OK || a->rows == 0) return st;
+  const int64_t eo = elem_size(a->dtype_out), ob = a->rows * a->d * eo;
+  const int64_t xb = rows_bytes(a->rows, a->d, a->x_sr, elem_size(a->dtype_x));
+  if (!a->out || !aligned(a->out, eo))
+    return fail(RP_ERR_INVALID, "layernorm args: NULL or misaligned out");
+  if (overlaps(a->out, ob, a->x, xb) || (a->w && overlaps(a->out, ob, a->w, a->d * 4)) ||
+      (a->b && overlaps(a->out, ob, a->b, a->d * 4)) ||
+      (a->stats && (overlaps(a->stats, a->rows * 8, a->out, ob) ||
+                    overlaps(a->stats, a->rows * 8, a->x, xb))))
+    return fail(RP_ERR_INVALID, "layernorm args: an output overlaps another buffer");
+  hipError_t e = rp::launch_layernorm_fwd(layernorm_params(a), (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "layernorm fwd launch");
+  return RP_OK;
+}
+
+int rp_layernorm_bwd(const rp_layernorm_args* a, const rp_layernorm_grad* g, void* stream) {
+  int st = rp_layernorm_check(a);
+  if (st != RP_OK) return st;
+  if (g == nullptr) return fail(RP_ERR_INVALID, "layernorm grad: NULL");
+  if ((g->dw == nullptr) != (g->db == nullptr))
+    return fail(RP_ERR_INVALID, "layernorm grad: dw and db go together");
+  if (!aligned(g->dw, 4) || !aligned(g->db, 4))
+    return fail(RP_ERR_INVALID, "layernorm grad: misaligned pointer");
+  struct Span { const void* p; int64_t n; };
+  Span outs[3] = {{nullptr, 0}, {g->dw, a->d * 4}, {g->db, a->d * 4}};
+  if (a->rows > 0) {
+    const int64_t ex = elem_size(a->dtype_x), eo = elem_size(a->dtype_out);
+    if (!g->dout || !aligned(g->dout, eo) || g->dout_sr < a->d ||
+        g->dout_sr > ((int64_t)1 << 60) / a->rows)
+      return fail(RP_ERR_INVALID, "layernorm grad: NULL or misaligned dout, or a row stride below d");
+    if (!a->stats) return fail(RP_ERR_INVALID, "layernorm grad: the forward's stats are needed");
+    if (!aligned(g->dx, ex)) return fail(RP_ERR_INVALID, "layernorm grad: misaligned pointer");
+    outs[0] = {g->dx, a->rows * a->d * ex};
+    const Span ins[4] = {{g->dout, rows_bytes(a->rows, a->d, g->dout_sr, eo)},
+                         {a->x, rows_bytes(a->rows, a->d, a->x_sr, ex)},
+                         {a->w, a->d * 4}, {a->stats, a->rows * 8}};
+    for (const Span& o : outs)
+      for (const Span& i : ins)
+        if (o.p && i.p && overlaps(o.p, o.n, i.p, i.n))
+          return fail(RP_ERR_INVALID, "layernorm grad: an output overlaps an input");
+  }
+  for (int i = 0; i < 3; ++i)
+    for (int j = i + 1; j < 3; ++j)
+      if (outs[i].p && outs[j].p && overlaps(outs[i].p, outs[i].n, outs[j].p, outs[j].n))
+        return fail(RP_ERR_INVALID, "layernorm grad: outputs overlap");
+  if (g->dw) {
+    const int64_t need = rp_layernorm_work_bytes(a);
+    if (need > 0 && (!g->work || g->work_bytes < need || !aligned(g->work, 256)))
+      return fail(RP_ERR_WORKSPACE, "layernorm bwd: workspace needs %lld bytes (256-aligned), got %lld",
+                  (long long)need, (long long)g->work_bytes);
+  }
+  rp::LayerNormGrad lg{};
+  lg.dout = g->dout;
+  lg.dosr = g->dout_sr;
+  lg.dx = g->dx;
+  lg.dw = g->dw;
+  lg.db = g->db;
+  lg.part = static_cast<float*>(g->work);
+  hipError_t e = rp::launch_layernorm_bwd(layernorm_params(a), lg, (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "layernorm bwd launch");
+  return RP_OK;
+}
+
+int rp_sample_check(const rp_sample_args* a) {
+  if (a == nullptr) return fail(RP_ERR_INVALID, "sample args: NULL");
+  if (a->R < 0 || a->V < 1 || a->M < 0)
+    return fail(RP_ERR_INVALID, "sample args: R < 0, V < 1 or M < 0");
+  if (a->V > ((int64_t)1 << 30) || a->M > ((int64_t)1 << 30) || a->R > ((int64_t)1 << 31))
+    return fail(RP_ERR_UNSUPPORTED, "sample args: V and M up to 2^30, R up to 2^31");
+  if (!known_dtype(a->dtype_logits))
+    return fail(RP_ERR_INVALID, "sample args: unknown dtype code %d", a->dtype_logits);
+  if (!a->temperature_row && !(a->temperature >= 0.0))
+    return fail(RP_ERR_INVALID, "sample args: temperature must be >= 0");
+  if (!a->top_p_row && !(a->top_p >= 0.0))
+    return fail(RP_ERR_INVALID, "sample args: top_p must be >= 0");
+  if (!a->min_p_row && !(a->min_p >= 0.0 && a->min_p <= 1.0))
+    return fail(RP_ERR_INVALID, "sample args: min_p must be in [0, 1]");
+  if (a->R == 0) return RP_OK;
+  if (!a->logits || !a->u || !a->ids) return fail(RP_ERR_INVALID, "sample args: NULL logits / u / ids");
+  const int64_t es = elem_size(a->dtype_logits);
+  if (a->logits_sr < a->V || a->logits_sr > ((int64_t)1 << 60) / a->R)
+    return fail(RP_ERR_INVALID, "sample args: logits row stride below V");
+  if (a->tokens && (a->tokens_sr < a->M || a->tokens_sr > ((int64_t)1 << 60) / a->R))
+    return fail(RP_ERR_INVALID, "sample args: tokens row stride below M");
+  const void* words[] = {a->u, a->tokens, a->temperature_row, a->top_p_row, a->min_p_row,
+                         a->top_k_row, a->logp};
+  for (const void* w : words)
+    if (!aligned(w, 4)) return fail(RP_ERR_INVALID, "sample args: misaligned pointer");
+  if (!aligned(a->logits, es) || !aligned(a->ids, 8))
+    return fail(RP_ERR_INVALID, "sample args: misaligned pointer");
+  struct Span { const void* p; int64_t n; };
+  const Span outs[2] = {{a->ids, a->R * 8}, {a->logp, a->R * 4}};
+  const Span ins[7] = {{a->logits, rows_bytes(a->R, a->V, a->logits_sr, es)},
+                       {a->u, a->R * 4},
+                       {a->tokens, a->tokens ? rows_bytes(a->R, a->M, a->tokens_sr, 4) : 0},
+                       {a->temperature_row, a->R * 4}, {a->top_p_row, a->R * 4},
+                       {a->min_p_row, a->R * 4}, {a->top_k_row, a->R * 4}};
+  for (const Span& o : outs)
+    for (const Span& i : ins)
+      if (o.p && i.p && overlaps(o.p, o.n, i.p, i.n))
+        return fail(RP_ERR_INVALID, "sample args: an output overlaps an input");
+  if (a->logp && overlaps(a->ids, a->R * 8, a->logp, a->R * 4))
+    return fail(RP_ERR_INVALID, "sample args: outputs overlap");
+  return RP_OK;
+}
+
+int rp_sample(const rp_sample_args* a, void* stream) {
+  int st = rp_sample_check(a);
+  if (st != RP_OK || a->R == 0) return st;
+  rp::SampleParams p{};
+  p.R = a->R;
+  p.V = (int)a->V;
+  p.n = (int)(a->tokens ? a->M : a->V);
+  p.dt = a->dtype_logits;
+  // n weights of at most 2^shift sum to at most 2^62
+  int bits = 0;
+  while (((int64_t)1 << bits) < p.n) ++bits;
+  p.shift = std::min(51, 62 - bits);
+  p.logits = a->logits;
+  p.lsr = a->logits_sr;
+  p.u = a->u;
+  p.tokens = a->tokens;
+  p.tsr = a->tokens_sr;
+  p.T = a->temperature;
+  p.tp = a->top_p;
+  p.mp = a->min_p;
+  p.k = a->top_k;
+  p.T_row = a->temperature_row;
+  p.tp_row = a->top_p_row;
+  p.mp_row = a->min_p_row;
+  p.k_row = a->top_k_row;
+  p.ids = a->ids;
+  p.logp = a->logp;
+  hipError_t e = rp::launch_sample(p, (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "sample launch");
   return RP_OK;
 }
 

@@ -11,8 +11,7 @@
 // fp32 or wider; the variance from the centred values (a second look at the
 // row), since a mean of squares would cancel for rows far from zero.
 
-#include "rp_heads.h"
-#include "rp_rows.h"
+#include "layernorm_rows.h"
 
 namespace rp {
 
@@ -43,7 +42,8 @@ __device__ __forceinline__ void load_weights(const float* w, int64_t col, int64_
 
 }  // namespace
 
-// One workgroup per row, any length.
+// One workgroup per row, any length (for rows beyond the shapes of
+// layernorm_rows.h).
 __global__ __launch_bounds__(kThreads) void layernorm_fwd_kernel(LayerNormParams p) {
   __shared__ float buf[kWaves];
   const uint64_t seed = drop_seed(p.drop);
@@ -191,43 +191,84 @@ __global__ __launch_bounds__(kThreads) void layernorm_dw_kernel(LayerNormParams 
   }
 }
 
-// dw, db: the partial sums of each column, in fp64 and in order.
-__global__ __launch_bounds__(kThreads) void layernorm_sum_kernel(const float* part, int n, int64_t d,
-                                                                 float* dw, float* db) {
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= 2 * d) return;
+// dw, db: the n partial sums of each column, in fp64 and in a fixed order: 16
+// waves take every 16th of them for 64 columns, then one adds the waves'.
+__global__ __launch_bounds__(16 * kWave) void layernorm_sum_kernel(const float* part, int n, int64_t d,
+                                                                   float* dw, float* db) {
+  __shared__ double buf[16][kWave];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t c = (int64_t)blockIdx.x * kWave + lane;
   double s = 0.0;
-  for (int i = 0; i < n; ++i) s += part[(int64_t)i * 2 * d + c];
+  if (c < 2 * d) {
+    const float* at = part + c;
+    int i = wave;
+    for (; i + 7 * 16 < n; i += 8 * 16) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = at[(int64_t)(i + 16 * k) * 2 * d];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
+    for (; i < n; i += 16) s += at[(int64_t)i * 2 * d];
+  }
+  buf[wave][lane] = s;
+  __syncthreads();
+  if (wave > 0 || c >= 2 * d) return;
+#pragma unroll
+  for (int w = 1; w < 16; ++w) s += buf[w][lane];
   (c < d ? dw : db)[c < d ? c : c - d] = (float)s;
 }
 
 namespace {
+
 unsigned row_grid(int64_t rows) { return (unsigned)(rows < (1 << 20) ? rows : (1 << 20)); }
+
+// Workgroups of a launch whose groups of G lanes walk rows.
+unsigned walk_grid(int64_t rows, int G, int most) {
+  const int groups = norm_threads(G) / G;
+  const int64_t n = (rows + groups - 1) / groups;
+  return (unsigned)(n < most ? n : most);
+}
+
 }  // namespace
 
 int layernorm_parts(int64_t rows, int64_t d) {
+  const int G = norm_group(d);
+  if (G != 0) return (int)walk_grid(rows, G, kNormBwdWorkgroups);
   const int64_t tiles = (d + 8 * kWave - 1) / (8 * kWave);
-  int64_t n = (rows + 4 * kWaves - 1) / (4 * kWaves);
+  const int64_t n = (rows + 4 * kWaves - 1) / (4 * kWaves);
   const int64_t most = (2048 + tiles - 1) / tiles;
   return (int)(n < most ? n : most);
 }
 
 hipError_t launch_layernorm_fwd(const LayerNormParams& p, hipStream_t st) {
   if (p.rows == 0) return hipSuccess;
+  const int G = norm_group(p.d);
+  if (G != 0) {
+    const unsigned wg = walk_grid(p.rows, G, kNormFwdWorkgroups);
+    return p.es_x == 4 ? launch_norm_fwd4(p, wg, st) : launch_norm_fwd2(p, wg, st);
+  }
   hipLaunchKernelGGL(layernorm_fwd_kernel, dim3(row_grid(p.rows)), dim3(kThreads), 0, st, p);
   return hipGetLastError();
 }
 
 hipError_t launch_layernorm_bwd(const LayerNormParams& p, const LayerNormGrad& g, hipStream_t st) {
-  if (g.dx != nullptr && p.rows > 0)
-    hipLaunchKernelGGL(layernorm_dx_kernel, dim3(row_grid(p.rows)), dim3(kThreads), 0, st, p, g);
-  if (g.dw != nullptr) {
-    const int n = layernorm_parts(p.rows, p.d);
-    const unsigned tiles = (unsigned)((p.d + 8 * kWave - 1) / (8 * kWave));
-    if (n > 0) hipLaunchKernelGGL(layernorm_dw_kernel, dim3(tiles, n), dim3(kThreads), 0, st, p, g);
-    hipLaunchKernelGGL(layernorm_sum_kernel, dim3((unsigned)((2 * p.d + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, st, g.part, n, p.d, g.dw, g.db);
+  const int n = layernorm_parts(p.rows, p.d);
+  if (p.rows > 0 && norm_group(p.d) != 0) {
+    auto* launch = p.es_x == 4 ? (p.es_out == 4 ? launch_norm_bwd44 : launch_norm_bwd42)
+                               : (p.es_out == 4 ? launch_norm_bwd24 : launch_norm_bwd22);
+    const hipError_t e = launch(p, g, (unsigned)n, st);
+    if (e != hipSuccess) return e;
+  } else if (p.rows > 0) {
+    if (g.dx != nullptr)
+      hipLaunchKernelGGL(layernorm_dx_kernel, dim3(row_grid(p.rows)), dim3(kThreads), 0, st, p, g);
+    if (g.dw != nullptr)
+      hipLaunchKernelGGL(layernorm_dw_kernel, dim3((unsigned)((p.d + 8 * kWave - 1) / (8 * kWave)), n),
+                         dim3(kThreads), 0, st, p, g);
   }
+  if (g.dw != nullptr)
+    hipLaunchKernelGGL(layernorm_sum_kernel, dim3((unsigned)((2 * p.d + kWave - 1) / kWave)),
+                       dim3(16 * kWave), 0, st, g.part, n, p.d, g.dw, g.db);
   return hipGetLastError();
 }
 

@@ -20,18 +20,26 @@ struct Raw8 {
   uint32_t w[2 * ES];
 };
 
+// The eight elements at `col` of a row that has them all.
+template <int ES>
+__device__ __forceinline__ Raw8<ES> load_full8(const char* row, int64_t col) {
+  Raw8<ES> r;
+#pragma unroll
+  for (int q = 0; q < ES / 2; ++q) {
+    const u32x4_any v = *reinterpret_cast<const u32x4_any*>(row + col * ES + 16 * q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[4 * q + i] = v[i];
+  }
+  return r;
+}
+
 // The eight elements at `col` of a row of d (those at or past d as zero bits;
 // nothing past the row's end is read).
 template <int ES>
 __device__ __forceinline__ Raw8<ES> load_raw8(const char* row, int64_t col, int64_t d) {
   Raw8<ES> r;
   if (col + 8 <= d) {
-#pragma unroll
-    for (int q = 0; q < ES / 2; ++q) {
-      const u32x4_any v = *reinterpret_cast<const u32x4_any*>(row + col * ES + 16 * q);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r.w[4 * q + i] = v[i];
-    }
+    r = load_full8<ES>(row, col);
   } else {
 #pragma unroll
     for (int i = 0; i < 2 * ES; ++i) r.w[i] = 0;
@@ -76,9 +84,10 @@ __device__ __forceinline__ void load8(const void* row, int64_t col, int64_t d, i
 }
 
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, int dtype) {
-  if (dtype == RP_BF16) {
-    const auto b = [](float f) { return __float_as_uint(round_storage(f, RP_BF16)) >> 16; };
-    return b(lo) | (b(hi) << 16);
+  if (dtype == RP_BF16) {  // one instruction: to nearest even, a NaN stays one
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
   }
   const auto h = [](float f) {
     return (uint32_t)__builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
@@ -86,36 +95,37 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, int dtype) {
   return h(lo) | (h(hi) << 16);
 }
 
-// Eight elements at `col`, rounded to nearest even; those past d are not stored.
-__device__ __forceinline__ void store8(void* row, int64_t col, int64_t d, int dtype,
-                                       const float (&v)[8]) {
-  char* at = static_cast<char*>(row) + col * (dtype == RP_F32 ? 4 : 2);
+// Eight elements at `col` of a row that has them all, rounded to nearest even.
+__device__ __forceinline__ void store_full8(char* row, int64_t col, int dtype, const float (&v)[8]) {
+  u32x4_any w;
   if (dtype == RP_F32) {
-    if (col + 8 <= d) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        u32x4_any w;
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[4 * q + i]);
-        *reinterpret_cast<u32x4_any*>(at + 16 * q) = w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < d) reinterpret_cast<float*>(at)[i] = v[i];
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[4 * q + i]);
+      *reinterpret_cast<u32x4_any*>(row + col * 4 + 16 * q) = w;
     }
   } else {
-    u32x4_any w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = pack16(v[2 * i], v[2 * i + 1], dtype);
-    if (col + 8 <= d) {
-      *reinterpret_cast<u32x4_any*>(at) = w;
-    } else {
+    *reinterpret_cast<u32x4_any*>(row + col * 2) = w;
+  }
+}
+
+// The same; those at and past d are not stored.
+__device__ __forceinline__ void store8(void* row, int64_t col, int64_t d, int dtype,
+                                       const float (&v)[8]) {
+  if (col + 8 <= d) {
+    store_full8(static_cast<char*>(row), col, dtype, v);
+    return;
+  }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + i < d)
-          reinterpret_cast<uint16_t*>(at)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-    }
+  for (int i = 0; i < 8; ++i) {
+    if (col + i >= d) break;
+    if (dtype == RP_F32)
+      static_cast<float*>(row)[col + i] = v[i];
+    else
+      static_cast<uint16_t*>(row)[col + i] = (uint16_t)pack16(v[i], 0.f, dtype);
   }
 }
 

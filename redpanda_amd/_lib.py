@@ -276,4 +276,7 @@ def ptr(t):
 
 
 def stream_of(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    """The handle of the device's current stream (the raw handle: making a
+    torch.cuda.Stream object for it takes 2-3 us of a small call's 10)."""
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if device.index is None else device.index)

@@ -22,17 +22,18 @@ def dtype_code(dtype, what):
 
 
 def rows_of(t, d):
-    """(rows, d) view of t with unit inner stride and rows that do not overlap,
-    or a contiguous copy of it."""
-    if not t.is_contiguous():
-        if t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < d:
-            t = t.contiguous()
-    return t if t.dim() == 2 else t.view(-1, d)
+    """t as rows of d elements with unit inner stride that do not overlap: (t or a
+    contiguous copy of it, the number of rows, their stride)."""
+    if t.is_contiguous():
+        return t, t.numel() // d, d
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= d:
+        return t, t.shape[0], t.stride(0)
+    return t.contiguous(), t.numel() // d, d
 
 
-def row_stride(t):
-    """A row view's stride (of a single row, which may carry any, its length)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def empty_rows(t, dtype):
+    """A contiguous tensor of t's shape."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def check_p(p, what):
@@ -46,7 +47,7 @@ def seed_arg(seed, device, what):
     """(value, tensor or None) of a seed: an int, or an int64 tensor of one
     element on the device, which the kernels read when they run."""
     if isinstance(seed, torch.Tensor):
-        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
+        if seed.dtype is not torch.int64 or seed.numel() != 1 or seed.device != device:
             raise ValueError(f"{what}: a seed tensor must be one int64 on {device}, got "
                              f"{tuple(seed.shape)} {seed.dtype} on {seed.device}")
         return 0, seed
@@ -57,18 +58,18 @@ def seed_arg(seed, device, what):
 
 def _run(x, res, p, seed, seed_t, stream, out_dtype):
     lib = _lib.load()
-    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    out = empty_rows(x, out_dtype)
     if out.numel() == 0:
         return out
     d = x.shape[-1]
-    xr = rows_of(x, d)
-    a = _lib.DropoutArgs(xr.shape[0], d, _lib.DTYPE_CODES[x.dtype], 0, _lib.DTYPE_CODES[out_dtype],
-                         stream, p, seed, _lib.ptr(seed_t), xr.data_ptr(), row_stride(xr), None, 0,
-                         out.data_ptr())
+    x, rows, sr = rows_of(x, d)
+    a = _lib.DropoutArgs(rows, d, _lib.DTYPE_CODES[x.dtype], 0, _lib.DTYPE_CODES[out_dtype], stream, p,
+                         seed, None if seed_t is None else seed_t.data_ptr(), x.data_ptr(), sr, None,
+                         0, out.data_ptr())
     if res is not None:
-        rr = rows_of(res, d)
-        a.dtype_res, a.res, a.res_sr = _lib.DTYPE_CODES[res.dtype], rr.data_ptr(), row_stride(rr)
-    _lib.check(lib.rp_dropout(ctypes.byref(a), _lib.stream_of(x.device)), lib)
+        res, _, rsr = rows_of(res, d)
+        a.dtype_res, a.res, a.res_sr = _lib.DTYPE_CODES[res.dtype], res.data_ptr(), rsr
+    _lib.check(lib.rp_dropout(ctypes.byref(a), _lib.stream_of(out.device)), lib)
     return out
 
 
@@ -76,22 +77,18 @@ class _HipDropout(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, res, p, seed, seed_t, stream, out_dtype):
-        ctx.args = (p, seed, stream)
-        ctx.dtypes = (x.dtype, None if res is None else res.dtype)
-        if seed_t is not None:
-            ctx.save_for_backward(seed_t)
+        ctx.args = (p, seed, stream, x.dtype, None if res is None else res.dtype)
+        ctx.save_for_backward(seed_t)
         return _run(x, res, p, seed, seed_t, stream, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        p, seed, stream = ctx.args
-        seed_t = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        dx = dres = None
-        if ctx.needs_input_grad[0]:
-            dx = _run(dy, None, p, seed, seed_t, stream, ctx.dtypes[0])
-        if ctx.needs_input_grad[1]:
-            dres = dy.to(ctx.dtypes[1])
+        p, seed, stream, x_dtype, res_dtype = ctx.args
+        (seed_t,) = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = _run(dy, None, p, seed, seed_t, stream, x_dtype) if need[0] else None
+        dres = dy.to(res_dtype) if need[1] else None
         return dx, dres, None, None, None, None, None
 
 
@@ -112,19 +109,20 @@ def hip_dropout(x, p, seed, residual=None, stream=0):
         raise RuntimeError("redpanda_amd dropout: inputs must be ROCm device tensors")
     if x.dim() == 0:
         raise ValueError("dropout: x must have at least one dimension")
-    dtype_code(x.dtype, "dropout")
     out_dtype = x.dtype
+    dtype_code(out_dtype, "dropout")
+    grad = x.requires_grad
     if residual is not None:
         if residual.shape != x.shape or residual.device != x.device:
             raise ValueError(f"dropout: residual {tuple(residual.shape)} on {residual.device} must be "
                              f"{tuple(x.shape)} on {x.device}")
         dtype_code(residual.dtype, "dropout")
-        out_dtype = torch.promote_types(x.dtype, residual.dtype)
+        out_dtype = torch.promote_types(out_dtype, residual.dtype)
+        grad = grad or residual.requires_grad
     p = check_p(p, "dropout")
     if not 0 <= stream < 1 << 32:
         raise ValueError(f"dropout: stream must be in [0, 2^32), got {stream}")
     seed, seed_t = seed_arg(seed, x.device, "dropout")
-    if torch.is_grad_enabled() and (x.requires_grad or
-                                    (residual is not None and residual.requires_grad)):
+    if grad and torch.is_grad_enabled():
         return _HipDropout.apply(x, residual, p, seed, seed_t, stream, out_dtype)
     return _run(x, residual, p, seed, seed_t, stream, out_dtype)

@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from redpanda_amd import _lib
-from redpanda_amd.dropout import check_p, dtype_code, row_stride, rows_of, seed_arg
+from redpanda_amd.dropout import check_p, dtype_code, empty_rows, rows_of, seed_arg
 
 
 def _f32c(t):
@@ -22,34 +22,32 @@ def _f32c(t):
     return t.detach().to(torch.float32).contiguous()
 
 
-def _args(xr, w, b, eps, gelu, p, seed, seed_t, stream, out_code, out, stats):
-    return _lib.LayerNormArgs(xr.shape[0], xr.shape[1], _lib.DTYPE_CODES[xr.dtype], out_code, gelu,
-                              stream, p, seed, _lib.ptr(seed_t), xr.data_ptr(), row_stride(xr),
-                              _lib.ptr(w), _lib.ptr(b), _lib.ptr(out), _lib.ptr(stats), eps, 0)
-
-
 def _forward(x, w, b, eps, gelu, p, seed, seed_t, stream, out_dtype, keep):
-    """(out, x as rows, w in fp32, the rows' stats or None)."""
+    """(out, w in fp32, the rows' stats or None, the arguments)."""
     lib = _lib.load()
-    xr = rows_of(x, x.shape[-1])
-    wc = _f32c(w)
-    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    stats = torch.empty((xr.shape[0], 2), dtype=torch.float32, device=x.device) if keep else None
-    a = _args(xr, wc, _f32c(b), eps, gelu, p, seed, seed_t, stream, _lib.DTYPE_CODES[out_dtype],
-              out, stats)
-    _lib.check(lib.rp_layernorm_fwd(ctypes.byref(a), _lib.stream_of(x.device)), lib)
-    return out, xr, wc, stats
+    d = x.shape[-1]
+    xr, rows, sr = rows_of(x, d)
+    w, b = _f32c(w), _f32c(b)
+    out = empty_rows(x, out_dtype)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=out.device) if keep else None
+    a = _lib.LayerNormArgs(rows, d, _lib.DTYPE_CODES[x.dtype], _lib.DTYPE_CODES[out_dtype], gelu,
+                           stream, p, seed, None if seed_t is None else seed_t.data_ptr(),
+                           xr.data_ptr(), sr, None if w is None else w.data_ptr(),
+                           None if b is None else b.data_ptr(), out.data_ptr(),
+                           None if stats is None else stats.data_ptr(), eps, 0)
+    _lib.check(lib.rp_layernorm_fwd(ctypes.byref(a), _lib.stream_of(out.device)), lib)
+    return out, w, stats, a
 
 
 class _HipLayerNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, eps, gelu, p, seed, seed_t, stream, out_dtype):
-        out, xr, wc, stats = _forward(x, w, b, eps, gelu, p, seed, seed_t, stream, out_dtype, True)
+        out, wc, stats, a = _forward(x, w, b, eps, gelu, p, seed, seed_t, stream, out_dtype, True)
         ctx.save_for_backward(x, wc, stats, seed_t)
-        ctx.args = (eps, gelu, p, seed, stream)
-        ctx.out_dtype = out_dtype
-        ctx.wdtypes = (None if w is None else w.dtype, None if b is None else b.dtype)
+        # the forward's settings; its pointers are set anew from the saved tensors
+        ctx.args = a
+        ctx.dtypes = (None if w is None else w.dtype, None if b is None else b.dtype)
         return out
 
     @staticmethod
@@ -57,27 +55,30 @@ class _HipLayerNorm(torch.autograd.Function):
     def backward(ctx, dout):
         lib = _lib.load()
         x, w, stats, seed_t = ctx.saved_tensors
-        eps, gelu, p, seed, stream = ctx.args
-        d = x.shape[-1]
-        xr, dr = rows_of(x, d), rows_of(dout, d)
+        a = _lib.LayerNormArgs.from_buffer_copy(ctx.args)
+        d = a.d
+        xr, _, a.x_sr = rows_of(x, d)
+        a.x, a.out, a.stats = xr.data_ptr(), None, stats.data_ptr()
+        a.w = None if w is None else w.data_ptr()
+        a.seed_ptr = None if seed_t is None else seed_t.data_ptr()
+        dr, _, dsr = rows_of(dout, d)
+        g = _lib.LayerNormGrad(dr.data_ptr(), dsr)
         need = ctx.needs_input_grad
-        a = _args(xr, w, None, eps, gelu, p, seed, seed_t, stream, _lib.DTYPE_CODES[ctx.out_dtype],
-                  None, stats)
-        g = _lib.LayerNormGrad(dr.data_ptr(), row_stride(dr))
-        dx = dwb = None
+        dx = dw = db = None
         if need[0]:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            dx = empty_rows(x, x.dtype)
             g.dx = dx.data_ptr()
         if need[1] or need[2]:
-            dwb = torch.empty((2, d), dtype=torch.float32, device=x.device)
-            g.dw, g.db = dwb.data_ptr(), dwb.data_ptr() + 4 * d
-            g.work_bytes = lib.rp_layernorm_work_bytes(ctypes.byref(a))
-            work = torch.empty(max(g.work_bytes, 256), dtype=torch.uint8, device=x.device)
-            g.work = work.data_ptr()
-        _lib.check(lib.rp_layernorm_bwd(ctypes.byref(a), ctypes.byref(g), _lib.stream_of(x.device)),
+            dw = torch.empty(d, dtype=torch.float32, device=stats.device)
+            db = torch.empty_like(dw)
+            nbytes = lib.rp_layernorm_work_bytes(ctypes.byref(a))
+            work = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=stats.device)
+            g.dw, g.db, g.work, g.work_bytes = dw.data_ptr(), db.data_ptr(), work.data_ptr(), nbytes
+        _lib.check(lib.rp_layernorm_bwd(ctypes.byref(a), ctypes.byref(g), _lib.stream_of(stats.device)),
                    lib)
-        dw = dwb[0].to(ctx.wdtypes[0]) if need[1] else None
-        db = dwb[1].to(ctx.wdtypes[1]) if need[2] else None
+        wt, bt = ctx.dtypes
+        dw = None if not need[1] else dw if wt is torch.float32 else dw.to(wt)
+        db = None if not need[2] else db if bt is torch.float32 else db.to(bt)
         return dx, dw, db, None, None, None, None, None, None, None
 
 
@@ -101,14 +102,13 @@ def hip_layernorm(x, weight=None, bias=None, eps=1e-5, gelu=False, p=0.0, seed=N
     else:
         dtype_code(out_dtype, "layernorm")
     grad = x.requires_grad
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            continue
-        if t.shape != x.shape[-1:] or t.device != x.device:
-            raise ValueError(f"layernorm: {name} {tuple(t.shape)} on {t.device} must be "
-                             f"({x.shape[-1]},) on {x.device}")
-        dtype_code(t.dtype, "layernorm")
-        grad = grad or t.requires_grad
+    for t in (weight, bias):
+        if t is not None:
+            if t.dim() != 1 or t.shape[0] != x.shape[-1] or t.device != x.device:
+                raise ValueError(f"layernorm: {'weight' if t is weight else 'bias'} {tuple(t.shape)} "
+                                 f"on {t.device} must be ({x.shape[-1]},) on {x.device}")
+            dtype_code(t.dtype, "layernorm")
+            grad = grad or t.requires_grad
     p = check_p(p, "layernorm")
     if not 0 <= stream < 1 << 32:
         raise ValueError(f"layernorm: stream must be in [0, 2^32), got {stream}")

@@ -13,7 +13,7 @@ import math
 import torch
 
 from redpanda_amd import _lib
-from redpanda_amd.dropout import dtype_code, row_stride
+from redpanda_amd.dropout import dtype_code
 
 
 def _setting(v, R, dtype, device, name):
@@ -28,6 +28,15 @@ def _setting(v, R, dtype, device, name):
     if v.dtype is not dtype or not v.is_contiguous():
         v = v.to(dtype).contiguous()
     return 0, v
+
+
+def _rows(t, n):
+    """(t or a contiguous copy with unit inner stride, its row stride)."""
+    if t.is_contiguous():
+        return t, n
+    if t.stride(1) == 1 and t.stride(0) >= n:
+        return t, t.stride(0)
+    return t.contiguous(), n
 
 
 def hip_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=None,
@@ -56,8 +65,7 @@ def hip_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
         raise ValueError("sample: the vocabulary is empty")
     if u.shape != (R,) or u.device != dev:
         raise ValueError(f"sample: u {tuple(u.shape)} on {u.device} must be ({R},) on {dev}")
-    if logits.stride(1) != 1 or logits.stride(0) < V:
-        logits = logits.contiguous()
+    logits, lsr = _rows(logits, V)
     if u.dtype is not torch.float32 or not u.is_contiguous():
         u = u.to(torch.float32).contiguous()
     T, T_row = _setting(temperature, R, torch.float32, dev, "temperature")
@@ -70,7 +78,7 @@ def hip_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
         raise ValueError(f"sample: top_p must be >= 0 and min_p in [0, 1], got {tp} and {mp}")
     ids = torch.empty(R, dtype=torch.int64, device=dev)
     logp = torch.empty(R, dtype=torch.float32, device=dev) if logprob else None
-    a = _lib.SampleArgs(R, V, 0, code, 0, logits.data_ptr(), row_stride(logits), u.data_ptr(), None, 0,
+    a = _lib.SampleArgs(R, V, 0, code, 0, logits.data_ptr(), lsr, u.data_ptr(), None, 0,
                         T, tp, mp, min(max(int(k), 0), 1 << 31), _lib.ptr(T_row), _lib.ptr(tp_row),
                         _lib.ptr(mp_row), _lib.ptr(k_row), ids.data_ptr(), _lib.ptr(logp))
     if tokens is not None:
@@ -84,9 +92,9 @@ def hip_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
             tokens = tokens.clamp(-1, 2**31 - 1).to(torch.int32)
         if tokens.shape[1] == 0:
             tokens = tokens.new_full((R, 1), -1)  # (a list without storage would read as none)
-        elif tokens.stride(1) != 1 or tokens.stride(0) < tokens.shape[1]:
-            tokens = tokens.contiguous()
-        a.M, a.tokens, a.tokens_sr = tokens.shape[1], tokens.data_ptr(), row_stride(tokens)
+        M = tokens.shape[1]
+        tokens, a.tokens_sr = _rows(tokens, M)
+        a.M, a.tokens = M, tokens.data_ptr()
     lib = _lib.load()
     _lib.check(lib.rp_sample(ctypes.byref(a), _lib.stream_of(dev)), lib)
     return (ids, logp) if logprob else ids

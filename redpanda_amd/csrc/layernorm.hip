@@ -234,7 +234,7 @@ unsigned walk_grid(int64_t rows, int G, int most) {
 
 int layernorm_parts(int64_t rows, int64_t d) {
   const int G = norm_group(d);
-  if (G != 0) return (int)walk_grid(rows, G, kNormBwdWorkgroups);
+  if (G != 0) return (int)walk_grid(rows, G, norm_workgroups(d, true));
   const int64_t tiles = (d + 8 * kWave - 1) / (8 * kWave);
   const int64_t n = (rows + 4 * kWaves - 1) / (4 * kWaves);
   const int64_t most = (2048 + tiles - 1) / tiles;
@@ -245,7 +245,7 @@ hipError_t launch_layernorm_fwd(const LayerNormParams& p, hipStream_t st) {
   if (p.rows == 0) return hipSuccess;
   const int G = norm_group(p.d);
   if (G != 0) {
-    const unsigned wg = walk_grid(p.rows, G, kNormFwdWorkgroups);
+    const unsigned wg = walk_grid(p.rows, G, norm_workgroups(p.d, false));
     return p.es_x == 4 ? launch_norm_fwd4(p, wg, st) : launch_norm_fwd2(p, wg, st);
   }
   hipLaunchKernelGGL(layernorm_fwd_kernel, dim3(row_grid(p.rows)), dim3(kThreads), 0, st, p);

@@ -223,8 +223,11 @@ __global__ __launch_bounds__(norm_threads(G)) void layernorm_bwd_rows_kernel(Lay
   const DropState drop(p.drop);
   const float scale = p.drop.t != 0 ? p.drop.scale : 1.f;
   const float invd = 1.f / (float)cols.d;
+  // 1024 threads have 128 registers each: there the weights are read for each
+  // row, and no row ahead
+  constexpr bool kAhead = G < 1024;
   float w[NB][8], dw[NB][8] = {}, db[NB][8] = {};
-  cols.load_weight(p.w, 1.f, scale, w);
+  if constexpr (kAhead) cols.load_weight(p.w, 1.f, 1.f, w);
   const char* x = static_cast<const char*>(p.x);
   const char* go = static_cast<const char*>(g.dout);
   Raw8<ES> rx[NB];
@@ -236,16 +239,17 @@ __global__ __launch_bounds__(norm_threads(G)) void layernorm_bwd_rows_kernel(Lay
     mu = p.stats[2 * row];
     r = p.stats[2 * row + 1];
   };
-  if (at.row < p.rows) load(at.row);
+  if (kAhead && at.row < p.rows) load(at.row);
   for (int it = 0; at.row < p.rows; at.row += at.step, it ^= 1) {
+    if constexpr (!kAhead) load(at.row);
     float xh[NB][8], q[NB][8], slope[NB][8];
-    const float r0 = r, shift = -mu * r;
+    const float r0 = r, shift = -mu * r, rs = r * scale;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       to_floats(rx[j], p.dt_x, xh[j]);
       to_floats(rg[j], p.dt_out, q[j]);
     }
-    if (at.row + at.step < p.rows) load(at.row + at.step);
+    if (kAhead && at.row + at.step < p.rows) load(at.row + at.step);
     if (p.drop.t != 0) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) drop.apply((uint32_t)(at.g + G * j), (uint64_t)at.row, q[j]);
@@ -258,14 +262,20 @@ __global__ __launch_bounds__(norm_threads(G)) void layernorm_bwd_rows_kernel(Lay
           const float v = xh[j][i];
           const Gelu ge = gelu_parts(v);
           xh[j][i] = gelu_of(v, ge);
-          slope[j][i] = r0 * gelu_slope(v, ge);
+          slope[j][i] = rs * gelu_slope(v, ge);
         }
     } else {
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) slope[j][i] = r0;
+        for (int i = 0; i < 8; ++i) slope[j][i] = rs;
     }
+    if constexpr (!kAhead) {
+      const float* pw = p.w;
+      asm volatile("" : "+s"(pw));
+      cols.load_weight(pw, 1.f, 1.f, w);
+    }
+    // (the dropout's scale is in rs, and at the end in dw and db)
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < NB; ++j)
@@ -341,7 +351,7 @@ __global__ __launch_bounds__(norm_threads(G)) void layernorm_bwd_rows_kernel(Lay
 
 // The shapes (G, NB), by the blocks they hold.
 #define RP_FOR_EACH_NORM_SHAPE(X) \
-  X(8, 1) X(16, 1) X(8, 3) X(32, 1) X(16, 3) X(64, 1) X(32, 3) X(64, 2) X(64, 3) X(64, 4) \
+  X(8, 1) X(16, 1) X(8, 3) X(32, 1) X(16, 3) X(64, 1) X(32, 3) X(64, 2) X(64, 3) X(256, 1) \
   X(256, 2) X(512, 2) X(1024, 2)
 
 // Lanes a row of d columns is taken by, and its groups in a workgroup; 0 for
@@ -352,6 +362,18 @@ inline int norm_group(int64_t d) {
   RP_FOR_EACH_NORM_SHAPE(RP_CASE)
 #undef RP_CASE
   return 0;
+}
+
+// Workgroups that a launch of G lanes a row fills the card with: as many as its
+// registers let be resident, since a second round of a part of them would cost
+// as much as a whole one (131072 x 1024 backward: 1024 workgroups where 768 fit
+// took a quarter longer).
+inline int norm_workgroups(int64_t d, bool backward) {
+  const int G = norm_group(d);
+  if (G > 256) return backward || G == 1024 ? 256 : 512;
+  const int nb = (int)((d + 8 * G - 1) / (8 * G));
+  const int a_cu = backward ? (nb == 1 ? 4 : nb == 2 ? 3 : 2) : (nb == 1 ? 7 : nb == 2 ? 5 : 3);
+  return 256 * a_cu;
 }
 
 template <int ES>

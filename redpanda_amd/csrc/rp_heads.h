@@ -55,10 +55,6 @@ struct LayerNormGrad {
   float* part;       // (layernorm_parts, 2, d) workspace
 };
 
-// Most workgroups of a launch whose groups of lanes walk rows.
-constexpr int kNormFwdWorkgroups = 2048;
-constexpr int kNormBwdWorkgroups = 1024;
-
 // Partial sums of the weights' gradients that a backward writes.
 int layernorm_parts(int64_t rows, int64_t d);
 hipError_t launch_layernorm_fwd(const LayerNormParams& p, hipStream_t st);

@@ -23,6 +23,11 @@ struct DropWords {
   uint32_t w[4];
 };
 
+// One instruction; the compiler makes two of it.
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
+
 __device__ __forceinline__ DropWords drop_words(uint32_t block, uint64_t row, uint32_t stream,
                                                 uint64_t seed) {
   uint32_t c0 = block, c1 = (uint32_t)row, c2 = stream, c3 = (uint32_t)(row >> 32);
@@ -30,9 +35,9 @@ __device__ __forceinline__ DropWords drop_words(uint32_t block, uint64_t row, ui
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c0 = xor3((uint32_t)(b >> 32), c1, k0);
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = xor3((uint32_t)(a >> 32), c3, k1);
     c3 = (uint32_t)a;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;

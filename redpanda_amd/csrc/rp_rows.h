@@ -137,7 +137,7 @@ __device__ __forceinline__ void store8(void* row, int64_t col, int64_t d, int dt
 // erfc of full relative accuracy would cost about twice the instructions, for
 // the far tail's own digits, which no sum over the row keeps.
 struct Gelu {
-  float tail;  // Phi(-|x|)
+  float half;  // Phi(|x|) - 1/2
   float e;     // exp(-x^2 / 2)
 };
 __device__ __forceinline__ Gelu gelu_parts(float x) {
@@ -151,17 +151,17 @@ __device__ __forceinline__ Gelu gelu_parts(float x) {
   q = ffma(q, t, -0.4882596902776471f);
   q = ffma(q, t, 0.25405431713520465f);
   q = ffma(q, t, -0.017066889858532747f);
-  return {e * q, e};
+  return {ffma(-e, q, 0.5f), e};
 }
-// x Phi(x) = max(x, 0) - |x| Phi(-|x|) (NaN for an infinite x, which leaves a
+// x Phi(x) = x / 2 + |x| (Phi(|x|) - 1/2) (NaN for an infinite x, which leaves a
 // row without a mean either way)
 __device__ __forceinline__ float gelu_of(float x, const Gelu& g) {
-  return ffma(-fabsf(x), g.tail, fmaxf(x, 0.f));
+  return ffma(fabsf(x), g.half, 0.5f * x);
 }
 // GELU'(x) = Phi(x) + x phi(x)
 __device__ __forceinline__ float gelu_slope(float x, const Gelu& g) {
   const float phi = g.e * 0.3989422804014327f;
-  return ffma(x, phi, 0.5f + copysignf(0.5f - g.tail, x));
+  return ffma(x, phi, 0.5f + copysignf(g.half, x));
 }
 
 }  // namespace rp

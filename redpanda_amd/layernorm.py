@@ -10,10 +10,9 @@ standard deviation are kept.
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from redpanda_amd import _lib
-from redpanda_amd.dropout import check_p, dtype_code, empty_rows, rows_of, seed_arg
+from redpanda_amd.dropout import check_p, dtype_code, empty_rows, once, rows_of, seed_arg
 
 
 def _f32c(t):
@@ -51,7 +50,7 @@ class _HipLayerNorm(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dout):
         lib = _lib.load()
         x, w, stats, seed_t = ctx.saved_tensors

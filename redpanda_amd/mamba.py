@@ -35,6 +35,7 @@ import torch.utils.checkpoint
 
 from redpanda_amd import layer_step
 from redpanda_amd.bcnorm import hip_bcnorm_psum
+from redpanda_amd.dropout import hip_dropout
 from redpanda_amd.mixer import hip_mixer_out
 from redpanda_amd.norm import hip_add_rmsnorm
 from redpanda_amd.scan import hip_scan_with_state, hip_trapezoidal_scan
@@ -373,12 +374,22 @@ class Mamba(nn.Module):
         elif isinstance(module, nn.Embedding):
             nn.init.normal_(module.weight, mean=0.0, std=0.02)
 
-    def forward(self, input_ids, input_embeds=None):
-        """(B, L) ids or (B, L, d_model) embeddings -> (B, L, d_model)."""
+    def forward(self, input_ids, input_embeds=None, dropout=0.0, seed=None):
+        """(B, L) ids or (B, L, d_model) embeddings -> (B, L, d_model).
+        dropout > 0: each layer's branch is dropped out with the residual added
+        in the same pass (hip_dropout with `seed`, the layer's index as its
+        stream), for training; 0 adds the branch as it is."""
         x = input_embeds if input_embeds is not None else self.embedding(input_ids)
-        for layer in self.layers:
+        for i, layer in enumerate(self.layers):
             mixer, norm = layer["mixer"], layer["norm"]
-            if self.grad_checkpoint and self.training and x.requires_grad:
+            if dropout:
+                if self.grad_checkpoint and self.training and x.requires_grad:
+                    out = torch.utils.checkpoint.checkpoint(
+                        lambda inp, m=mixer, nm=norm: m(nm(inp)), x, use_reentrant=False)
+                else:
+                    out = mixer(norm(x))
+                x = hip_dropout(out, dropout, seed, residual=x, stream=i)
+            elif self.grad_checkpoint and self.training and x.requires_grad:
                 # the scan is stateless and deterministic, so recomputation in
                 # backward reproduces the forward exactly
                 x = x + torch.utils.checkpoint.checkpoint(

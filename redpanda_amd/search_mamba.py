@@ -6,7 +6,10 @@ redpanda_amd.mamba: prime_board (one causal scan returning the cache, on the
 HIP scan kernel), _expand_cache, eval_step / backbone.step (the fused step
 kernel), dynamics_rollout (trains through step via the scan kernel's analytic
 backward), and the line-evaluation helpers.  The heads are plain torch
-modules with the reference's names and init.
+modules with the reference's names and init; the paths that the reference does
+not have (dropout in dynamics_rollout, sample_moves, sample_rollout) run their
+middle, GELU and layer norm, in one kernel, with dropout and sampling from
+given random numbers on the device.
 """
 
 import json
@@ -16,7 +19,9 @@ from dataclasses import fields as dc_fields
 import torch
 import torch.nn as nn
 
+from redpanda_amd.layernorm import hip_layernorm
 from redpanda_amd.mamba import Mamba, MambaConfig
+from redpanda_amd.sampling import hip_sample
 
 
 class SearchMambaConfig(MambaConfig):
@@ -146,18 +151,78 @@ class SearchMamba(nn.Module):
         quality = self.line_value_head(hidden).squeeze(-1)
         return quality.item(), self.continuation_head(hidden).squeeze(0)
 
-    def dynamics_rollout(self, board_encoding, move_tokens):
+    @staticmethod
+    def _fused_head(head, h, dropout=0.0, seed=None, stream=0):
+        """A head's Linear -> GELU -> LayerNorm [-> dropout] -> rest, GELU, norm
+        and dropout in one pass; the norm's result in the first Linear's dtype
+        (fp32, or the autocast dtype that the next Linear takes)."""
+        x, norm = head[0](h), head[2]
+        x = hip_layernorm(x, norm.weight, norm.bias, norm.eps, gelu=True, p=dropout, seed=seed,
+                          stream=stream)
+        for m in head[3:]:
+            x = m(x)
+        return x
+
+    def dynamics_rollout(self, board_encoding, move_tokens, dropout=0.0, seed=None):
         """Differentiable: prime on (B, L_board), step through (B, T) moves;
         returns per-step values (B, T), continuation logits (B, T, vocab) and
-        consistency features (B, T, eval_dim) (engine/search_mamba.py:252-273)."""
+        consistency features (B, T, eval_dim) (engine/search_mamba.py:252-273).
+
+        dropout > 0 (training): the value and the continuation head drop out
+        behind their norms, with masks of `seed` (an int, or an int64 tensor of
+        one element on the device, which a captured step reads on each replay)
+        that no pass stores; step t draws streams 2 t and 2 t + 1."""
         _, cache = self.backbone.prime_cache(board_encoding)
         vs, cs, fs = [], [], []
         for t in range(move_tokens.shape[1]):
             h, cache = self.backbone.step(token_id=move_tokens[:, t], cache=cache)
-            vs.append(torch.tanh(self.value_head(h)).squeeze(-1))
-            cs.append(self.continuation_head(h))
+            if dropout:
+                v = self._fused_head(self.value_head, h, dropout, seed, 2 * t)
+                c = self._fused_head(self.continuation_head, h, dropout, seed, 2 * t + 1)
+            else:
+                v, c = self.value_head(h), self.continuation_head(h)
+            vs.append(torch.tanh(v).squeeze(-1))
+            cs.append(c)
             fs.append(self.consistency_proj(h))
         return torch.stack(vs, 1), torch.stack(cs, 1), torch.stack(fs, 1)
+
+    @torch.no_grad()
+    def sample_moves(self, hidden, u, legal=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """The next move of every rollout, drawn from the continuation head:
+        (token ids (R,) int64, their log-probabilities (R,)).  hidden (R,
+        d_model); u (R,) uniform numbers; legal: None or (R, M) ids padded with
+        -1, the moves to draw among (their logits alone are read); the settings
+        as in hip_sample.  -1 for a rollout without a move.  The reference draws
+        on the host from the top candidates (engine/mars_search.py:261-276)."""
+        logits = self._fused_head(self.continuation_head, hidden)
+        return hip_sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                          tokens=legal, logprob=True)
+
+    @torch.no_grad()
+    def sample_rollout(self, board_encoding, u, legal=None, compact=True, **settings):
+        """K rollouts of T plies from one board, on the device from end to end:
+        u (T, K) uniform numbers -> tokens (T, K) int64, log-probabilities
+        (T, K), values (T, K) of the states the moves lead to.  legal: None, or a
+        function of (ply, the tokens before it or None) that gives the ply's (K,
+        M) legal ids padded with -1.  A rollout without a move ends: its tokens
+        are -1 from there on, its value stays.  settings: hip_sample's."""
+        T, k = u.shape
+        hidden, cache = self.prime_board(board_encoding.to(self._device()), compact=compact)
+        hidden, cache = hidden.expand(k, -1).contiguous(), self._expand_cache(cache, k)
+        tokens, logps, values, alive, value = [], [], [], None, None
+        for t in range(T):
+            moves = None if legal is None else legal(t, tokens[-1] if tokens else None)
+            ids, logp = self.sample_moves(hidden, u[t], moves, **settings)
+            alive = ids >= 0 if alive is None else alive & (ids >= 0)
+            ids = torch.where(alive, ids, -1)
+            # an ended rollout steps on with token 0, unseen
+            hidden, cache = self.backbone.step(token_id=ids.clamp(min=0), cache=cache)
+            v = torch.tanh(self._fused_head(self.value_head, hidden)).squeeze(-1)
+            value = torch.where(alive, v, torch.zeros_like(v) if value is None else value)
+            tokens.append(ids)
+            logps.append(torch.where(alive, logp, float("-inf")))
+            values.append(value)
+        return torch.stack(tokens), torch.stack(logps), torch.stack(values)
 
     @torch.no_grad()
     def eval_step(self, cache, move_token):

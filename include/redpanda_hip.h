@@ -474,6 +474,8 @@ int rp_layernorm_bwd(const rp_layernorm_args* a, const rp_layernorm_grad* g, voi
  * ids: (R,) int64, -1 for a row without candidates; logp: NULL or (R,) fp32, the
  * logarithm of the token's share of the kept weights (-inf without candidates).
  * Weights are summed as 64-bit integers, so results do not depend on order.
+ * work: NULL, or rp_sample_work_bytes() of scratch, 256-byte aligned: few long
+ * rows are then shared by several workgroups each (the same results, sooner).
  */
 typedef struct rp_sample_args {
   int64_t R, V, M;
@@ -489,10 +491,15 @@ typedef struct rp_sample_args {
   const int32_t* top_k_row;
   int64_t* ids;
   float* logp;
+  void* work;
+  int64_t work_bytes;
 } rp_sample_args;
 
 /* Validate rp_sample arguments on the host without launching anything. */
 int rp_sample_check(const rp_sample_args* a);
+
+/* Bytes of scratch that rp_sample makes use of (0: none). */
+int64_t rp_sample_work_bytes(const rp_sample_args* a);
 int rp_sample(const rp_sample_args* a, void* stream);
 
 /* ABI version this library was built with (RP_ABI_VERSION). */

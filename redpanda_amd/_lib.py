@@ -167,7 +167,7 @@ class SampleArgs(ctypes.Structure):
         ("logits", _vp), ("logits_sr", _i64), ("u", _vp), ("tokens", _vp), ("tokens_sr", _i64),
         ("temperature", _f64), ("top_p", _f64), ("min_p", _f64), ("top_k", _i64),
         ("temperature_row", _vp), ("top_p_row", _vp), ("min_p_row", _vp), ("top_k_row", _vp),
-        ("ids", _vp), ("logp", _vp),
+        ("ids", _vp), ("logp", _vp), ("work", _vp), ("work_bytes", _i64),
     ]
 
 
@@ -207,6 +207,7 @@ SIGNATURES = {
     "rp_layernorm_bwd": (ctypes.c_int, [ctypes.POINTER(LayerNormArgs),
                                         ctypes.POINTER(LayerNormGrad), _vp]),
     "rp_sample_check": (ctypes.c_int, [ctypes.POINTER(SampleArgs)]),
+    "rp_sample_work_bytes": (_i64, [ctypes.POINTER(SampleArgs)]),
     "rp_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), _vp]),
     "rp_mixer_out_check": (ctypes.c_int, [ctypes.POINTER(MixerOutArgs)]),
     "rp_mixer_out_work_bytes": (_i64, [ctypes.POINTER(MixerOutArgs)]),

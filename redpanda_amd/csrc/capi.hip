@@ -1468,9 +1468,19 @@ int rp_sample_check(const rp_sample_args* a) {
   return RP_OK;
 }
 
+int64_t rp_sample_work_bytes(const rp_sample_args* a) {
+  if (rp_sample_check(a) != RP_OK) return -1;
+  if (!rp::sample_is_wide(a->R, a->tokens ? a->M : a->V, a->tokens != nullptr)) return 0;
+  return round_up(rp::sample_wide_bytes(a->R), 256);
+}
+
 int rp_sample(const rp_sample_args* a, void* stream) {
   int st = rp_sample_check(a);
   if (st != RP_OK || a->R == 0) return st;
+  const int64_t need = rp_sample_work_bytes(a);
+  if (a->work != nullptr && need > 0 && (a->work_bytes < need || !aligned(a->work, 256)))
+    return fail(RP_ERR_WORKSPACE, "sample: workspace needs %lld bytes (256-aligned), got %lld",
+                (long long)need, (long long)a->work_bytes);
   rp::SampleParams p{};
   p.R = a->R;
   p.V = (int)a->V;
@@ -1495,7 +1505,9 @@ int rp_sample(const rp_sample_args* a, void* stream) {
   p.k_row = a->top_k_row;
   p.ids = a->ids;
   p.logp = a->logp;
-  hipError_t e = rp::launch_sample(p, (hipStream_t)stream);
+  p.work = a->work;
+  hipError_t e = need > 0 && a->work != nullptr ? rp::launch_sample_wide(p, (hipStream_t)stream)
+                                                : rp::launch_sample(p, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "sample launch");
   return RP_OK;
 }

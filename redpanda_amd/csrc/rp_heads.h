@@ -80,8 +80,16 @@ struct SampleParams {
   const int32_t* k_row;
   int64_t* ids;  // (R,)
   float* logp;   // (R,) or null
+  void* work;    // sample_wide_bytes, or null
 };
 
 hipError_t launch_sample(const SampleParams& p, hipStream_t st);
+
+// Few long rows, which several workgroups share (sample_wide.hip): whether a call
+// is of that kind, its workspace, and its launches.
+constexpr int kSampleWideRows = 128;
+bool sample_is_wide(int64_t R, int64_t n, bool lists);
+int64_t sample_wide_bytes(int64_t R);
+hipError_t launch_sample_wide(const SampleParams& p, hipStream_t st);
 
 }  // namespace rp

@@ -16,6 +16,9 @@ from redpanda_amd import _lib
 from redpanda_amd.dropout import dtype_code
 
 
+_WIDE = 8192  # (no row up to it takes a workspace)
+
+
 def _setting(v, R, dtype, device, name):
     """(value, None) of a number, (0, (R,) tensor) of a setting per row."""
     if not isinstance(v, torch.Tensor):
@@ -96,5 +99,10 @@ def hip_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
         tokens, a.tokens_sr = _rows(tokens, M)
         a.M, a.tokens = M, tokens.data_ptr()
     lib = _lib.load()
+    if V > _WIDE and tokens is None:
+        a.work_bytes = lib.rp_sample_work_bytes(ctypes.byref(a))
+        if a.work_bytes > 0:
+            work = torch.empty(a.work_bytes, dtype=torch.uint8, device=dev)
+            a.work = work.data_ptr()
     _lib.check(lib.rp_sample(ctypes.byref(a), _lib.stream_of(dev)), lib)
     return (ids, logp) if logprob else ids

@@ -246,3 +246,59 @@ def test_refusals(gpu_lib):
     assert hip_sample(lg[:0], u[:0]).shape == (0,)
     assert np.array_equal(hip_sample(lg[:1], u[:1]).cpu().numpy(),
                           hip_sample(lg, u)[:1].cpu().numpy())
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V", [(1, 16385), (2, 20000), (5, 32769), (3, 70001), (2, 131073)])
+def test_rows_that_workgroups_share(gpu_lib, R, V, t):
+    """Few long rows: each plan, masked and equal values, and what the shared looks
+    do not hold."""
+    lg, u = make(R, V, t, V)
+    lg[0, V // 3:] = -float("inf")  # whole stretches without a candidate
+    for s in SETTINGS + [dict(k=191), dict(k=192, tp=0.5), dict(k=3000, mp=0.001), dict(tp=0.99, mp=0.01)]:
+        check(lg, u, **s)
+    flat = torch.zeros(R, V, device=dev)
+    flat[0, 7::5] = 0.5
+    for s in (dict(tp=0.3), dict(k=150), dict(), dict(T=0.0), dict(mp=0.9, tp=0.8)):
+        check(flat.to(t), u, **s)
+    odd = lg.clone()
+    odd[0] = -float("inf")
+    odd[-1, V - 1] = float("inf")
+    if R > 2:
+        odd[1] = float("nan")
+    for s in (dict(tp=0.9), dict(k=5), dict(), dict(T=0.0)):
+        check(odd, u, **s)
+
+
+def test_shared_rows_with_settings_of_their_own(gpu_lib):
+    R, V = 60, 30011
+    lg, u = make(R, V, seed=5)
+    g = torch.Generator(device=dev).manual_seed(2)
+
+    def r():
+        return torch.rand(R, generator=g, device=dev)
+
+    T = torch.where(r() < 0.2, torch.zeros(R, device=dev), 0.3 + r())
+    k = (r() * 300).to(torch.int32) * (r() < 0.6)
+    tp = torch.where(r() < 0.3, torch.ones(R, device=dev), r())
+    mp = torch.where(r() < 0.5, torch.zeros(R, device=dev), 0.1 * r())
+    check(lg, u, T=T, k=k.to(torch.int32), tp=tp, mp=mp)
+    for _ in range(3):  # the same bits each time
+        a = hip_sample(lg, u, temperature=T, top_p=tp, logprob=True)
+        b = hip_sample(lg, u, temperature=T, top_p=tp, logprob=True)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_shared_rows_in_a_graph(gpu_lib):
+    lg, u = make(9, 20001, torch.bfloat16, 2)
+    hip_sample(lg, u, top_p=0.9, logprob=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = hip_sample(lg, u, top_p=0.9, logprob=True)
+    for i in range(4):
+        u.copy_(torch.rand(9, generator=torch.Generator(device=dev).manual_seed(i), device=dev))
+        graph.replay()
+        a = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        b = hip_sample(lg, u, top_p=0.9, logprob=True)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

@@ -175,3 +175,17 @@ def test_host_tensors_are_refused():
         hip_layernorm(x)
     with pytest.raises(ValueError, match="device tensor"):
         hip_sample(x, torch.zeros(2))
+
+
+def test_sample_workspace(lib):
+    """Few long rows have one, which may be left out; a short or unaligned one is
+    refused."""
+    assert lib.rp_sample_work_bytes(ctypes.byref(_sample())) == 0
+    a = _sample(V=100003, logits_sr=100003, ids=FAKE + 0x1000000, u=FAKE + 0x2000000)
+    need = lib.rp_sample_work_bytes(ctypes.byref(a))
+    assert need > 0 and need % 256 == 0
+    for work, nbytes in ((FAKE * 0x1000, need - 1), (FAKE * 0x1000 + 8, need)):
+        a.work, a.work_bytes = work, nbytes
+        assert lib.rp_sample(ctypes.byref(a), None) < 0
+        assert "workspace" in lib.rp_last_error().decode()
+    assert lib.rp_sample_work_bytes(ctypes.byref(_sample(R=-1))) < 0

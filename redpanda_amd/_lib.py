@@ -277,7 +277,9 @@ def ptr(t):
 
 
 def stream_of(device):
-    """The handle of the device's current stream (the raw handle: making a
-    torch.cuda.Stream object for it takes 2-3 us of a small call's 10)."""
-    return torch._C._cuda_getCurrentRawStream(
-        torch.cuda.current_device() if device.index is None else device.index)
+    """The handle of the device's current stream.  For a tensor's device the raw
+    handle: making a torch.cuda.Stream object for it takes 2-3 us of a small
+    call's 10.  Names and numbers of devices go through torch's own lookup."""
+    if isinstance(device, torch.device) and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream

@@ -141,3 +141,11 @@ def test_under_autocast(gpu_lib):
         ids, logp = m.sample_moves(h, torch.rand(33, device=dev), top_p=0.9)
     assert a.dtype == torch.bfloat16 and nrel(a.float(), b.float()) <= 3e-2
     assert bool((ids >= 0).all()) and bool(torch.isfinite(logp).all())
+
+
+def test_stream_of_every_form_of_a_device(gpu_lib):
+    from redpanda_amd import _lib
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        for d in (torch.device("cuda", 0), torch.device("cuda"), "cuda", "cuda:0", 0, None):
+            assert _lib.stream_of(d) == st.cuda_stream

@@ -57,25 +57,23 @@ void go(const SampleParams& p, hipStream_t st) {
   const dim3 grid((unsigned)x, (unsigned)((p.R + x - 1) / x));
 #define RP_GO(WAVES, NBLK)                                                                       \
   hipLaunchKernelGGL((sample_kernel<WAVES, NBLK, ES>), grid, dim3(WAVES* kWave), 0, st, p)
-  // a wave a row where that fills the card (nuclei of 8192: 1000 rows 54 us by
-  // one wave each, 41 by four; 2000 rows of 1000: 24 and 79); else as many as the
-  // row keeps busy (600 rows of 30000: 67 us by four, 103 by sixteen, of which a CU
-  // holds two workgroups; 200 of 50000: 78 and 52)
-  const bool few = p.R < 512;
+  // A wave a row where that fills the card (nuclei of 8192: 1000 rows 54 us by
+  // one wave each, 41 by four; 2000 rows of 1000: 24 and 79).  Four waves a row
+  // else, in registers up to 8192 elements; sixteen for the rows that are too few
+  // and too long for that (300 rows of 16000: 37 us by four, 54 by sixteen, of
+  // which a CU holds two workgroups; 130 of 131072: 165 and 84).
   const bool wave_list = p.k_row != nullptr || p.k < 192;  // (a list of a wave's LDS)
-  if (p.n <= 512 && !few)
+  if (p.n <= 512 && p.R >= 512)
     RP_GO(1, 1);
   else if (p.R >= (p.n <= 2048 ? 512 : 1280) && wave_list)
     RP_GO(1, 0);
   else if (p.n <= 2048)
     RP_GO(4, 1);
-  else if (p.n <= 8192 && few)
-    RP_GO(16, 1);
   else if (p.n <= 4096)
     RP_GO(4, 2);
   else if (p.n <= 8192)
     RP_GO(4, 4);
-  else if (p.R > 320 && wave_list)
+  else if (p.R > (p.n <= 16384 ? 64 : 320) && wave_list)
     RP_GO(4, 0);
   else
     RP_GO(16, 0);

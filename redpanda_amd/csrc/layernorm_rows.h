@@ -12,6 +12,13 @@
 // present one is worked on; its columns stay, so the weights are read once, the
 // backward keeps the columns' sums in registers over all its rows, and the
 // generator's first products, which depend on the column alone, leave the loop.
+//
+// 131072 x 1024 in bf16: without GELU and dropout 93 us forward (5.8 TB/s) and 152
+// backward (5.3), which HBM bounds; with both 150 and 220, which vector
+// instructions bound (about 31 and 43 an element: GELU 16 forward and 22 backward,
+// the generator 5).  16384 x 768, bf16 in and fp32 out, no GELU: 18 and 22 us.
+// A few rows are a launch's latency: one row of 384 3.8 us, 512 x 768 fp32 with
+// both 5.7 and 8.3, and 3.5 for the partial sums.
 #pragma once
 
 #include "rp_heads.h"

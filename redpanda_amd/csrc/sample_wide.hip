@@ -8,6 +8,11 @@
 // workgroups add to them does not matter.  Rows that this does not hold (a long
 // list, a large top-k, +inf) the last launch does by itself, as sample_kernel
 // does.
+//
+// 64 rows of 100003 fp32 logits: top-50 29 us (31 by a workgroup a row), a nucleus
+// 52 (67), no cut 27 (38); one row of 131072 bf16: top-50 22 (32), a nucleus 35
+// (78).  A launch is 4 us of it whatever it does; the first look reads the 26 MB
+// in 8.
 
 #include "sample_row.h"
 

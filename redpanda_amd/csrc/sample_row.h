@@ -651,14 +651,15 @@ __device__ __forceinline__ bool cut_steps(Scratch<WAVES>& s, int n, double tp, f
 
 // Exact weights of a thread's elements: all of them (*sum), those before the
 // steps (*ahead, and by segment in `seg`, the wave's), and a list of those in
-// them.
-template <int WAVES, class R>
+// them.  kMin: those that min-p leaves, too, by segment in min_seg.
+template <bool kMin, int WAVES, class R>
 __device__ __forceinline__ void exact_weights(Scratch<WAVES>& s, const RowWeights& rw, R& row, float lo,
-                                              float hi, uint64_t* seg, uint64_t* sum, uint64_t* ahead) {
+                                              float hi, uint64_t* seg, uint64_t* sum, uint64_t* ahead,
+                                              double mp, uint64_t* min_seg) {
   __syncthreads();
   if (threadIdx.x == 0) s.count = 0;
   __syncthreads();
-  uint64_t all = 0, before = 0, part = 0;
+  uint64_t all = 0, before = 0, part = 0, min_part = 0;
   const uint64_t base = rw.base();
   row.walk(
       [&](const float (&x)[8], int at) {
@@ -666,12 +667,15 @@ __device__ __forceinline__ void exact_weights(Scratch<WAVES>& s, const RowWeight
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           y[i] = (rw.top - x[i]) * rw.fscale;
-          const uint64_t q = rw.raw(rw.weight(x[i]));
+          const double weight = rw.weight(x[i]);
+          const uint64_t q = rw.raw(weight);
           all += q;
           part += y[i] < lo ? q : base;
+          if constexpr (kMin) min_part += weight >= mp ? q : base;
         }
         all -= 8 * base;
         part -= 8 * base;
+        if constexpr (kMin) min_part -= 8 * base;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (!(y[i] < lo) && y[i] < hi && x[i] > -__builtin_inff()) {
@@ -685,6 +689,11 @@ __device__ __forceinline__ void exact_weights(Scratch<WAVES>& s, const RowWeight
         part = wave_all(part, Add());
         if (threadIdx.x % kWave == 0) seg[g] = part;
         part = 0;
+        if constexpr (kMin) {
+          min_part = wave_all(min_part, Add());
+          if (threadIdx.x % kWave == 0) min_seg[g] = min_part;
+          min_part = 0;
+        }
       });
   *sum = all;
   *ahead = before;
@@ -712,7 +721,8 @@ __device__ __forceinline__ uint64_t nucleus(Scratch<WAVES>& s, const RowWeights&
   uint64_t sum, ahead;
   fine_weights(s, rw, row, grain);
   if (!cut_steps(s, row.n, tp, &lo, &hi)) return 0;
-  exact_weights(s, rw, row, lo, hi, &s.seg[threadIdx.x / kWave * R::kSegs], &sum, &ahead);
+  exact_weights<false>(s, rw, row, lo, hi, &s.seg[threadIdx.x / kWave * R::kSegs], &sum, &ahead, 0.0,
+                       nullptr);
   block_sums(sum, ahead, s);
   __syncthreads();
   return nucleus_cut(s, rw, row, tp, sum, ahead);

@@ -40,6 +40,7 @@ struct WideRow {
   uint32_t groups[kGroups];
   uint32_t fine[kWideFine];
   uint64_t seg[kWideSegs];
+  uint64_t min_seg[kWideSegs];  // of what min-p leaves (a nucleus' rows)
   uint64_t key[kWideList];
 };
 
@@ -177,7 +178,10 @@ __global__ __launch_bounds__(kSliceWaves* kWave) void sample_wide_weights_kernel
     return;
   }
   uint64_t sum, ahead;
-  exact_weights(s, rw, row, lo, hi, seg, &sum, &ahead);
+  if (set.mp > 0.0)
+    exact_weights<true>(s, rw, row, lo, hi, seg, &sum, &ahead, set.mp, &w.min_seg[share * row.kSegs]);
+  else
+    exact_weights<false>(s, rw, row, lo, hi, seg, &sum, &ahead, 0.0, nullptr);
   block_sums(sum, ahead, s);
   if (threadIdx.x == 0) {
     atomicAdd(&w.sum, (unsigned long long)sum);
@@ -228,16 +232,14 @@ __global__ __launch_bounds__(kLastWaves* kWave) void sample_wide_draw_kernel(Sam
     }
     const uint64_t floor = nucleus_cut(s, rw, row, set.tp, w.sum, w.ahead);
     if (floor != 0) {
-      // (min-p keeps all of the nucleus when it keeps the last of it)
+      // (min-p keeps all of the nucleus when it keeps the last of it; else all
+      // that it leaves is in the nucleus)
       if (rw.weight(Floor(floor).value) >= set.mp) {
         draw(s, rw, row, floor, set.mp, set.u, give);
-        return;
+      } else {
+        for (int i = tid; i < kWideSegs; i += kT) s.seg[i] = w.min_seg[i];
+        draw(s, rw, row, 0, set.mp, set.u, give);
       }
-      Row<kLastWaves, 0, ES> own(p, r);
-      __syncthreads();
-      segment_weights(rw, own, floor, set.mp, keep_bound(rw, set.T, set.mp, floor),
-                      &s.seg[tid / kWave * own.kSegs]);
-      draw(s, rw, own, floor, set.mp, set.u, give);
       return;
     }
   }

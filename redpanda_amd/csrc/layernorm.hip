@@ -112,12 +112,7 @@ __device__ __forceinline__ void load_grad(const LayerNormParams& p, const LayerN
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     slope[i] = 1.f;
-    if (p.gelu) {
-      const float x = xh[i];
-      const Gelu ge = gelu_parts(x);
-      xh[i] = gelu_of(x, ge);
-      slope[i] = gelu_slope(x, ge);
-    }
+    if (p.gelu) gelu_both(xh[i], xh[i], slope[i]);
     xh[i] = (xh[i] - mu) * r;
   }
 }

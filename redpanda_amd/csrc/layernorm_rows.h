@@ -266,10 +266,8 @@ __global__ __launch_bounds__(norm_threads(G)) void layernorm_bwd_rows_kernel(Lay
       for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = xh[j][i];
-          const Gelu ge = gelu_parts(v);
-          xh[j][i] = gelu_of(v, ge);
-          slope[j][i] = rs * gelu_slope(v, ge);
+          gelu_both(xh[j][i], xh[j][i], slope[j][i]);
+          slope[j][i] *= rs;
         }
     } else {
 #pragma unroll

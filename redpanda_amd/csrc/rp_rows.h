@@ -158,10 +158,12 @@ __device__ __forceinline__ Gelu gelu_parts(float x) {
 __device__ __forceinline__ float gelu_of(float x, const Gelu& g) {
   return ffma(fabsf(x), g.half, 0.5f * x);
 }
-// GELU'(x) = Phi(x) + x phi(x)
-__device__ __forceinline__ float gelu_slope(float x, const Gelu& g) {
-  const float phi = g.e * 0.3989422804014327f;
-  return ffma(x, phi, 0.5f + copysignf(g.half, x));
+// The same and GELU'(x) = Phi(x) + x phi(x), which share Phi(x).
+__device__ __forceinline__ void gelu_both(const float x, float& value, float& slope) {
+  const Gelu g = gelu_parts(x);
+  const float cdf = 0.5f + copysignf(g.half, x);
+  value = x * cdf;
+  slope = ffma(x, g.e * 0.3989422804014327f, cdf);
 }
 
 }  // namespace rp

@@ -15,7 +15,7 @@
 //
 // 131072 x 1024 in bf16: without GELU and dropout 93 us forward (5.8 TB/s) and 152
 // backward (5.3), which HBM bounds; with both 150 and 220, which vector
-// instructions bound (about 31 and 43 an element: GELU 16 forward and 22 backward,
+// instructions bound (about 31 and 42 an element: GELU 16 forward and 21 backward,
 // the generator 5).  16384 x 768, bf16 in and fp32 out, no GELU: 18 and 22 us.
 // A few rows are a launch's latency: one row of 384 3.8 us, 512 x 768 fp32 with
 // both 5.7 and 8.3, and 3.5 for the partial sums.

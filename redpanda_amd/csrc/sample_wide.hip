@@ -6,8 +6,8 @@
 // that makes the cut and draws.  What they share of a row is in the workspace.
 // Sums are of whole numbers and lists are put in order, so the order in which
 // workgroups add to them does not matter.  Rows that this does not hold (a long
-// list, a large top-k, +inf) the last launch does by itself, as sample_kernel
-// does.
+// list, a large top-k, +inf, min-p above 1) the last launch does by itself, as
+// sample_kernel does.
 //
 // 64 rows of 100003 fp32 logits: top-50 29 us (31 by a workgroup a row), a nucleus
 // 52 (67), no cut 27 (38); one row of 131072 bf16: top-50 22 (32), a nucleus 35
@@ -200,7 +200,10 @@ __global__ __launch_bounds__(kLastWaves* kWave) void sample_wide_draw_kernel(Sam
   const WideRow& w = static_cast<const WideRow*>(p.work)[r];
   const Settings set(p, r);
   const float top = wide_top(w);
-  const Plan plan = plan_of(p, set, top);
+  Plan plan = plan_of(p, set, top);
+  // no look has found the first place: min-p above 1 is a row's own setting, which
+  // the host does not see, and too rare for a launch in every call that has min-p a row
+  if (plan == kFirst && w.first == 0xffffffffu) plan = kAlone;
   if (plan == kNone || plan == kFirst) {
     if (tid == 0) {
       if (plan == kNone)

@@ -1495,7 +1495,9 @@ int rp_sample(const rp_sample_args* a, void* stream) {
   p.u = a->u;
   p.tokens = a->tokens;
   p.tsr = a->tokens_sr;
-  p.T = a->temperature;
+  // below 1e-300 all weights but those of the largest value are nothing, as at it,
+  // and the kernels' log2(e) / T would not be finite
+  p.T = a->temperature > 0.0 ? std::max(a->temperature, 1e-300) : a->temperature;
   p.tp = a->top_p;
   p.mp = a->min_p;
   p.k = a->top_k;

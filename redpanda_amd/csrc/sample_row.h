@@ -779,6 +779,12 @@ __device__ __forceinline__ void draw(Scratch<WAVES>& s, const RowWeights& rw, R&
   const uint64_t b = 2 * lane + 1 < kAll ? s.seg[2 * lane + 1] : 0;
   const uint64_t incl = wave_scan(a + b, lane);
   const uint64_t total = shfl64(incl, kWave - 1);
+  if (total == 0) {
+    // The largest value is kept and weighs 2^shift, so that there is a total unless
+    // the logits are written while they are looked at: no segment then holds u.
+    if (threadIdx.x == 0) give(-1, -__builtin_inff(), 1);
+    return;
+  }
   const uint64_t want = draw_at(u, total);
   const int l = __ffsll((unsigned long long)__ballot(incl > want)) - 1;
   uint64_t before = shfl64(incl - a - b, l);

@@ -35,3 +35,19 @@ def test_one_setting_a_row(gpu_lib, R, V):
         first = lg.argmax(1)
         alone = {"min_p": ~(v <= 1), "top_k": v == 1, "top_p": ~(v > 0), "temperature": ~(v > 0)}[name]
         assert torch.equal(ids[alone], first[alone]) and bool((logp[alone] == 0).all()), name
+
+
+@pytest.mark.parametrize("V", [300, 3000, 9001, 20001])
+def test_the_smallest_temperatures(gpu_lib, V):
+    """Only the largest logits have a weight, equal ones the same, down to the least
+    positive number."""
+    lg, u = make(5, V, seed=V)
+    lg[1, [3, V // 2, V - 1]] = 30.0
+    lg[2] = 0.25
+    lg[3, [V // 3, V - 2]] = float("inf")
+    lg[4, 5:] = -float("inf")
+    u[1], u[2], u[3] = 0.5, 0.75, 0.9
+    for T in (5e-324, 1e-310, 8e-309, 1e-300, 1e-45):
+        for s in (dict(), dict(k=2), dict(tp=0.9), dict(mp=1.0), dict(k=200, tp=0.5)):
+            check(lg, u, T=T, **s)
+    check(lg, u, T=torch.full((5,), 1e-45, device=dev), tp=0.9)

@@ -79,6 +79,8 @@ def sample_row(values, u, T=1.0, k=0, tp=1.0, mp=0.0):
         order = order[:k]
     with np.errstate(invalid="ignore"):
         w = np.where(values[order] == top, 1.0, np.exp((values[order] - top) / T))
+    if top == np.inf:  # nothing else has a weight beside it, at T = inf either
+        w[values[order] < top] = 0.0
     before = np.concatenate(([0.0], np.cumsum(w)[:-1]))
     keep = (w >= mp) & ((tp >= 1.0) | (before < tp * w.sum()))
     keep[0] = True

@@ -880,7 +880,7 @@ __device__ __forceinline__ void put_token(const SampleParams& p, int64_t r, int 
 // A value below which nothing is kept: min-p's bound (a little below it), or the
 // last kept one's.
 __device__ __forceinline__ float keep_bound(const RowWeights& rw, double T, double mp, uint64_t floor) {
-  const double b = rw.topd + T * log(mp);
+  const double b = mp < 1.0 ? rw.topd + T * log(mp) : rw.topd;  // (T may be infinite)
   const float least = mp > 0.0 ? (float)(b - 1e-6 * (fabs(b) + T)) : -__builtin_inff();
   return floor != 0 ? fmaxf(least, Floor(floor).value) : least;
 }

@@ -51,3 +51,22 @@ def test_the_smallest_temperatures(gpu_lib, V):
         for s in (dict(), dict(k=2), dict(tp=0.9), dict(mp=1.0), dict(k=200, tp=0.5)):
             check(lg, u, T=T, **s)
     check(lg, u, T=torch.full((5,), 1e-45, device=dev), tp=0.9)
+
+
+@pytest.mark.parametrize("R,V", [(8, 300), (8, 3000), (8, 9001), (8, 20001), (1300, 3000), (400, 17000)])
+def test_infinite_temperatures_a_row(gpu_lib, R, V):
+    """Every candidate weighs the same, whatever min-p asks for."""
+    lg, u = make(R, V, seed=V)
+    lg[1, ::3] = -float("inf")
+    lg[2, 7:9] = float("inf")
+    lg[4] = 0.0
+    T = torch.tensor([float("inf"), float("inf"), float("inf"), 1.0, float("inf"), 0.0, 3e38, 1e30],
+                     device=dev).repeat(-(-R // 8))[:R]
+    some = slice(0, 8)
+    for s in (dict(mp=1.0), dict(mp=0.5), dict(), dict(tp=0.3), dict(k=7), dict(k=7, mp=1.0),
+              dict(tp=0.5, mp=1.0), dict(k=200, tp=0.9)):
+        want = check(lg[some], u[some], T=T[some], **s)
+        ids = hip_sample(lg, u, temperature=T, top_k=s.get("k", 0), top_p=s.get("tp", 1.0),
+                         min_p=s.get("mp", 0.0))
+        assert torch.equal(ids[some], want)
+    check(lg[some], u[some], T=T[some], mp=torch.ones(8, device=dev))

@@ -47,7 +47,7 @@ struct RowWeights {
   __device__ __forceinline__ RowWeights(const SampleParams& p, float t, double T)
       : top(t), topd((double)t), c(1.4426950408889634 / T) {
     c32 = (float)c;
-    xmax = fminf((float)(36.1 * T), 3.4e38f);  // w < 2^-52
+    xmax = (float)(36.1 * T);  // w < 2^-52 (infinite where the type's lowest value has a weight)
     magic = __longlong_as_double((int64_t)(1023 + 52 - p.shift) << 52);
   }
   // log(w / total)

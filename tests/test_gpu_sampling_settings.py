@@ -70,3 +70,20 @@ def test_infinite_temperatures_a_row(gpu_lib, R, V):
                          min_p=s.get("mp", 0.0))
         assert torch.equal(ids[some], want)
     check(lg[some], u[some], T=T[some], mp=torch.ones(8, device=dev))
+
+
+@pytest.mark.parametrize("R,V", [(6, 20001), (6, 9001), (1300, 6000), (6, 600)])
+def test_temperatures_that_even_out_all_values(gpu_lib, R, V):
+    """A temperature at which even the type's lowest value has a weight: masked
+    places of that value count, and the cut falls among them."""
+    lg, u = make(R, V, seed=V + 1)
+    lg[:, 100:] = torch.finfo(torch.float32).min
+    lg[1, 50:100] = torch.finfo(torch.float32).max
+    some = slice(0, 6)
+    u[:6] = torch.tensor([0.999, 0.2, 0.5, 0.9, 1e-4, 0.97], device=dev)
+    for T in (1e38, 3e37, 1e300):
+        for s in (dict(tp=0.9), dict(tp=0.99), dict(k=500), dict(k=300, tp=0.5), dict(), dict(mp=0.01)):
+            want = check(lg[some], u[some], T=T, **s)
+            ids = hip_sample(lg, u, temperature=T, top_k=s.get("k", 0), top_p=s.get("tp", 1.0),
+                             min_p=s.get("mp", 0.0))
+            assert torch.equal(ids[some], want)

@@ -9,6 +9,7 @@ pre-norm layers' x + dropout(branch) needs it.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from redpanda_amd import _lib
@@ -73,6 +74,13 @@ def _run(x, res, p, seed, seed_t, stream, out_dtype):
     return out
 
 
+def recorded(grad):
+    """Whether a call goes through its autograd Function: where an input requires a
+    gradient, and within a forward-mode level, whose tangents (they do not show in
+    requires_grad) the Function refuses and the plain call would lose."""
+    return (grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0
+
+
 def once(backward):
     """A backward that may not be differentiated again: once_differentiable's
     marks where a graph of it is being recorded, and the function itself (5 us
@@ -116,7 +124,8 @@ def hip_dropout(x, p, seed, residual=None, stream=0):
     between a forward and its backward it must not change, which autograd
     checks).  The mask depends on the seed, `stream` (give each place of a model
     that drops its own, 0 .. 2^32 - 1), the row and the column only.
-    Differentiable in x and residual."""
+    Differentiable in x and residual, once and in reverse mode (a tangent is
+    refused)."""
     if not x.is_cuda:
         raise RuntimeError("redpanda_amd dropout: inputs must be ROCm device tensors")
     if x.dim() == 0:
@@ -135,6 +144,6 @@ def hip_dropout(x, p, seed, residual=None, stream=0):
     if not 0 <= stream < 1 << 32:
         raise ValueError(f"dropout: stream must be in [0, 2^32), got {stream}")
     seed, seed_t = seed_arg(seed, x.device, "dropout")
-    if grad and torch.is_grad_enabled():
+    if recorded(grad):
         return _HipDropout.apply(x, residual, p, seed, seed_t, stream, out_dtype)
     return _run(x, residual, p, seed, seed_t, stream, out_dtype)

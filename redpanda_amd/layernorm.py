@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from redpanda_amd import _lib
-from redpanda_amd.dropout import check_p, dtype_code, empty_rows, once, rows_of, seed_arg
+from redpanda_amd.dropout import check_p, dtype_code, empty_rows, once, recorded, rows_of, seed_arg
 
 
 def _f32c(t):
@@ -90,7 +90,8 @@ def hip_layernorm(x, weight=None, bias=None, eps=1e-5, gelu=False, p=0.0, seed=N
     the result, as hip_dropout draws it (seed may be None where p is 0);
     out_dtype: the result's dtype, x's by default (torch's layer norm under
     autocast gives fp32).  Everything between is fp32.  Differentiable in x,
-    weight and bias; the weights' gradients are summed in a fixed order."""
+    weight and bias, once and in reverse mode (a tangent is refused); the weights'
+    gradients are summed in a fixed order."""
     if not x.is_cuda:
         raise RuntimeError("redpanda_amd layernorm: inputs must be ROCm device tensors")
     if x.dim() == 0 or x.shape[-1] == 0:
@@ -116,6 +117,6 @@ def hip_layernorm(x, weight=None, bias=None, eps=1e-5, gelu=False, p=0.0, seed=N
     if not eps >= 0.0:
         raise ValueError(f"layernorm: eps must be >= 0, got {eps}")
     gelu = 1 if gelu else 0
-    if grad and torch.is_grad_enabled():
+    if recorded(grad):
         return _HipLayerNorm.apply(x, weight, bias, eps, gelu, p, seed, seed_t, stream, out_dtype)
     return _forward(x, weight, bias, eps, gelu, p, seed, seed_t, stream, out_dtype, False)[0]

@@ -470,7 +470,8 @@ int rp_layernorm_bwd(const rp_layernorm_args* a, const rp_layernorm_grad* g, voi
  * ones' total (u in [0, 1); from 1 on: the last kept one).
  * logits: (R, V) in dtype_logits with row stride logits_sr; u: (R,) fp32;
  * tokens: NULL or (R, M) int32 with row stride tokens_sr.  temperature, top_p,
- * min_p, top_k: one value, or where the *_row pointer is given (R,) values.
+ * min_p, top_k: one value, or where the *_row pointer is given (R,) values (which
+ * are not checked: a NaN or a min_p above 1 keeps the first alone).
  * ids: (R,) int64, -1 for a row without candidates; logp: NULL or (R,) fp32, the
  * logarithm of the token's share of the kept weights (-inf without candidates).
  * Weights are summed as 64-bit integers, so results do not depend on order.

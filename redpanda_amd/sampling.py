@@ -56,8 +56,14 @@ def hip_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
     place, at which the running sum of weights exceeds u times the total of the
     kept ones.  tokens: None, or (R, M) ids in whose order the candidates stand
     instead of the vocabulary's (ids outside [0, V), like -1, are padding).  Each
-    setting is a number or an (R,) tensor.  A row without candidates gives -1 (and
-    -inf); logprob is the logarithm of the token's share of the kept weights."""
+    setting is a number or an (R,) tensor, taken in fp32 and not looked at on the
+    host: there a temperature of 0 or less, a top_p of 0 or less, a min_p above 1
+    or a NaN keeps the first alone, and an infinite temperature gives every
+    candidate the same weight (beside +inf only other +inf have one).  A row
+    without candidates gives -1 (and -inf); logprob is the logarithm of the token's
+    share of the kept weights.  Neither result is differentiable: a logits' gradient
+    or tangent ends here, and a loss that needs the log-probability's forms it
+    from the logits."""
     if logits.dim() != 2 or not logits.is_cuda:
         raise ValueError(f"sample: logits must be a (R, V) device tensor, got {tuple(logits.shape)} on "
                          f"{logits.device}")

@@ -205,11 +205,13 @@ class SearchMamba(nn.Module):
         (T, K), values (T, K) of the states the moves lead to.  legal: None, or a
         function of (ply, the tokens before it or None) that gives the ply's (K,
         M) legal ids padded with -1.  A rollout without a move ends: its tokens
-        are -1 from there on, its value stays.  settings: hip_sample's."""
+        are -1 from there on, its value stays (the board's own before the first
+        move).  settings: hip_sample's."""
         T, k = u.shape
         hidden, cache = self.prime_board(board_encoding.to(self._device()), compact=compact)
+        value = torch.tanh(self._fused_head(self.value_head, hidden)).squeeze(-1).expand(k)
         hidden, cache = hidden.expand(k, -1).contiguous(), self._expand_cache(cache, k)
-        tokens, logps, values, alive, value = [], [], [], None, None
+        tokens, logps, values, alive = [], [], [], None
         for t in range(T):
             moves = None if legal is None else legal(t, tokens[-1] if tokens else None)
             ids, logp = self.sample_moves(hidden, u[t], moves, **settings)
@@ -218,7 +220,7 @@ class SearchMamba(nn.Module):
             # an ended rollout steps on with token 0, unseen
             hidden, cache = self.backbone.step(token_id=ids.clamp(min=0), cache=cache)
             v = torch.tanh(self._fused_head(self.value_head, hidden)).squeeze(-1)
-            value = torch.where(alive, v, torch.zeros_like(v) if value is None else value)
+            value = torch.where(alive, v, value)
             tokens.append(ids)
             logps.append(torch.where(alive, logp, float("-inf")))
             values.append(value)

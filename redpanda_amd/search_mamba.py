@@ -224,6 +224,9 @@ class SearchMamba(nn.Module):
             tokens.append(ids)
             logps.append(torch.where(alive, logp, float("-inf")))
             values.append(value)
+        if T == 0:
+            return (u.new_empty((0, k), dtype=torch.int64), u.new_empty((0, k), dtype=torch.float32),
+                    value.new_empty((0, k)))
         return torch.stack(tokens), torch.stack(logps), torch.stack(values)
 
     @torch.no_grad()

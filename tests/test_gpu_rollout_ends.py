@@ -29,3 +29,14 @@ def test_a_rollout_without_a_first_move_has_the_boards_value(gpu_lib, compact):
                                          compact=compact)
     assert torch.equal(tok[:, live], tok2)
     assert float((val[:, live] - val2).abs().max()) <= 1e-5
+
+
+def test_no_plies(gpu_lib):
+    m = model(4)
+    tok, logp, val = m.sample_rollout(torch.arange(9), torch.rand(0, 5, device=dev))
+    assert tok.shape == logp.shape == val.shape == (0, 5)
+    assert tok.dtype == torch.int64 and logp.dtype == val.dtype == torch.float32
+    with torch.autocast("cuda", torch.bfloat16):
+        a = m.sample_rollout(torch.arange(9), torch.rand(0, 5, device=dev))
+        b = m.sample_rollout(torch.arange(9), torch.rand(1, 5, device=dev))
+    assert [t.dtype for t in a] == [t.dtype for t in b]

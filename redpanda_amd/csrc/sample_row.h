@@ -779,14 +779,15 @@ __device__ __forceinline__ void draw(Scratch<WAVES>& s, const RowWeights& rw, R&
   const uint64_t b = 2 * lane + 1 < kAll ? s.seg[2 * lane + 1] : 0;
   const uint64_t incl = wave_scan(a + b, lane);
   const uint64_t total = shfl64(incl, kWave - 1);
-  if (total == 0) {
-    // The largest value is kept and weighs 2^shift, so that there is a total unless
-    // the logits are written while they are looked at: no segment then holds u.
+  const uint64_t want = draw_at(u, total);
+  const uint64_t past = __ballot(incl > want);
+  if (past == 0) {
+    // The largest value is kept and weighs 2^shift, so that some segment holds u
+    // unless the logits are written while they are looked at.
     if (threadIdx.x == 0) give(-1, -__builtin_inff(), 1);
     return;
   }
-  const uint64_t want = draw_at(u, total);
-  const int l = __ffsll((unsigned long long)__ballot(incl > want)) - 1;
+  const int l = __ffsll((unsigned long long)past) - 1;
   uint64_t before = shfl64(incl - a - b, l);
   const uint64_t head = shfl64(a, l);
   int g = 2 * l;
@@ -861,6 +862,9 @@ struct Settings {
   float u;
   __device__ __forceinline__ Settings(const SampleParams& p, int64_t r) {
     T = p.T_row != nullptr ? (double)p.T_row[r] : p.T;
+    // (infinity times the logarithm of a min-p of 1 would be a NaN; all weights are 1
+    // from far below this on)
+    if (T > 1e300) T = 1e300;
     tp = p.tp_row != nullptr ? (double)p.tp_row[r] : p.tp;
     mp = p.mp_row != nullptr ? (double)p.mp_row[r] : p.mp;
     k = p.k_row != nullptr ? (int64_t)p.k_row[r] : p.k;
@@ -880,7 +884,7 @@ __device__ __forceinline__ void put_token(const SampleParams& p, int64_t r, int 
 // A value below which nothing is kept: min-p's bound (a little below it), or the
 // last kept one's.
 __device__ __forceinline__ float keep_bound(const RowWeights& rw, double T, double mp, uint64_t floor) {
-  const double b = mp < 1.0 ? rw.topd + T * log(mp) : rw.topd;  // (T may be infinite)
+  const double b = rw.topd + T * log(mp);
   const float least = mp > 0.0 ? (float)(b - 1e-6 * (fabs(b) + T)) : -__builtin_inff();
   return floor != 0 ? fmaxf(least, Floor(floor).value) : least;
 }

@@ -68,10 +68,18 @@ void go(const SampleParams& p, hipStream_t st) {
   // else, in registers up to 8192 elements; sixteen for the rows that are too few
   // and too long for that (300 rows of 16000: 37 us by four, 54 by sixteen, of
   // which a CU holds two workgroups; 130 of 131072: 165 and 84).
-  const bool wave_list = p.k_row != nullptr || p.k < 192;  // (a list of a wave's LDS)
+  // A top-k beyond what a shape lists is cut by histograms, from several more looks
+  // at the row.  One wave does that sooner than four list it while the row is short
+  // (4096 rows of 8192, top-129: 93 and 134 us; the rows' own k are taken so, too),
+  // not beyond (1300 of 16000: 130 and 55; 4000 of 12000: 127 and 108, though at
+  // top-191 135 and 152); and sixteen waves list what four do later once there are
+  // more rows than the card holds at a time (1000 of 30000, top-192: 108 by sixteen,
+  // 49 by four; 330 of 100000: 77 and 96).
+  const int64_t k = p.k_row != nullptr ? 0 : p.k;
+  const bool few = k < 192;
   if (p.n <= 512 && p.R >= 512)
     RP_GO(1, 1);
-  else if (p.R >= (p.n <= 2048 ? 512 : 1280) && wave_list)
+  else if (p.R >= (p.n <= 2048 ? 512 : 1280) && (p.n <= 8192 ? few : k <= listed_of(1)))
     RP_GO(1, 0);
   else if (p.n <= 2048)
     RP_GO(4, 1);
@@ -79,7 +87,7 @@ void go(const SampleParams& p, hipStream_t st) {
     RP_GO(4, 2);
   else if (p.n <= 8192)
     RP_GO(4, 4);
-  else if (p.R > (p.n <= 16384 ? 64 : 320) && wave_list)
+  else if ((p.R > (p.n <= 16384 ? 64 : 320) && few) || (p.R > 512 && k <= listed_of(4)))
     RP_GO(4, 0);
   else
     RP_GO(16, 0);

@@ -15,6 +15,10 @@ constexpr int kSegments = 8;  // of a wave's stretch, for the draw
 // several take together: 8 KB, so that LDS holds as many rows on a CU as the
 // registers do (16; with 16 KB it held 9).
 constexpr int list_of(int waves) { return waves == 1 ? 256 : waves == 4 ? 1024 : 2048; }
+// the largest top-k that is listed: as many as bound a list that mostly fits it
+constexpr int listed_of(int waves) {
+  return 2 * waves * kWave < list_of(waves) ? 2 * waves * kWave : list_of(waves) - 1;
+}
 // bits of an exact histogram's steps
 constexpr int bits_of(int waves) { return waves == 1 ? 9 : waves == 4 ? 10 : 11; }
 constexpr int bins_of(int waves) { return 1 << bits_of(waves); }
@@ -962,7 +966,7 @@ __device__ __forceinline__ void sample_row(const SampleParams& p, int64_t r, Scr
   const bool cut_k = k > 0 && k < p.n, cut_p = tp < 1.0;
   // a list of all that can be kept
   bool listed = false;
-  if (cut_k && k <= 2 * kT && k < s.kList) {
+  if (cut_k && k <= listed_of(WAVES)) {
     uint32_t g[4], bound;
 #pragma unroll
     for (int i = 0; i < 4; ++i) g[i] = value_key(look.most[i]);

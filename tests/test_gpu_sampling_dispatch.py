@@ -106,3 +106,13 @@ def test_lists_of_every_shape(gpu_lib, R, M, t):
     tok = torch.where(torch.arange(M, device=dev) < n, tok, -1)
     for s in (dict(), dict(tp=0.9), dict(k=40, tp=0.95), dict(mp=0.05, T=0.7), dict(k=150), dict(T=0.0)):
         check(lg, u, tokens=tok, **s)
+
+
+@pytest.mark.parametrize("R,V", [(1300, 1500), (1300, 7001), (1300, 9001), (600, 17001), (1400, 17001)])
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_top_k_around_what_a_shape_lists(gpu_lib, R, V, t):
+    lg, u = rows_of_all_kinds(R, V, t, V)
+    for k in (127, 128, 129, 191, 192, 511, 512, 513, V - 1, V, V + 1):
+        check(lg, u, k=k)
+    k = torch.arange(R, device=dev, dtype=torch.int32) % 7 * 40
+    check(lg, u, k=k, tp=0.95)

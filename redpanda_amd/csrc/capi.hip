@@ -1357,7 +1357,9 @@ rp::LayerNormParams layernorm_params(const rp_layernorm_args* a) {
 
 int64_t rp_layernorm_work_bytes(const rp_layernorm_args* a) {
   if (rp_layernorm_check(a) != RP_OK) return -1;
-  return round_up((int64_t)rp::layernorm_parts(a->rows, a->d) * 2 * a->d * 4, 256);
+  const int n = rp::layernorm_parts(a->rows, a->d, (int)elem_size(a->dtype_x),
+                                    (int)elem_size(a->dtype_out));
+  return round_up((int64_t)n * 2 * a->d * 4, 256);
 }
 
 int rp_layernorm_fwd(const rp_layernorm_args* a, void* stream) {

@@ -227,9 +227,9 @@ unsigned walk_grid(int64_t rows, int G, int most) {
 
 }  // namespace
 
-int layernorm_parts(int64_t rows, int64_t d) {
+int layernorm_parts(int64_t rows, int64_t d, int es_x, int es_out) {
   const int G = norm_group(d);
-  if (G != 0) return (int)walk_grid(rows, G, norm_workgroups(d, true));
+  if (G != 0) return (int)walk_grid(rows, G, norm_workgroups_bwd(d, es_x, es_out));
   const int64_t tiles = (d + 8 * kWave - 1) / (8 * kWave);
   const int64_t n = (rows + 4 * kWaves - 1) / (4 * kWaves);
   const int64_t most = (2048 + tiles - 1) / tiles;
@@ -240,7 +240,7 @@ hipError_t launch_layernorm_fwd(const LayerNormParams& p, hipStream_t st) {
   if (p.rows == 0) return hipSuccess;
   const int G = norm_group(p.d);
   if (G != 0) {
-    const unsigned wg = walk_grid(p.rows, G, norm_workgroups(p.d, false));
+    const unsigned wg = walk_grid(p.rows, G, norm_workgroups_fwd(p.d));
     return p.es_x == 4 ? launch_norm_fwd4(p, wg, st) : launch_norm_fwd2(p, wg, st);
   }
   hipLaunchKernelGGL(layernorm_fwd_kernel, dim3(row_grid(p.rows)), dim3(kThreads), 0, st, p);
@@ -248,7 +248,7 @@ hipError_t launch_layernorm_fwd(const LayerNormParams& p, hipStream_t st) {
 }
 
 hipError_t launch_layernorm_bwd(const LayerNormParams& p, const LayerNormGrad& g, hipStream_t st) {
-  const int n = layernorm_parts(p.rows, p.d);
+  const int n = layernorm_parts(p.rows, p.d, p.es_x, p.es_out);
   if (p.rows > 0 && norm_group(p.d) != 0) {
     auto* launch = p.es_x == 4 ? (p.es_out == 4 ? launch_norm_bwd44 : launch_norm_bwd42)
                                : (p.es_out == 4 ? launch_norm_bwd24 : launch_norm_bwd22);

@@ -372,13 +372,22 @@ inline int norm_group(int64_t d) {
 // Workgroups that a launch of G lanes a row fills the card with: as many as its
 // registers let be resident, since a second round of a part of them would cost
 // as much as a whole one (131072 x 1024 backward: 1024 workgroups where 768 fit
-// took a quarter longer).
-inline int norm_workgroups(int64_t d, bool backward) {
+// took a quarter longer).  The backward's registers go by the bytes of an element
+// of x and of a gradient: with fp32 on both sides fewer fit (two blocks a lane
+// 173 of them, three 262 or 252; backward of 131072 x 1024 309 us by 768
+// workgroups, 278 by the 512 that fit; 16384 x 768 33 and 29).
+inline int norm_workgroups_fwd(int64_t d) {
   const int G = norm_group(d);
-  if (G > 256) return backward || G == 1024 ? 256 : 512;
+  if (G > 256) return G == 1024 ? 256 : 512;
   const int nb = (int)((d + 8 * G - 1) / (8 * G));
-  const int a_cu = backward ? (nb == 1 ? 4 : nb == 2 ? 3 : 2) : (nb == 1 ? 7 : nb == 2 ? 5 : 3);
-  return 256 * a_cu;
+  return 256 * (nb == 1 ? 7 : nb == 2 ? 5 : 3);
+}
+inline int norm_workgroups_bwd(int64_t d, int es_x, int es_out) {
+  const int G = norm_group(d);
+  if (G > 256) return 256;
+  const int nb = (int)((d + 8 * G - 1) / (8 * G));
+  const bool wide = es_x + es_out == 8 || (G == 256 && es_out == 4);
+  return 256 * (nb == 1 ? 4 : nb == 2 ? (wide ? 2 : 3) : es_x + es_out == 8 && G < kWave ? 1 : 2);
 }
 
 template <int ES>

@@ -55,8 +55,9 @@ struct LayerNormGrad {
   float* part;       // (layernorm_parts, 2, d) workspace
 };
 
-// Partial sums of the weights' gradients that a backward writes.
-int layernorm_parts(int64_t rows, int64_t d);
+// Partial sums of the weights' gradients that a backward writes (es: bytes of an
+// element).
+int layernorm_parts(int64_t rows, int64_t d, int es_x, int es_out);
 hipError_t launch_layernorm_fwd(const LayerNormParams& p, hipStream_t st);
 hipError_t launch_layernorm_bwd(const LayerNormParams& p, const LayerNormGrad& g, hipStream_t st);
 

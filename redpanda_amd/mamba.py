@@ -378,7 +378,9 @@ class Mamba(nn.Module):
         """(B, L) ids or (B, L, d_model) embeddings -> (B, L, d_model).
         dropout > 0: each layer's branch is dropped out with the residual added
         in the same pass (hip_dropout with `seed`, the layer's index as its
-        stream), for training; 0 adds the branch as it is."""
+        stream: a seed of its own for each call, since SearchMamba's heads count
+        their streams from 0, too), for training, but wherever it is asked for:
+        self.training is not looked at; 0 adds the branch as it is."""
         x = input_embeds if input_embeds is not None else self.embedding(input_ids)
         for i, layer in enumerate(self.layers):
             mixer, norm = layer["mixer"], layer["norm"]

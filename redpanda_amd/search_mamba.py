@@ -171,7 +171,10 @@ class SearchMamba(nn.Module):
         dropout > 0 (training): the value and the continuation head drop out
         behind their norms, with masks of `seed` (an int, or an int64 tensor of
         one element on the device, which a captured step reads on each replay)
-        that no pass stores; step t draws streams 2 t and 2 t + 1."""
+        that no pass stores; step t draws streams 2 t and 2 t + 1, so that a call
+        takes a seed of its own beside the backbone's (whose layers draw streams
+        from 0 on).  It drops wherever it is asked to: self.training is not looked
+        at."""
         _, cache = self.backbone.prime_cache(board_encoding)
         vs, cs, fs = [], [], []
         for t in range(move_tokens.shape[1]):

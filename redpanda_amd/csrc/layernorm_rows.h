@@ -13,12 +13,14 @@
 // backward keeps the columns' sums in registers over all its rows, and the
 // generator's first products, which depend on the column alone, leave the loop.
 //
-// 131072 x 1024 in bf16: without GELU and dropout 93 us forward (5.8 TB/s) and 152
-// backward (5.3), which HBM bounds; with both 150 and 220, which vector
-// instructions bound (about 31 and 42 an element: GELU 16 forward and 21 backward,
-// the generator 5).  16384 x 768, bf16 in and fp32 out, no GELU: 18 and 22 us.
-// A few rows are a launch's latency: one row of 384 3.8 us, 512 x 768 fp32 with
-// both 5.7 and 8.3, and 3.5 for the partial sums.
+// 131072 x 1024 in bf16: without GELU and dropout 93 us forward (5.8 TB/s) and 150
+// backward (5.4), which HBM bounds; with both 151 and 217, which vector
+// instructions bound (31 and 41 an element: GELU 16 forward and 21 backward, the
+// generator 5).  16384 x 768, bf16 in and fp32 out, no GELU: 18 and 22 us; fp32 both
+// 18 and 29.  A few rows are a launch's latency: one row of 384 3.9 us, 512 x 768
+// fp32 with both 5.6 and 8.3, and 3.4 for the partial sums.  Rows of 8193 to 16384
+// fall behind: their 1024 lanes have 128 registers each, the backward spills 46 to
+// 88 of what it keeps (8192 x 9000 with both: fp32 189 and 335 us, bf16 139 and 447).
 #pragma once
 
 #include "rp_heads.h"

@@ -39,10 +39,11 @@
 // one that u falls into again.
 //
 // What bounds it: vector instructions.  A nucleus of 4096 rows of 8192 bf16
-// logits takes 82-91 us, of which 59 are issue: some 70 instructions an element,
+// logits takes 83-93 us, of which 63 are issue: some 72 instructions an element,
 // 16 of them in the first look, 15 for the histogram and 32 for the exact weights
-// (its 67 MB would take 13 us).  Without cuts 63 us (fp32, 134 MB), top-40 58, one
-// row of 8192 12.6, 777 lists of up to 218 ids 10.
+// (its 67 MB would take 13 us).  Without cuts 63 us (fp32, 134 MB), top-40 58,
+// top-200 and top-1000 (bf16, the lists' order and the exact histograms) 159 and
+// 196; one row of 8192 12.6, 777 lists of up to 218 ids 10.
 
 #include "sample_row.h"
 

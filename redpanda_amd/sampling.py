@@ -61,7 +61,7 @@ def hip_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens
     or a NaN keeps the first alone, and an infinite temperature gives every
     candidate the same weight (beside +inf only other +inf have one).  A row
     without candidates gives -1 (and -inf); logprob is the logarithm of the token's
-    share of the kept weights.  Neither result is differentiable: a logits' gradient
+    share of the kept weights.  Neither result is differentiable: the logits' gradient
     or tangent ends here, and a loss that needs the log-probability's forms it
     from the logits."""
     if logits.dim() != 2 or not logits.is_cuda:

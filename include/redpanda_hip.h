@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define RP_ABI_VERSION 15
+#define RP_ABI_VERSION 16
 
 /* element type codes of the streamed scan inputs (delta, u, Bc, Cc); each
  * tensor carries its own code, as autocast hands over mixed dtypes */
@@ -502,6 +502,168 @@ int rp_sample_check(const rp_sample_args* a);
 /* Bytes of scratch that rp_sample makes use of (0: none). */
 int64_t rp_sample_work_bytes(const rp_sample_args* a);
 int rp_sample(const rp_sample_args* a, void* stream);
+
+/*
+ * Embedding: rows of a table, scaled.
+ *     out[i] = scale w[ids[i]]
+ * rounded once to dtype_out.  ids: (N,) int32, or int64 with ids64 = 1; an id
+ * outside [0, V), like -1, is padding: a row of zeros, and no gradient.  w: (V, d)
+ * in dtype_w with row stride w_sr; out: (N, d) contiguous in dtype_out, which must
+ * not overlap w.  padding: an id of the table whose row gets no gradient (its rows
+ * come out as they are), or -1.
+ */
+typedef struct rp_embedding_args {
+  int64_t N, V, d;
+  int32_t dtype_w, dtype_out, ids64;
+  float scale;
+  int64_t padding;
+  const void* ids;
+  const void* w;  int64_t w_sr;
+  void* out;
+} rp_embedding_args;
+
+/*
+ * The table's gradient: dw[v] = scale times the sum of dout[i] over the places i
+ * with ids[i] = v, in fp32 and in a fixed order (the places are sorted by their
+ * ids), rounded once; zeros for ids that do not occur.  dout: (N, d) in dtype_out
+ * with row stride dout_sr; dw: (V, d) contiguous in dtype_w.  The forward's w and
+ * out are not read.  work: rp_embedding_work_bytes() of scratch, 256-byte aligned.
+ */
+typedef struct rp_embedding_grad {
+  const void* dout; int64_t dout_sr;
+  void* dw;
+  void* work;
+  int64_t work_bytes;
+} rp_embedding_grad;
+
+/* Validate embedding arguments on the host without launching anything. */
+int rp_embedding_check(const rp_embedding_args* a);
+
+/* Bytes of scratch rp_embedding_bwd needs. */
+int64_t rp_embedding_work_bytes(const rp_embedding_args* a);
+int rp_embedding_fwd(const rp_embedding_args* a, void* stream);
+int rp_embedding_bwd(const rp_embedding_args* a, const rp_embedding_grad* g, void* stream);
+
+/*
+ * Rows in 8 bits.  Each block of 32 columns of a row (the last one what is left)
+ * shares a power of two, the least 2^E >= 2^-126 that takes the block's largest
+ * magnitude to an integer of at most 127: q = round(x 2^-E), to nearest even, and
+ * e = E + 127.  What is held, q 2^E, is off by half of 2^E at most.  A block with an
+ * infinity or a NaN has e = 255 and comes back as NaN.
+ * x: (rows, d) in dtype with row stride x_sr (contiguous for rp_unpack, which
+ * writes it); q: (rows, d) int8 contiguous; e: (rows, ceil(d / 32)) contiguous.
+ */
+typedef struct rp_pack_args {
+  int64_t rows, d;
+  int32_t dtype, reserved;
+  void* x;  int64_t x_sr;
+  int8_t* q;
+  uint8_t* e;
+} rp_pack_args;
+
+int rp_pack_check(const rp_pack_args* a);
+int rp_pack(const rp_pack_args* a, void* stream);
+int rp_unpack(const rp_pack_args* a, void* stream);
+
+/*
+ * RMS norm with the residual's addition (engine/mamba.py:82-89, and the
+ * pre-norm residual loop of :592-597), for training: per row
+ *     s = x [+ add],  r = 1 / sqrt(mean(s^2) + eps),  out = s r w
+ * s rounded to dtype_sum first (without add it is x, and dtype_sum is dtype_x).  x:
+ * (rows, d) in dtype_x with row stride x_sr; add: NULL or (rows, d) in dtype_add;
+ * w: (d,) fp32 or NULL (1); sum: (rows, d) contiguous in dtype_sum (NULL without
+ * add); out: (rows, d) contiguous in dtype_out, or NULL; q, e: NULL, or s in 8 bits
+ * (as rp_pack writes it) beside the rest.
+ * With x NULL the rows are those that q and e hold (dtype_sum names no buffer then,
+ * add and sum are NULL): a checkpointed layer's norm, computed again.
+ * All arithmetic in fp32.
+ */
+typedef struct rp_addnorm_args {
+  int64_t rows, d;
+  int32_t dtype_x, dtype_add, dtype_sum, dtype_out;
+  const void* x;    int64_t x_sr;
+  const void* add;  int64_t add_sr;
+  const float* w;
+  void* sum;
+  void* out;
+  int8_t* q;
+  uint8_t* e;
+  float eps;
+  int32_t reserved;
+} rp_addnorm_args;
+
+/*
+ * Its backward: with g = dout, q = g w and xh = s r
+ *     ds = dsum + r (q - xh mean(q xh)),  dw = sum over the rows of g xh
+ * where s is a->x (row stride x_sr, in dtype_sum), or with a->x NULL what a->q and
+ * a->e hold: the gradient at the values that were kept.  dout: (rows, d) in
+ * dtype_out; dsum: NULL or (rows, d) in dtype_sum; dx, dadd: NULL or (rows, d)
+ * contiguous, ds in dtype_x and in dtype_add; dw: NULL or (d,) fp32, summed in a
+ * fixed order.  The forward's add, sum and out are not read.  work:
+ * rp_addnorm_work_bytes() of scratch, 256-byte aligned (unused without dw).
+ */
+typedef struct rp_addnorm_grad {
+  const void* dout; int64_t dout_sr;
+  const void* dsum; int64_t dsum_sr;
+  void* dx;
+  void* dadd;
+  float* dw;
+  void* work;
+  int64_t work_bytes;
+} rp_addnorm_grad;
+
+int rp_addnorm_check(const rp_addnorm_args* a);
+int64_t rp_addnorm_work_bytes(const rp_addnorm_args* a);
+int rp_addnorm_fwd(const rp_addnorm_args* a, void* stream);
+int rp_addnorm_bwd(const rp_addnorm_args* a, const rp_addnorm_grad* g, void* stream);
+
+/*
+ * Gated linear recurrence along a sequence, each channel by itself:
+ *     a_t = 1 / (1 + exp(-gate_t)),   h_t = a_t h_{t-1} + (1 - a_t) x_t,   y_t = h_t
+ * from h_{-1} = h0 (NULL: 0).  Where starts is not 0 a sequence begins anew: h_{t-1}
+ * counts as 0 (1 - a_t stays).  A gate of +inf keeps the state, -inf takes x_t.
+ * x, gate: (B, L, D) in dtype with strides *_sb and *_sl and unit stride along D;
+ * h0: (B, D) fp32; starts: NULL or (B, L) bytes with batch stride starts_sb and unit
+ * stride along L; y: (B, L, D) contiguous in dtype; h_last: NULL or (B, D) fp32;
+ * ckpt: NULL, or rp_gated_ckpt_bytes() for a later backward.  The state is fp32
+ * throughout.  work: rp_gated_work_bytes(a, 0) of scratch, 256-byte aligned: few
+ * channels of a long sequence are split along it.
+ */
+typedef struct rp_gated_args {
+  int64_t B, L, D;
+  int32_t dtype, reserved;
+  const void* x;     int64_t x_sb, x_sl;
+  const void* gate;  int64_t gate_sb, gate_sl;
+  const float* h0;
+  const uint8_t* starts;  int64_t starts_sb;
+  void* y;
+  float* h_last;
+  float* ckpt;
+  void* work;
+  int64_t work_bytes;
+} rp_gated_args;
+
+/*
+ * Its backward.  With dh_t the gradient that reaches h_t (dy_t, and a_{t+1}
+ * dh_{t+1} from the step behind it unless that one starts anew; dh_last at the end):
+ *     dx_t = (1 - a_t) dh_t,  dgate_t = (h_{t-1} - x_t) a_t (1 - a_t) dh_t
+ * dy: NULL or (B, L, D) in dtype with strides; dh_last: NULL or (B, D); dx, dgate:
+ * (B, L, D) contiguous in dtype; dh0: NULL or (B, D) fp32.  a->ckpt: what the forward
+ * wrote; a->y and a->h_last are not read.  a->work: rp_gated_work_bytes(a, 1).
+ */
+typedef struct rp_gated_grad {
+  const void* dy;  int64_t dy_sb, dy_sl;
+  const float* dh_last;
+  void* dx;
+  void* dgate;
+  float* dh0;
+} rp_gated_grad;
+
+int rp_gated_check(const rp_gated_args* a);
+int64_t rp_gated_ckpt_bytes(const rp_gated_args* a);
+int64_t rp_gated_work_bytes(const rp_gated_args* a, int backward);
+int rp_gated_fwd(const rp_gated_args* a, void* stream);
+int rp_gated_bwd(const rp_gated_args* a, const rp_gated_grad* g, void* stream);
 
 /* ABI version this library was built with (RP_ABI_VERSION). */
 int rp_abi_version(void);

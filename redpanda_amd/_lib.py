@@ -13,7 +13,7 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libredpanda_hip.so")
 
-ABI_VERSION = 15
+ABI_VERSION = 16
 RP_F32, RP_BF16, RP_F16 = 0, 1, 2
 DTYPE_CODES = {torch.float32: RP_F32, torch.bfloat16: RP_BF16, torch.float16: RP_F16}
 MAX_STATE = 128
@@ -171,6 +171,60 @@ class SampleArgs(ctypes.Structure):
     ]
 
 
+class EmbeddingArgs(ctypes.Structure):
+    _fields_ = [
+        ("N", _i64), ("V", _i64), ("d", _i64), ("dtype_w", _i32), ("dtype_out", _i32),
+        ("ids64", _i32), ("scale", ctypes.c_float), ("padding", _i64), ("ids", _vp),
+        ("w", _vp), ("w_sr", _i64), ("out", _vp),
+    ]
+
+
+class EmbeddingGrad(ctypes.Structure):
+    _fields_ = [
+        ("dout", _vp), ("dout_sr", _i64), ("dw", _vp), ("work", _vp), ("work_bytes", _i64),
+    ]
+
+
+class PackArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("d", _i64), ("dtype", _i32), ("reserved", _i32),
+        ("x", _vp), ("x_sr", _i64), ("q", _vp), ("e", _vp),
+    ]
+
+
+class AddNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("d", _i64), ("dtype_x", _i32), ("dtype_add", _i32), ("dtype_sum", _i32),
+        ("dtype_out", _i32), ("x", _vp), ("x_sr", _i64), ("add", _vp), ("add_sr", _i64),
+        ("w", _vp), ("sum", _vp), ("out", _vp), ("q", _vp), ("e", _vp),
+        ("eps", ctypes.c_float), ("reserved", _i32),
+    ]
+
+
+class AddNormGrad(ctypes.Structure):
+    _fields_ = [
+        ("dout", _vp), ("dout_sr", _i64), ("dsum", _vp), ("dsum_sr", _i64),
+        ("dx", _vp), ("dadd", _vp), ("dw", _vp), ("work", _vp), ("work_bytes", _i64),
+    ]
+
+
+class GatedArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _i64), ("L", _i64), ("D", _i64), ("dtype", _i32), ("reserved", _i32),
+        ("x", _vp), ("x_sb", _i64), ("x_sl", _i64),
+        ("gate", _vp), ("gate_sb", _i64), ("gate_sl", _i64),
+        ("h0", _vp), ("starts", _vp), ("starts_sb", _i64),
+        ("y", _vp), ("h_last", _vp), ("ckpt", _vp), ("work", _vp), ("work_bytes", _i64),
+    ]
+
+
+class GatedGrad(ctypes.Structure):
+    _fields_ = [
+        ("dy", _vp), ("dy_sb", _i64), ("dy_sl", _i64), ("dh_last", _vp),
+        ("dx", _vp), ("dgate", _vp), ("dh0", _vp),
+    ]
+
+
 # Every symbol include/redpanda_hip.h declares, with its ctypes signature.
 SIGNATURES = {
     "rp_abi_version": (ctypes.c_int, []),
@@ -209,6 +263,23 @@ SIGNATURES = {
     "rp_sample_check": (ctypes.c_int, [ctypes.POINTER(SampleArgs)]),
     "rp_sample_work_bytes": (_i64, [ctypes.POINTER(SampleArgs)]),
     "rp_sample": (ctypes.c_int, [ctypes.POINTER(SampleArgs), _vp]),
+    "rp_embedding_check": (ctypes.c_int, [ctypes.POINTER(EmbeddingArgs)]),
+    "rp_embedding_work_bytes": (_i64, [ctypes.POINTER(EmbeddingArgs)]),
+    "rp_embedding_fwd": (ctypes.c_int, [ctypes.POINTER(EmbeddingArgs), _vp]),
+    "rp_embedding_bwd": (ctypes.c_int, [ctypes.POINTER(EmbeddingArgs),
+                                        ctypes.POINTER(EmbeddingGrad), _vp]),
+    "rp_pack_check": (ctypes.c_int, [ctypes.POINTER(PackArgs)]),
+    "rp_pack": (ctypes.c_int, [ctypes.POINTER(PackArgs), _vp]),
+    "rp_unpack": (ctypes.c_int, [ctypes.POINTER(PackArgs), _vp]),
+    "rp_addnorm_check": (ctypes.c_int, [ctypes.POINTER(AddNormArgs)]),
+    "rp_addnorm_work_bytes": (_i64, [ctypes.POINTER(AddNormArgs)]),
+    "rp_addnorm_fwd": (ctypes.c_int, [ctypes.POINTER(AddNormArgs), _vp]),
+    "rp_addnorm_bwd": (ctypes.c_int, [ctypes.POINTER(AddNormArgs), ctypes.POINTER(AddNormGrad), _vp]),
+    "rp_gated_check": (ctypes.c_int, [ctypes.POINTER(GatedArgs)]),
+    "rp_gated_ckpt_bytes": (_i64, [ctypes.POINTER(GatedArgs)]),
+    "rp_gated_work_bytes": (_i64, [ctypes.POINTER(GatedArgs), ctypes.c_int]),
+    "rp_gated_fwd": (ctypes.c_int, [ctypes.POINTER(GatedArgs), _vp]),
+    "rp_gated_bwd": (ctypes.c_int, [ctypes.POINTER(GatedArgs), ctypes.POINTER(GatedGrad), _vp]),
     "rp_mixer_out_check": (ctypes.c_int, [ctypes.POINTER(MixerOutArgs)]),
     "rp_mixer_out_work_bytes": (_i64, [ctypes.POINTER(MixerOutArgs)]),
     "rp_mixer_out_fwd": (ctypes.c_int, [ctypes.POINTER(MixerOutArgs), _vp]),
@@ -270,6 +341,17 @@ def check(status, lib=None):
         lib = lib or _LIB
         msg = lib.rp_last_error().decode(errors="replace") if lib is not None else ""
         raise RuntimeError(f"redpanda_amd: status {status}: {msg}")
+
+
+def call(fn, device, *args):
+    """fn(*args, the device's current stream), made on that device."""
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        status = fn(*args, stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, stream_of(device))
+    if status != 0:
+        check(status)
 
 
 def ptr(t):

@@ -15,6 +15,7 @@
 #include "redpanda_hip.h"
 #include "rp_heads.h"
 #include "rp_launch.h"
+#include "rp_train.h"
 
 namespace {
 
@@ -1424,6 +1425,471 @@ int rp_layernorm_bwd(const rp_layernorm_args* a, const rp_layernorm_grad* g, voi
   lg.part = static_cast<float*>(g->work);
   hipError_t e = rp::launch_layernorm_bwd(layernorm_params(a), lg, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "layernorm bwd launch");
+  return RP_OK;
+}
+
+namespace {
+
+// A buffer of a call, for the checks that outputs overlap nothing.
+struct Span {
+  const void* p;
+  int64_t n;
+};
+
+int check_outputs(const Span* outs, int no, const Span* ins, int ni, const char* what) {
+  for (int i = 0; i < no; ++i) {
+    if (outs[i].p == nullptr || outs[i].n <= 0) continue;
+    for (int j = 0; j < ni; ++j)
+      if (ins[j].p && ins[j].n > 0 && overlaps(outs[i].p, outs[i].n, ins[j].p, ins[j].n))
+        return fail(RP_ERR_INVALID, "%s: an output overlaps an input", what);
+    for (int j = i + 1; j < no; ++j)
+      if (outs[j].p && outs[j].n > 0 && overlaps(outs[i].p, outs[i].n, outs[j].p, outs[j].n))
+        return fail(RP_ERR_INVALID, "%s: outputs overlap", what);
+  }
+  return RP_OK;
+}
+
+// Rows of a buffer that may not be the first of their call (whose sizes check_rows
+// has seen): given, aligned to their elements, and of a stride that holds them.
+bool good_rows(const void* p, int64_t rows, int64_t d, int64_t sr, int64_t es) {
+  return p != nullptr && aligned(p, es) && sr >= d && sr <= ((int64_t)1 << 60) / rows;
+}
+
+int check_work(const void* work, int64_t bytes, int64_t need, const char* what) {
+  if (need > 0 && (work == nullptr || bytes < need || !aligned(work, 256)))
+    return fail(RP_ERR_WORKSPACE, "%s: workspace needs %lld bytes (256-aligned), got %lld", what,
+                (long long)need, (long long)bytes);
+  return RP_OK;
+}
+
+}  // namespace
+
+int rp_embedding_check(const rp_embedding_args* a) {
+  if (a == nullptr) return fail(RP_ERR_INVALID, "embedding args: NULL");
+  if (a->N < 0 || a->V < 1 || a->d < 0)
+    return fail(RP_ERR_INVALID, "embedding args: N < 0, V < 1 or d < 0");
+  // (what the launches' grids and the 32-bit places hold)
+  if (a->N > ((int64_t)1 << 26) || a->V > ((int64_t)1 << 27) || a->d > ((int64_t)1 << 22))
+    return fail(RP_ERR_UNSUPPORTED, "embedding args: N up to 2^26, V up to 2^27, d up to 2^22");
+  if (!known_dtype(a->dtype_w) || !known_dtype(a->dtype_out))
+    return fail(RP_ERR_INVALID, "embedding args: unknown dtype code");
+  if (a->ids64 != 0 && a->ids64 != 1) return fail(RP_ERR_INVALID, "embedding args: ids64 must be 0 or 1");
+  if (a->N == 0 || a->d == 0) return RP_OK;
+  if (!a->ids || !aligned(a->ids, a->ids64 ? 8 : 4))
+    return fail(RP_ERR_INVALID, "embedding args: NULL or misaligned ids");
+  return RP_OK;
+}
+
+namespace {
+
+rp::EmbedParams embed_params(const rp_embedding_args* a) {
+  rp::EmbedParams p{};
+  p.N = a->N;
+  p.V = a->V;
+  p.d = a->d;
+  p.dt_w = a->dtype_w;
+  p.dt_out = a->dtype_out;
+  p.es_w = (int)elem_size(p.dt_w);
+  p.es_out = (int)elem_size(p.dt_out);
+  p.ids64 = a->ids64;
+  p.pad = a->padding;
+  p.scale = a->scale;
+  p.ids = a->ids;
+  p.w = a->w;
+  p.wsr = a->w_sr;
+  p.out = a->out;
+  return p;
+}
+
+struct EmbedWork {
+  int64_t start, place, sorted, part, bytes;
+};
+
+EmbedWork embed_work(const rp_embedding_args* a) {
+  EmbedWork w;
+  w.start = 0;
+  w.place = round_up((a->V + 1) * 4, 256);
+  w.sorted = w.place + round_up(a->N * 4, 256);
+  w.part = w.sorted + round_up(a->N * 4, 256);
+  w.bytes = w.part + round_up(rp::embed_chunks(a->N) * 2 * a->d * 4, 256);
+  return w;
+}
+
+}  // namespace
+
+int64_t rp_embedding_work_bytes(const rp_embedding_args* a) {
+  if (rp_embedding_check(a) != RP_OK) return -1;
+  return embed_work(a).bytes;
+}
+
+int rp_embedding_fwd(const rp_embedding_args* a, void* stream) {
+  int st = rp_embedding_check(a);
+  if (st != RP_OK || a->N == 0 || a->d == 0) return st;
+  const int64_t ew = elem_size(a->dtype_w), eo = elem_size(a->dtype_out);
+  if (!good_rows(a->w, a->V, a->d, a->w_sr, ew))
+    return fail(RP_ERR_INVALID, "embedding args: NULL or misaligned w, or a row stride below d");
+  if (!a->out || !aligned(a->out, eo))
+    return fail(RP_ERR_INVALID, "embedding args: NULL or misaligned out");
+  const Span out = {a->out, a->N * a->d * eo};
+  const Span ins[2] = {{a->w, rows_bytes(a->V, a->d, a->w_sr, ew)}, {a->ids, a->N * (a->ids64 ? 8 : 4)}};
+  st = check_outputs(&out, 1, ins, 2, "embedding args");
+  if (st != RP_OK) return st;
+  hipError_t e = rp::launch_embed_fwd(embed_params(a), (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "embedding fwd launch");
+  return RP_OK;
+}
+
+int rp_embedding_bwd(const rp_embedding_args* a, const rp_embedding_grad* g, void* stream) {
+  int st = rp_embedding_check(a);
+  if (st != RP_OK) return st;
+  if (g == nullptr) return fail(RP_ERR_INVALID, "embedding grad: NULL");
+  if (a->d == 0) return RP_OK;
+  const int64_t ew = elem_size(a->dtype_w), eo = elem_size(a->dtype_out);
+  if (!g->dw || !aligned(g->dw, ew))
+    return fail(RP_ERR_INVALID, "embedding grad: NULL or misaligned dw");
+  if (a->N > 0 && !good_rows(g->dout, a->N, a->d, g->dout_sr, eo))
+    return fail(RP_ERR_INVALID, "embedding grad: NULL or misaligned dout, or a row stride below d");
+  const EmbedWork at = embed_work(a);
+  st = check_work(g->work, g->work_bytes, at.bytes, "embedding bwd");
+  if (st != RP_OK) return st;
+  const Span outs[2] = {{g->dw, a->V * a->d * ew}, {g->work, at.bytes}};
+  const Span ins[2] = {{g->dout, a->N > 0 ? rows_bytes(a->N, a->d, g->dout_sr, eo) : 0},
+                       {a->ids, a->N * (a->ids64 ? 8 : 4)}};
+  st = check_outputs(outs, 2, ins, 2, "embedding grad");
+  if (st != RP_OK) return st;
+  rp::EmbedGrad eg{};
+  char* work = static_cast<char*>(g->work);
+  eg.dout = g->dout;
+  eg.dosr = g->dout_sr;
+  eg.dw = g->dw;
+  eg.start = reinterpret_cast<int32_t*>(work + at.start);
+  eg.place = reinterpret_cast<int32_t*>(work + at.place);
+  eg.sorted = reinterpret_cast<int32_t*>(work + at.sorted);
+  eg.part = reinterpret_cast<float*>(work + at.part);
+  hipError_t e = rp::launch_embed_bwd(embed_params(a), eg, (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "embedding bwd launch");
+  return RP_OK;
+}
+
+namespace {
+int64_t pack_exps(int64_t d) { return (d + 31) / 32; }
+}  // namespace
+
+int rp_pack_check(const rp_pack_args* a) {
+  if (a == nullptr) return fail(RP_ERR_INVALID, "pack args: NULL");
+  int st = check_rows(a->rows, a->d, a->x_sr, "pack");
+  if (st != RP_OK) return st;
+  if (!known_dtype(a->dtype)) return fail(RP_ERR_INVALID, "pack args: unknown dtype code %d", a->dtype);
+  if (a->rows == 0 || a->d == 0) return RP_OK;
+  if (!a->x || !a->q || !a->e || !aligned(a->x, elem_size(a->dtype)))
+    return fail(RP_ERR_INVALID, "pack args: NULL or misaligned pointer");
+  const Span all[3] = {{a->x, rows_bytes(a->rows, a->d, a->x_sr, elem_size(a->dtype))},
+                       {a->q, a->rows * a->d}, {a->e, a->rows * pack_exps(a->d)}};
+  return check_outputs(all, 3, nullptr, 0, "pack args");
+}
+
+namespace {
+rp::Pack8Params pack_params(const rp_pack_args* a) {
+  rp::Pack8Params p{};
+  p.rows = a->rows;
+  p.d = a->d;
+  p.dt = a->dtype;
+  p.es = (int)elem_size(a->dtype);
+  p.x = a->x;
+  p.xsr = a->x_sr;
+  p.q8 = a->q;
+  p.e8 = a->e;
+  return p;
+}
+}  // namespace
+
+int rp_pack(const rp_pack_args* a, void* stream) {
+  int st = rp_pack_check(a);
+  if (st != RP_OK) return st;
+  hipError_t e = rp::launch_pack8(pack_params(a), (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "pack launch");
+  return RP_OK;
+}
+
+int rp_unpack(const rp_pack_args* a, void* stream) {
+  int st = rp_pack_check(a);
+  if (st != RP_OK) return st;
+  if (a->x_sr != a->d) return fail(RP_ERR_INVALID, "unpack args: x must be contiguous");
+  hipError_t e = rp::launch_unpack8(pack_params(a), (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "unpack launch");
+  return RP_OK;
+}
+
+int rp_addnorm_check(const rp_addnorm_args* a) {
+  if (a == nullptr) return fail(RP_ERR_INVALID, "addnorm args: NULL");
+  int st = check_rows(a->rows, a->d, a->x ? a->x_sr : a->d, "addnorm");
+  if (st != RP_OK) return st;
+  if (a->d == 0) return fail(RP_ERR_INVALID, "addnorm args: rows of no elements have no mean");
+  if (!known_dtype(a->dtype_x) || !known_dtype(a->dtype_sum) || !known_dtype(a->dtype_out) ||
+      !known_dtype(a->dtype_add))
+    return fail(RP_ERR_INVALID, "addnorm args: unknown dtype code");
+  if (!(a->eps >= 0.f)) return fail(RP_ERR_INVALID, "addnorm args: eps must be >= 0");
+  if ((a->q == nullptr) != (a->e == nullptr))
+    return fail(RP_ERR_INVALID, "addnorm args: q and e go together");
+  if (!aligned(a->w, 4)) return fail(RP_ERR_INVALID, "addnorm args: misaligned pointer");
+  if (a->rows == 0) return RP_OK;
+  if (!a->x && !a->q) return fail(RP_ERR_INVALID, "addnorm args: neither x nor q");
+  return RP_OK;
+}
+
+namespace {
+rp::AddNormParams addnorm_params(const rp_addnorm_args* a) {
+  rp::AddNormParams p{};
+  p.rows = a->rows;
+  p.d = a->d;
+  p.dt_x = a->dtype_x;
+  p.dt_add = a->dtype_add;
+  p.dt_sum = a->dtype_sum;
+  p.dt_out = a->dtype_out;
+  p.es_x = (int)elem_size(p.dt_x);
+  p.es_add = (int)elem_size(p.dt_add);
+  p.es_sum = (int)elem_size(p.dt_sum);
+  p.es_out = (int)elem_size(p.dt_out);
+  p.eps = a->eps;
+  p.x = a->x;
+  p.xsr = a->x_sr;
+  p.add = a->add;
+  p.asr = a->add_sr;
+  p.w = a->w;
+  p.sum = a->sum;
+  p.out = a->out;
+  p.q8 = a->q;
+  p.e8 = a->e;
+  return p;
+}
+}  // namespace
+
+int64_t rp_addnorm_work_bytes(const rp_addnorm_args* a) {
+  if (rp_addnorm_check(a) != RP_OK) return -1;
+  return round_up(4 * rp::addnorm_work_floats(a->rows, a->d, a->x ? (int)elem_size(a->dtype_sum) : 1,
+                                              (int)elem_size(a->dtype_out)), 256);
+}
+
+int rp_addnorm_fwd(const rp_addnorm_args* a, void* stream) {
+  int st = rp_addnorm_check(a);
+  if (st != RP_OK || a->rows == 0) return st;
+  const int64_t n = a->rows * a->d, ne = a->rows * pack_exps(a->d);
+  const int64_t es = elem_size(a->dtype_sum), eo = elem_size(a->dtype_out);
+  if (!aligned(a->out, eo)) return fail(RP_ERR_INVALID, "addnorm args: misaligned out");
+  Span outs[4] = {{a->out, n * eo}, {nullptr, 0}, {nullptr, 0}, {nullptr, 0}};
+  Span ins[4] = {{a->w, a->d * 4}, {nullptr, 0}, {nullptr, 0}, {nullptr, 0}};
+  if (a->x) {
+    const int64_t ex = elem_size(a->dtype_x), ea = elem_size(a->dtype_add);
+    if (!aligned(a->x, ex)) return fail(RP_ERR_INVALID, "addnorm args: misaligned x");
+    if ((a->add == nullptr) != (a->sum == nullptr))
+      return fail(RP_ERR_INVALID, "addnorm args: add and sum go together");
+    if (!a->add && a->dtype_sum != a->dtype_x)
+      return fail(RP_ERR_INVALID, "addnorm args: without add the sum's type is x's");
+    if (a->add && (!good_rows(a->add, a->rows, a->d, a->add_sr, ea) || !aligned(a->sum, es)))
+      return fail(RP_ERR_INVALID, "addnorm args: add row stride shorter than d, or a misaligned pointer");
+    ins[1] = {a->x, rows_bytes(a->rows, a->d, a->x_sr, ex)};
+    if (a->add) ins[2] = {a->add, rows_bytes(a->rows, a->d, a->add_sr, ea)};
+    outs[1] = {a->sum, n * es};
+    outs[2] = {a->q, n};
+    outs[3] = {a->e, ne};
+  } else {
+    if (a->add || a->sum) return fail(RP_ERR_INVALID, "addnorm args: rows in 8 bits take no add or sum");
+    if (!a->out) return fail(RP_ERR_INVALID, "addnorm args: NULL out");
+    ins[1] = {a->q, n};
+    ins[2] = {a->e, ne};
+  }
+  st = check_outputs(outs, 4, ins, 4, "addnorm args");
+  if (st != RP_OK) return st;
+  hipError_t e = rp::launch_addnorm_fwd(addnorm_params(a), (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "addnorm fwd launch");
+  return RP_OK;
+}
+
+int rp_addnorm_bwd(const rp_addnorm_args* a, const rp_addnorm_grad* g, void* stream) {
+  int st = rp_addnorm_check(a);
+  if (st != RP_OK) return st;
+  if (g == nullptr) return fail(RP_ERR_INVALID, "addnorm grad: NULL");
+  if (!aligned(g->dw, 4)) return fail(RP_ERR_INVALID, "addnorm grad: misaligned dw");
+  const int64_t n = a->rows * a->d;
+  const int64_t ex = elem_size(a->dtype_x), ea = elem_size(a->dtype_add);
+  const int64_t es = elem_size(a->dtype_sum), eo = elem_size(a->dtype_out);
+  const int64_t need = rp_addnorm_work_bytes(a);
+  Span outs[4] = {{g->dx, n * ex}, {g->dadd, n * ea}, {g->dw, a->d * 4}, {nullptr, 0}};
+  Span ins[5] = {{a->w, a->d * 4}, {nullptr, 0}, {nullptr, 0}, {nullptr, 0}, {nullptr, 0}};
+  // (rows beyond the register shapes keep their r there whatever is asked for)
+  const bool work = g->dw != nullptr || (a->rows > 0 && need > 0 && a->d > 16384);
+  if (work) {
+    st = check_work(g->work, g->work_bytes, need, "addnorm bwd");
+    if (st != RP_OK) return st;
+    outs[3] = {g->work, need};
+  }
+  if (a->rows > 0) {
+    if (!good_rows(g->dout, a->rows, a->d, g->dout_sr, eo))
+      return fail(RP_ERR_INVALID, "addnorm grad: NULL or misaligned dout, or a row stride below d");
+    if (g->dsum && !good_rows(g->dsum, a->rows, a->d, g->dsum_sr, es))
+      return fail(RP_ERR_INVALID, "addnorm grad: misaligned dsum, or a row stride below d");
+    if (!aligned(g->dx, ex) || !aligned(g->dadd, ea) || (a->x && !aligned(a->x, es)))
+      return fail(RP_ERR_INVALID, "addnorm grad: misaligned pointer");
+    ins[1] = {g->dout, rows_bytes(a->rows, a->d, g->dout_sr, eo)};
+    if (g->dsum) ins[2] = {g->dsum, rows_bytes(a->rows, a->d, g->dsum_sr, es)};
+    if (a->x) {
+      ins[3] = {a->x, rows_bytes(a->rows, a->d, a->x_sr, es)};
+    } else {
+      ins[3] = {a->q, n};
+      ins[4] = {a->e, a->rows * pack_exps(a->d)};
+    }
+  }
+  st = check_outputs(outs, 4, ins, 5, "addnorm grad");
+  if (st != RP_OK) return st;
+  rp::AddNormGrad ag{};
+  ag.dout = g->dout;
+  ag.dosr = g->dout_sr;
+  ag.dsum = g->dsum;
+  ag.dssr = g->dsum_sr;
+  ag.dx = g->dx;
+  ag.dadd = g->dadd;
+  ag.dw = g->dw;
+  ag.part = static_cast<float*>(g->work);
+  hipError_t e = rp::launch_addnorm_bwd(addnorm_params(a), ag, (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "addnorm bwd launch");
+  return RP_OK;
+}
+
+namespace {
+
+// Whether (B, L, D) with these strides is a buffer whose offsets stay in int64.
+bool good_strides(const rp_gated_args* a, int64_t sb, int64_t sl) {
+  return sb >= 0 && sl >= a->D && sl <= ((int64_t)1 << 58) / (a->L > 0 ? a->L : 1) &&
+         sb <= ((int64_t)1 << 58) / (a->B > 0 ? a->B : 1);
+}
+
+int64_t seq_bytes(const rp_gated_args* a, int64_t sb, int64_t sl, int64_t es) {
+  return ((a->B - 1) * sb + (a->L - 1) * sl + a->D) * es;
+}
+
+rp::GatedParams gated_params(const rp_gated_args* a) {
+  rp::GatedParams p{};
+  p.B = a->B;
+  p.L = a->L;
+  p.D = a->D;
+  p.dt = a->dtype;
+  p.es = (int)elem_size(a->dtype);
+  p.x = a->x;
+  p.xsb = a->x_sb;
+  p.xsl = a->x_sl;
+  p.g = a->gate;
+  p.gsb = a->gate_sb;
+  p.gsl = a->gate_sl;
+  p.h0 = a->h0;
+  p.starts = a->starts;
+  p.ssb = a->starts_sb;
+  p.y = a->y;
+  p.h_last = a->h_last;
+  p.ckpt = a->ckpt;
+  p.agg = static_cast<float*>(a->work);
+  return p;
+}
+
+// (before the first use of a->y and the gradients)
+int check_gated_inputs(const rp_gated_args* a) {
+  const int64_t es = elem_size(a->dtype);
+  if (!a->x || !a->gate || !aligned(a->x, es) || !aligned(a->gate, es))
+    return fail(RP_ERR_INVALID, "gated args: NULL or misaligned x / gate");
+  if (!good_strides(a, a->x_sb, a->x_sl) || !good_strides(a, a->gate_sb, a->gate_sl))
+    return fail(RP_ERR_INVALID, "gated args: a stride of x or gate is negative, below D or too large");
+  if (!aligned(a->h0, 4) || !aligned(a->h_last, 4) || !aligned(a->ckpt, 4))
+    return fail(RP_ERR_INVALID, "gated args: misaligned pointer");
+  if (a->starts && (a->starts_sb < 0 || a->starts_sb > ((int64_t)1 << 58) / a->B))
+    return fail(RP_ERR_INVALID, "gated args: bad batch stride of starts");
+  return RP_OK;
+}
+
+}  // namespace
+
+int rp_gated_check(const rp_gated_args* a) {
+  if (a == nullptr) return fail(RP_ERR_INVALID, "gated args: NULL");
+  if (a->B < 0 || a->L < 0 || a->D < 0) return fail(RP_ERR_INVALID, "gated args: negative size");
+  if (a->B > kI32Max || a->L > kI32Max || a->D > kI32Max)
+    return fail(RP_ERR_UNSUPPORTED, "gated args: sizes must fit in int32");
+  if (!known_dtype(a->dtype)) return fail(RP_ERR_INVALID, "gated args: unknown dtype code %d", a->dtype);
+  if (a->B == 0 || a->L == 0 || a->D == 0) return RP_OK;
+  // (the launches hold a wave for each 64 to 256 channels of a sequence's chunk)
+  if (a->B > ((int64_t)1 << 25) / ((a->D + 63) / 64) || a->L > ((int64_t)1 << 50) / a->D / a->B)
+    return fail(RP_ERR_UNSUPPORTED, "gated args: too many channels or elements");
+  return RP_OK;
+}
+
+int64_t rp_gated_ckpt_bytes(const rp_gated_args* a) {
+  if (rp_gated_check(a) != RP_OK) return -1;
+  return a->B * ((a->L + rp::kGatedK - 1) / rp::kGatedK) * a->D * 4;
+}
+
+int64_t rp_gated_work_bytes(const rp_gated_args* a, int backward) {
+  if (rp_gated_check(a) != RP_OK) return -1;
+  if (a->B == 0 || a->L == 0 || a->D == 0) return 0;
+  rp::GatedParams p = gated_params(a);
+  return round_up(4 * rp::gated_plan(&p, backward != 0), 256);
+}
+
+int rp_gated_fwd(const rp_gated_args* a, void* stream) {
+  int st = rp_gated_check(a);
+  if (st != RP_OK || a->B == 0 || a->L == 0 || a->D == 0) return st;
+  st = check_gated_inputs(a);
+  if (st != RP_OK) return st;
+  const int64_t es = elem_size(a->dtype), m = a->B * a->D * 4;
+  if (!a->y || !aligned(a->y, es)) return fail(RP_ERR_INVALID, "gated args: NULL or misaligned y");
+  rp::GatedParams p = gated_params(a);
+  const int64_t need = round_up(4 * rp::gated_plan(&p, false), 256);
+  st = check_work(a->work, a->work_bytes, need, "gated fwd");
+  if (st != RP_OK) return st;
+  const Span outs[4] = {{a->y, a->B * a->L * a->D * es}, {a->h_last, m},
+                        {a->ckpt, rp_gated_ckpt_bytes(a)}, {a->work, need}};
+  const Span ins[4] = {{a->x, seq_bytes(a, a->x_sb, a->x_sl, es)},
+                       {a->gate, seq_bytes(a, a->gate_sb, a->gate_sl, es)}, {a->h0, m},
+                       {a->starts, (a->B - 1) * a->starts_sb + a->L}};
+  st = check_outputs(outs, 4, ins, 4, "gated args");
+  if (st != RP_OK) return st;
+  hipError_t e = rp::launch_gated_fwd(p, (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "gated fwd launch");
+  return RP_OK;
+}
+
+int rp_gated_bwd(const rp_gated_args* a, const rp_gated_grad* g, void* stream) {
+  int st = rp_gated_check(a);
+  if (st != RP_OK) return st;
+  if (g == nullptr) return fail(RP_ERR_INVALID, "gated grad: NULL");
+  if (a->B == 0 || a->L == 0 || a->D == 0) return RP_OK;
+  st = check_gated_inputs(a);
+  if (st != RP_OK) return st;
+  const int64_t es = elem_size(a->dtype), n = a->B * a->L * a->D * es, m = a->B * a->D * 4;
+  if (!a->ckpt) return fail(RP_ERR_INVALID, "gated grad: the forward's ckpt is needed");
+  if (!g->dx || !g->dgate || !aligned(g->dx, es) || !aligned(g->dgate, es) || !aligned(g->dy, es) ||
+      !aligned(g->dh_last, 4) || !aligned(g->dh0, 4))
+    return fail(RP_ERR_INVALID, "gated grad: NULL dx / dgate, or a misaligned pointer");
+  if (g->dy && !good_strides(a, g->dy_sb, g->dy_sl))
+    return fail(RP_ERR_INVALID, "gated grad: a stride of dy is negative, below D or too large");
+  rp::GatedParams p = gated_params(a);
+  const int64_t need = round_up(4 * rp::gated_plan(&p, true), 256);
+  st = check_work(a->work, a->work_bytes, need, "gated bwd");
+  if (st != RP_OK) return st;
+  const Span outs[4] = {{g->dx, n}, {g->dgate, n}, {g->dh0, m}, {a->work, need}};
+  const Span ins[6] = {{a->x, seq_bytes(a, a->x_sb, a->x_sl, es)},
+                       {a->gate, seq_bytes(a, a->gate_sb, a->gate_sl, es)},
+                       {a->starts, (a->B - 1) * a->starts_sb + a->L},
+                       {g->dy, g->dy ? seq_bytes(a, g->dy_sb, g->dy_sl, es) : 0}, {g->dh_last, m},
+                       {a->ckpt, rp_gated_ckpt_bytes(a)}};
+  st = check_outputs(outs, 4, ins, 6, "gated grad");
+  if (st != RP_OK) return st;
+  rp::GatedGrad gg{};
+  gg.dy = g->dy;
+  gg.dysb = g->dy_sb;
+  gg.dysl = g->dy_sl;
+  gg.dh = g->dh_last;
+  gg.dx = g->dx;
+  gg.dg = g->dgate;
+  gg.dh0 = g->dh0;
+  hipError_t e = rp::launch_gated_bwd(p, gg, (hipStream_t)stream);
+  if (e != hipSuccess) return fail_hip(e, "gated bwd launch");
   return RP_OK;
 }
 

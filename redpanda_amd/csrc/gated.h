@@ -1,0 +1,128 @@
+// What the gated recurrence's passes share (the mathematics is in gated_fwd.hip).
+//
+// A wave takes 64 V adjacent channels of one sequence, V a lane, and walks a stretch
+// of its steps; its last lane's channels are moved back to end with the row, so that
+// every access is a whole vector (channels in two lanes get the same values twice).
+#pragma once
+
+#include "rp_rows.h"
+#include "rp_train.h"
+
+namespace rp {
+
+// V adjacent elements as stored.
+template <int ES, int V>
+struct GatedRaw {
+  static constexpr int kWords = ES * V >= 4 ? ES * V / 4 : 1;
+  uint32_t w[kWords];
+};
+
+template <int ES, int V>
+__device__ __forceinline__ GatedRaw<ES, V> gated_load(const char* p) {
+  GatedRaw<ES, V> r;
+  if constexpr (ES * V == 2) {
+    r.w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else if constexpr (ES * V == 4) {
+    typedef uint32_t u32_any __attribute__((aligned(1)));
+    r.w[0] = *reinterpret_cast<const u32_any*>(p);
+  } else if constexpr (ES * V == 8) {
+    const u32x2_any v = *reinterpret_cast<const u32x2_any*>(p);
+    r.w[0] = v[0];
+    r.w[1] = v[1];
+  } else {
+    const u32x4_any v = *reinterpret_cast<const u32x4_any*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = v[i];
+  }
+  return r;
+}
+
+template <int ES, int V>
+__device__ __forceinline__ float gated_value(const GatedRaw<ES, V>& r, int i, int dtype) {
+  if constexpr (ES == 4) {
+    return __uint_as_float(r.w[i]);
+  } else {
+    if (dtype == RP_BF16)
+      return __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
+    return static_cast<float>(
+        __builtin_bit_cast(_Float16, static_cast<uint16_t>(r.w[i / 2] >> (16 * (i & 1)))));
+  }
+}
+
+template <int ES, int V>
+__device__ __forceinline__ void gated_store(char* p, const float (&v)[V], int dtype) {
+  if constexpr (ES == 4) {
+    if constexpr (V == 4) {
+      u32x4_any w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
+      *reinterpret_cast<u32x4_any*>(p) = w;
+    } else if constexpr (V == 2) {
+      u32x2_any w;
+      w[0] = __float_as_uint(v[0]);
+      w[1] = __float_as_uint(v[1]);
+      *reinterpret_cast<u32x2_any*>(p) = w;
+    } else {
+      *reinterpret_cast<float*>(p) = v[0];
+    }
+  } else if constexpr (V == 4) {
+    u32x2_any w;
+    w[0] = pack16(v[0], v[1], dtype);
+    w[1] = pack16(v[2], v[3], dtype);
+    *reinterpret_cast<u32x2_any*>(p) = w;
+  } else if constexpr (V == 2) {
+    typedef uint32_t u32_any __attribute__((aligned(1)));
+    *reinterpret_cast<u32_any*>(p) = pack16(v[0], v[1], dtype);
+  } else {
+    *reinterpret_cast<uint16_t*>(p) = (uint16_t)pack16(v[0], 0.f, dtype);
+  }
+}
+
+// a = 1 / (1 + exp(-z)) and 1 - a, both to full relative accuracy: of exp(-|z|) / (1 +
+// exp(-|z|)) and 1 / (1 + exp(-|z|)) each is the one or the other.
+__device__ __forceinline__ void gate_of(float z, float& a, float& na) {
+  const float e = exp2_hw(fabsf(z) * -kLog2e);
+  const float big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;
+  a = z >= 0.f ? big : small;
+  na = z >= 0.f ? small : big;
+}
+
+// Which of the `n` steps (up to 16) from t on begin a sequence, a bit each, the same in
+// every lane.
+__device__ __forceinline__ uint32_t start_bits(const GatedParams& p, int64_t b, int64_t t, int n) {
+  if (p.starts == nullptr) return 0;
+  const int lane = threadIdx.x % kWave;
+  return (uint32_t)__ballot(lane < n && p.starts[b * p.ssb + t + (lane < n ? lane : 0)] != 0);
+}
+
+// A wave's place: its sequence, its time chunk and its lane's first channel.
+template <int V>
+struct GatedAt {
+  int64_t b, c, ch, t0, t1;
+  __device__ __forceinline__ GatedAt(const GatedParams& p) {
+    const uint32_t tiles = (uint32_t)((p.D + kWave * V - 1) / (kWave * V));
+    const uint32_t rest = blockIdx.x / tiles, tile = blockIdx.x - rest * tiles;
+    b = rest / (uint32_t)p.nchunk;
+    c = rest - (uint32_t)b * (uint32_t)p.nchunk;
+    ch = ((int64_t)tile * kWave + threadIdx.x) * V;
+    if (ch > p.D - V) ch = p.D - V;
+    t0 = c * p.chunk;
+    t1 = t0 + p.chunk < p.L ? t0 + p.chunk : p.L;
+  }
+};
+
+// (product of the gates, end) of a chunk that anything may enter: a chunk in which a
+// sequence begins has the product -0, and passes nothing on, not even an infinity.
+__device__ __forceinline__ float gated_join(float prod, float end, float in) {
+  return __float_as_uint(prod) == 0x80000000u ? end : ffma(prod, in, end);
+}
+
+// Channels a lane takes.
+inline int gated_lane_channels(int64_t B, int64_t D, bool backward) {
+  if (D >= 4 && !backward && B * ((D + 4 * kWave - 1) / (4 * kWave)) >= 512) return 4;
+  return D >= 2 ? 2 : 1;
+}
+
+hipError_t launch_gated_fold(const GatedParams& p, const float* in, bool backward, hipStream_t st);
+
+}  // namespace rp

@@ -13,6 +13,7 @@ namespace rp {
 // accesses at any byte address, and a row of odd length puts every other row's
 // start off a vector boundary.
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 
 // Eight elements as stored: 8 words of fp32, or 4 words of two 16-bit values.
 template <int ES>

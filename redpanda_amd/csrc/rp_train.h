@@ -1,0 +1,116 @@
+// Parameter blocks and host-side launchers of the training operators: embedding,
+// RMS norm with the residual's addition, checkpoints in 8 bits, and the gated
+// recurrence (internal to the library).
+#pragma once
+
+#include "rp_launch.h"
+
+namespace rp {
+
+// Embedding (embedding.hip).
+struct EmbedParams {
+  int64_t N, V, d;
+  int dt_w, dt_out, es_w, es_out;
+  int ids64;        // ids are int64, else int32
+  int64_t pad;      // an id whose row gets no gradient, or -1
+  float scale;
+  const void* ids;  // (N,)
+  const void* w;    // (V, d), row stride wsr
+  int64_t wsr;
+  void* out;        // (N, d) contiguous
+};
+
+struct EmbedGrad {
+  const void* dout;  // (N, d) in dt_out, row stride dosr
+  int64_t dosr;
+  void* dw;          // (V, d) contiguous in dt_w
+  int32_t* start;    // (V + 1,) workspace: where each id's places begin in `place`
+  int32_t* place;    // (N,) workspace: the places 0 .. N - 1 in order of their ids
+  int32_t* sorted;   // (N,) workspace: the ids in order
+  float* part;       // (chunks, 2, d) workspace
+};
+
+int64_t embed_chunks(int64_t N);
+hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st);
+hipError_t launch_embed_bwd(const EmbedParams& p, const EmbedGrad& g, hipStream_t st);
+
+// RMS norm with the residual's addition (addnorm.hip).
+struct AddNormParams {
+  int64_t rows, d;
+  int dt_x, dt_add, dt_sum, dt_out;
+  int es_x, es_add, es_sum, es_out;
+  float eps;
+  const void* x;    // (rows, d), row stride xsr; null: the rows are held in q8, e8
+  int64_t xsr;
+  const void* add;  // (rows, d) or null, row stride asr
+  int64_t asr;
+  const float* w;   // (d,) or null
+  void* sum;        // (rows, d) contiguous in dt_sum, or null
+  void* out;        // (rows, d) contiguous, or null
+  int8_t* q8;       // (rows, d) and (rows, ceil(d / 32)): the sum in 8 bits
+  uint8_t* e8;      //   (written where x is given, read where it is not), or null
+};
+
+struct AddNormGrad {
+  const void* dout;  // (rows, d) in dt_out, row stride dosr
+  int64_t dosr;
+  const void* dsum;  // (rows, d) in dt_sum or null, row stride dssr
+  int64_t dssr;
+  void* dx;          // (rows, d) contiguous in dt_x, or null
+  void* dadd;        // (rows, d) contiguous in dt_add, or null
+  float* dw;         // (d,), or null
+  float* part;       // addnorm_work_floats of workspace
+};
+
+// Floats of workspace that a backward needs (es_s: bytes of an
+// element of the rows it reads, 1 for those in 8 bits).
+int64_t addnorm_work_floats(int64_t rows, int64_t d, int es_s, int es_out);
+hipError_t launch_addnorm_fwd(const AddNormParams& p, hipStream_t st);
+// The backward's rows are p.x (row stride p.xsr, in dt_sum), or p.q8 and p.e8.
+hipError_t launch_addnorm_bwd(const AddNormParams& p, const AddNormGrad& g, hipStream_t st);
+
+// Rows in 8 bits (pack8.hip).
+struct Pack8Params {
+  int64_t rows, d;
+  int dt, es;
+  void* x;       // (rows, d), row stride xsr; read by the pack, written by the unpack
+  int64_t xsr;
+  int8_t* q8;    // (rows, d) contiguous
+  uint8_t* e8;   // (rows, ceil(d / 32))
+};
+hipError_t launch_pack8(const Pack8Params& p, hipStream_t st);
+hipError_t launch_unpack8(const Pack8Params& p, hipStream_t st);
+
+// Gated linear recurrence (gated_fwd.hip, gated_bwd.hip).
+constexpr int kGatedK = 16;  // steps between the states that the backward starts from
+struct GatedParams {
+  int64_t B, L, D;
+  int dt, es;
+  const void* x;     // (B, L, D), strides xsb, xsl
+  int64_t xsb, xsl;
+  const void* g;     // the gates, likewise
+  int64_t gsb, gsl;
+  const float* h0;   // (B, D) or null
+  const uint8_t* starts;  // (B, L), batch stride ssb, or null
+  int64_t ssb;
+  void* y;           // (B, L, D) contiguous
+  float* h_last;     // (B, D) or null
+  float* ckpt;       // (B, ceil(L / kGatedK), D) or null: the state before every 16th step
+  float* agg;        // workspace of gated_work_floats
+  int nchunk;        // time chunks, each of `chunk` steps (a multiple of kGatedK)
+  int64_t chunk;
+};
+struct GatedGrad {
+  const void* dy;    // (B, L, D) or null, strides dysb, dysl
+  int64_t dysb, dysl;
+  const float* dh;   // (B, D) or null: the gradient of the last state
+  void* dx;          // (B, L, D) contiguous each
+  void* dg;
+  float* dh0;        // (B, D) or null
+};
+// Sets p.nchunk and p.chunk; the floats of workspace that p.agg needs.
+int64_t gated_plan(GatedParams* p, bool backward);
+hipError_t launch_gated_fwd(const GatedParams& p, hipStream_t st);
+hipError_t launch_gated_bwd(const GatedParams& p, const GatedGrad& g, hipStream_t st);
+
+}  // namespace rp

@@ -87,8 +87,8 @@ def once(backward):
     less of a small call) where not."""
     marked = once_differentiable(backward)
 
-    def run(ctx, grad):
-        return marked(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+    def run(ctx, *grads):
+        return marked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
 

@@ -19,7 +19,9 @@ What differs is where the selective scan and the O(1) step run:
     (SearchMamba.dynamics_rollout trains through step) it runs the scan
     kernel with L = 1 from the cached state, whose analytic backward carries
     gradients into the previous state.
-Projections, norms and the residual stack stay plain torch (GEMMs).  There is
+Projections, norms and the residual stack stay plain torch (GEMMs); with fused=True
+Mamba.forward runs the embedding, the residual additions and the norms on HIP
+kernels too.  There is
 no PyTorch fallback for the SSM core: device tensors on a ROCm GPU are
 required, and a missing library raises.  `use_triton_scan` is accepted for
 config compatibility; the HIP path does not depend on it.
@@ -35,9 +37,11 @@ import torch.utils.checkpoint
 
 from redpanda_amd import layer_step
 from redpanda_amd.bcnorm import hip_bcnorm_psum
+from redpanda_amd.checkpoint8 import hip_checkpoint8
 from redpanda_amd.dropout import hip_dropout
+from redpanda_amd.embedding import hip_embedding
 from redpanda_amd.mixer import hip_mixer_out
-from redpanda_amd.norm import hip_add_rmsnorm
+from redpanda_amd.norm import hip_add_rmsnorm, hip_rmsnorm
 from redpanda_amd.scan import hip_scan_with_state, hip_trapezoidal_scan
 from redpanda_amd.step import compact_beta, full_beta, hip_softplus, hip_step, is_compact
 
@@ -374,13 +378,24 @@ class Mamba(nn.Module):
         elif isinstance(module, nn.Embedding):
             nn.init.normal_(module.weight, mean=0.0, std=0.02)
 
-    def forward(self, input_ids, input_embeds=None, dropout=0.0, seed=None):
+    def forward(self, input_ids, input_embeds=None, dropout=0.0, seed=None, fused=False,
+                embed_scale=1.0, keep8=False):
         """(B, L) ids or (B, L, d_model) embeddings -> (B, L, d_model).
         dropout > 0: each layer's branch is dropped out with the residual added
         in the same pass (hip_dropout with `seed`, the layer's index as its
         stream: a seed of its own for each call, since SearchMamba's heads count
         their streams from 0, too), for training, but wherever it is asked for:
-        self.training is not looked at; 0 adds the branch as it is."""
+        self.training is not looked at; 0 adds the branch as it is.
+        fused: the embedding (times embed_scale, with its gradient in a fixed order) and
+        each residual addition with the norm behind it run on the HIP kernels, one pass
+        each way, where torch takes one for each operation; the norm's result is in the
+        dtype that in_proj reads it in.  keep8 (fused too): each layer is checkpointed
+        with its input in 8 bits (hip_checkpoint8), whatever grad_checkpoint says: the
+        output is the same, the gradients are those at the kept values."""
+        if fused or keep8:
+            return self._forward_fused(input_ids, input_embeds, dropout, seed, embed_scale, keep8)
+        if embed_scale != 1.0:
+            raise ValueError("Mamba.forward: embed_scale needs fused=True (the plain path has no scale)")
         x = input_embeds if input_embeds is not None else self.embedding(input_ids)
         for i, layer in enumerate(self.layers):
             mixer, norm = layer["mixer"], layer["norm"]
@@ -399,6 +414,31 @@ class Mamba(nn.Module):
             else:
                 x = x + mixer(norm(x))
         return self.norm_f(x)
+
+    def _forward_fused(self, input_ids, input_embeds, dropout, seed, embed_scale, keep8):
+        x = input_embeds
+        if x is None:
+            x = hip_embedding(input_ids, self.embedding.weight, scale=embed_scale)
+        branch, dtype = None, _gate_out_dtype()
+        for i, layer in enumerate(self.layers):
+            mixer, norm = layer["mixer"], layer["norm"]
+            if keep8:
+                got = hip_checkpoint8(mixer, x, norm.weight, norm.eps, add=branch, out_dtype=dtype,
+                                      params=mixer.parameters())
+                x, out = (x, got) if branch is None else got
+            else:
+                got = hip_rmsnorm(x, norm.weight, norm.eps, add=branch, out_dtype=dtype)
+                x, normed = (x, got) if branch is None else got
+                if self.grad_checkpoint and self.training and normed.requires_grad:
+                    out = torch.utils.checkpoint.checkpoint(mixer, normed, use_reentrant=False)
+                else:
+                    out = mixer(normed)
+            if dropout:
+                x, branch = hip_dropout(out, dropout, seed, residual=x, stream=i), None
+            else:
+                branch = out  # added with the next norm
+        got = hip_rmsnorm(x, self.norm_f.weight, self.norm_f.eps, add=branch)
+        return got if branch is None else got[1]
 
     def init_cache(self, batch_size, device):
         """An empty per-layer cache (engine/mamba.py:560-562)."""

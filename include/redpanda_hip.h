@@ -626,7 +626,7 @@ int rp_addnorm_bwd(const rp_addnorm_args* a, const rp_addnorm_grad* g, void* str
  * h0: (B, D) fp32; starts: NULL or (B, L) bytes with batch stride starts_sb and unit
  * stride along L; y: (B, L, D) contiguous in dtype; h_last: NULL or (B, D) fp32;
  * ckpt: NULL, or rp_gated_ckpt_bytes() for a later backward.  The state is fp32
- * throughout.  work: rp_gated_work_bytes(a, 0) of scratch, 256-byte aligned: few
+ * throughout.  work: rp_gated_work_bytes() of scratch, 256-byte aligned: few
  * channels of a long sequence are split along it.
  */
 typedef struct rp_gated_args {
@@ -649,7 +649,8 @@ typedef struct rp_gated_args {
  *     dx_t = (1 - a_t) dh_t,  dgate_t = (h_{t-1} - x_t) a_t (1 - a_t) dh_t
  * dy: NULL or (B, L, D) in dtype with strides; dh_last: NULL or (B, D); dx, dgate:
  * (B, L, D) contiguous in dtype; dh0: NULL or (B, D) fp32.  a->ckpt: what the forward
- * wrote; a->y and a->h_last are not read.  a->work: rp_gated_work_bytes(a, 1).
+ * wrote; a->y and a->h_last are not read.  a->work: as the
+ * forward's.
  */
 typedef struct rp_gated_grad {
   const void* dy;  int64_t dy_sb, dy_sl;
@@ -661,7 +662,8 @@ typedef struct rp_gated_grad {
 
 int rp_gated_check(const rp_gated_args* a);
 int64_t rp_gated_ckpt_bytes(const rp_gated_args* a);
-int64_t rp_gated_work_bytes(const rp_gated_args* a, int backward);
+/* Bytes of scratch that rp_gated_fwd and rp_gated_bwd need, each. */
+int64_t rp_gated_work_bytes(const rp_gated_args* a);
 int rp_gated_fwd(const rp_gated_args* a, void* stream);
 int rp_gated_bwd(const rp_gated_args* a, const rp_gated_grad* g, void* stream);
 

@@ -277,7 +277,7 @@ SIGNATURES = {
     "rp_addnorm_bwd": (ctypes.c_int, [ctypes.POINTER(AddNormArgs), ctypes.POINTER(AddNormGrad), _vp]),
     "rp_gated_check": (ctypes.c_int, [ctypes.POINTER(GatedArgs)]),
     "rp_gated_ckpt_bytes": (_i64, [ctypes.POINTER(GatedArgs)]),
-    "rp_gated_work_bytes": (_i64, [ctypes.POINTER(GatedArgs), ctypes.c_int]),
+    "rp_gated_work_bytes": (_i64, [ctypes.POINTER(GatedArgs)]),
     "rp_gated_fwd": (ctypes.c_int, [ctypes.POINTER(GatedArgs), _vp]),
     "rp_gated_bwd": (ctypes.c_int, [ctypes.POINTER(GatedArgs), ctypes.POINTER(GatedGrad), _vp]),
     "rp_mixer_out_check": (ctypes.c_int, [ctypes.POINTER(MixerOutArgs)]),

@@ -1824,11 +1824,11 @@ int64_t rp_gated_ckpt_bytes(const rp_gated_args* a) {
   return a->B * ((a->L + rp::kGatedK - 1) / rp::kGatedK) * a->D * 4;
 }
 
-int64_t rp_gated_work_bytes(const rp_gated_args* a, int backward) {
+int64_t rp_gated_work_bytes(const rp_gated_args* a) {
   if (rp_gated_check(a) != RP_OK) return -1;
   if (a->B == 0 || a->L == 0 || a->D == 0) return 0;
   rp::GatedParams p = gated_params(a);
-  return round_up(4 * rp::gated_plan(&p, backward != 0), 256);
+  return round_up(4 * rp::gated_plan(&p), 256);
 }
 
 int rp_gated_fwd(const rp_gated_args* a, void* stream) {
@@ -1839,7 +1839,7 @@ int rp_gated_fwd(const rp_gated_args* a, void* stream) {
   const int64_t es = elem_size(a->dtype), m = a->B * a->D * 4;
   if (!a->y || !aligned(a->y, es)) return fail(RP_ERR_INVALID, "gated args: NULL or misaligned y");
   rp::GatedParams p = gated_params(a);
-  const int64_t need = round_up(4 * rp::gated_plan(&p, false), 256);
+  const int64_t need = round_up(4 * rp::gated_plan(&p), 256);
   st = check_work(a->work, a->work_bytes, need, "gated fwd");
   if (st != RP_OK) return st;
   const Span outs[4] = {{a->y, a->B * a->L * a->D * es}, {a->h_last, m},
@@ -1869,7 +1869,7 @@ int rp_gated_bwd(const rp_gated_args* a, const rp_gated_grad* g, void* stream) {
   if (g->dy && !good_strides(a, g->dy_sb, g->dy_sl))
     return fail(RP_ERR_INVALID, "gated grad: a stride of dy is negative, below D or too large");
   rp::GatedParams p = gated_params(a);
-  const int64_t need = round_up(4 * rp::gated_plan(&p, true), 256);
+  const int64_t need = round_up(4 * rp::gated_plan(&p), 256);
   st = check_work(a->work, a->work_bytes, need, "gated bwd");
   if (st != RP_OK) return st;
   const Span outs[4] = {{g->dx, n}, {g->dgate, n}, {g->dh0, m}, {a->work, need}};

@@ -1,8 +1,9 @@
 // What the gated recurrence's passes share (the mathematics is in gated_fwd.hip).
 //
-// A wave takes 64 V adjacent channels of one sequence, V a lane, and walks a stretch
-// of its steps; its last lane's channels are moved back to end with the row, so that
-// every access is a whole vector (channels in two lanes get the same values twice).
+// A workgroup takes 64 V adjacent channels of one sequence, V a lane, and a chunk of its
+// steps, NW waves times 16 steps at a time, each wave the 16 behind those of the wave
+// before it.  A row's last lanes take channels that end with the row, so that every
+// access is a whole vector (channels in two lanes get the same values twice).
 #pragma once
 
 #include "rp_rows.h"
@@ -95,7 +96,7 @@ __device__ __forceinline__ uint32_t start_bits(const GatedParams& p, int64_t b, 
   return (uint32_t)__ballot(lane < n && p.starts[b * p.ssb + t + (lane < n ? lane : 0)] != 0);
 }
 
-// A wave's place: its sequence, its time chunk and its lane's first channel.
+// A workgroup's place: its sequence, its time chunk and its lanes' first channels.
 template <int V>
 struct GatedAt {
   int64_t b, c, ch, t0, t1;
@@ -104,25 +105,37 @@ struct GatedAt {
     const uint32_t rest = blockIdx.x / tiles, tile = blockIdx.x - rest * tiles;
     b = rest / (uint32_t)p.nchunk;
     c = rest - (uint32_t)b * (uint32_t)p.nchunk;
-    ch = ((int64_t)tile * kWave + threadIdx.x) * V;
+    ch = ((int64_t)tile * kWave + threadIdx.x % kWave) * V;
     if (ch > p.D - V) ch = p.D - V;
     t0 = c * p.chunk;
     t1 = t0 + p.chunk < p.L ? t0 + p.chunk : p.L;
   }
 };
 
-// (product of the gates, end) of a chunk that anything may enter: a chunk in which a
-// sequence begins has the product -0, and passes nothing on, not even an infinity.
+// The (product of the gates, end from 0) of a stretch, applied to what enters it.  A
+// stretch in which a sequence begins has the product -0 and passes nothing on, not even
+// an infinity.
 __device__ __forceinline__ float gated_join(float prod, float end, float in) {
   return __float_as_uint(prod) == 0x80000000u ? end : ffma(prod, in, end);
 }
-
-// Channels a lane takes.
-inline int gated_lane_channels(int64_t B, int64_t D, bool backward) {
-  if (D >= 4 && !backward && B * ((D + 4 * kWave - 1) / (4 * kWave)) >= 512) return 4;
-  return D >= 2 ? 2 : 1;
+// And of two stretches, one behind the other.
+__device__ __forceinline__ float gated_product(float first, float second) {
+  const float p = first * second;
+  return __float_as_uint(first) == 0x80000000u || __float_as_uint(second) == 0x80000000u ? -0.f : p;
 }
 
+// What the waves of a workgroup know of their stretches.
+template <int V, int NW>
+struct GatedShare {
+  float prod[2][NW][kWave * V];
+  float end[2][NW][kWave * V];
+};
+
+// Channels a lane takes: four bytes of them.
+inline int gated_lane_channels(int es, int64_t D) { return es == 2 && D >= 2 ? 2 : 1; }
+
 hipError_t launch_gated_fold(const GatedParams& p, const float* in, bool backward, hipStream_t st);
+
+#define RP_GATED_WAVES(X) X(1) X(2) X(4) X(8) X(16)
 
 }  // namespace rp

@@ -3,25 +3,28 @@
 // h_t = a_t h_{t-1} + (1 - a_t) x_t:
 //     dx_t = (1 - a_t) l_t,   dz_t = (h_{t-1} - x_t) a_t (1 - a_t) l_t
 // The states are computed again, 16 steps at a time from the forward's checkpoints (a
-// sixteenth of the states, in fp32), so that only x, z and dy are read; the gates and
-// states of 16 steps stay in registers between the way there and the way back.  The
-// time axis is split as in the forward.
+// sixteenth of the states, in fp32), so that only x, z and dy are read.  As in the
+// forward the waves of a workgroup stand one behind the other in time, and the time
+// axis is split among workgroups where there are few.
 
 #include "gated.h"
 
 namespace rp {
 
-template <int ES, int V, bool kWhole>
-__global__ __launch_bounds__(kWave) void gated_bwd_kernel(GatedParams p, GatedGrad d) {
+template <int ES, int V, int NW, bool kWhole>
+__global__ __launch_bounds__(kWave* NW) void gated_bwd_kernel(GatedParams p, GatedGrad d) {
   constexpr int K = kGatedK;
+  __shared__ GatedShare<V, NW> share;
   const GatedAt<V> at(p);
   if (!kWhole && at.c == 0) return;  // (nothing comes before the first)
-  float l[V], prod[V];
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  float l[V], total[V];  // what enters the waves' steps from behind; the chunk's product
   float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D + at.ch;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     l[i] = 0.f;
-    prod[i] = 1.f;
+    total[i] = 1.f;
     if (kWhole && p.nchunk > 1) l[i] = slot[i];
     if (kWhole && p.nchunk == 1 && d.dh != nullptr) l[i] = d.dh[at.b * p.D + at.ch + i];
   }
@@ -31,91 +34,158 @@ __global__ __launch_bounds__(kWave) void gated_bwd_kernel(GatedParams p, GatedGr
   char* dx = static_cast<char*>(d.dx) + (at.b * p.L * p.D + at.ch) * ES;
   char* dg = static_cast<char*>(d.dg) + (at.b * p.L * p.D + at.ch) * ES;
   const float* ck = p.ckpt + at.b * ((p.L + K - 1) / K) * p.D + at.ch;
-  GatedRaw<ES, V> rx[K], rg[K], rd[K];
-  GatedRaw<4, V> rh;
-  uint32_t bits = 0;
-  auto load = [&](int64_t t) {
+  int turn = 0;
+  for (int64_t t0 = at.t0 + (at.t1 - at.t0 - 1) / (K * NW) * (K * NW); t0 >= at.t0;
+       t0 -= K * NW, turn ^= 1) {
+    const int64_t t = t0 + wave * K;
+    const int n = at.t1 - t < K ? (int)(at.t1 - t) : K;  // (0 or less: no steps left)
+    GatedRaw<ES, V> rx[K], rg[K], rd[K];
+    float h[V] = {};
 #pragma unroll
     for (int u = 0; u < K; ++u) {
-      const int64_t s = t + u < at.t1 ? t + u : at.t1 - 1;
-      if (kWhole) rx[u] = gated_load<ES, V>(x + s * p.xsl * ES);
-      rg[u] = gated_load<ES, V>(g + s * p.gsl * ES);
-      if (d.dy != nullptr) rd[u] = gated_load<ES, V>(dy + s * d.dysl * ES);
+#pragma unroll
+      for (int i = 0; i < GatedRaw<ES, V>::kWords; ++i) rd[u].w[i] = 0;
+      if (u < n) {
+        if (kWhole) rx[u] = gated_load<ES, V>(x + (t + u) * p.xsl * ES);
+        rg[u] = gated_load<ES, V>(g + (t + u) * p.gsl * ES);
+        if (d.dy != nullptr) rd[u] = gated_load<ES, V>(dy + (t + u) * d.dysl * ES);
+      }
     }
-    if (kWhole) rh = gated_load<4, V>(reinterpret_cast<const char*>(ck + t / K * p.D));
-    bits = start_bits(p, at.b, t, (int)(at.t1 - t < K ? at.t1 - t : K));
-  };
-  int64_t t = (at.t1 - 1) / K * K;  // (chunks begin at multiples of K)
-  load(t);
-  for (; t >= at.t0; t -= K) {
-    // the way there: a, 1 - a and (h_{t-1} - x) a (1 - a)
-    float a[K][V], na[K][V], c[K][V], gy[K][V], h[V];
-    const uint32_t now = bits;
+    uint32_t bits = 0;
+    if (n > 0) {
+      bits = start_bits(p, at.b, t, n);
+      if (kWhole) {
+        const GatedRaw<4, V> r = gated_load<4, V>(reinterpret_cast<const char*>(ck + t / K * p.D));
 #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = kWhole ? __uint_as_float(rh.w[i]) : 0.f;
+        for (int i = 0; i < V; ++i) h[i] = __uint_as_float(r.w[i]);
+      }
+    }
+    // the states, of which h_{t-1} - x_t stays, and the gates
+    float a[K][V], na[K][V], c[K][V];
 #pragma unroll
     for (int u = 0; u < K; ++u) {
+      if (u < n) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        gate_of(gated_value(rg[u], i, p.dt), a[u][i], na[u][i]);
-        gy[u][i] = d.dy != nullptr ? gated_value(rd[u], i, p.dt) : 0.f;
-        if (kWhole) {
-          const float xv = gated_value(rx[u], i, p.dt);
-          const float prev = now >> u & 1 ? 0.f : h[i];
-          c[u][i] = (prev - xv) * (a[u][i] * na[u][i]);
-          h[i] = ffma(a[u][i], prev, na[u][i] * xv);
+        for (int i = 0; i < V; ++i) {
+          gate_of(gated_value(rg[u], i, p.dt), a[u][i], na[u][i]);
+          if (kWhole) {
+            const float xv = gated_value(rx[u], i, p.dt);
+            const float prev = bits >> u & 1 ? 0.f : h[i];
+            c[u][i] = prev - xv;
+            h[i] = ffma(a[u][i], prev, na[u][i] * xv);
+          }
         }
       }
     }
-    if (t - K >= at.t0) load(t - K);
-    // the way back
+    // the way back from 0, for what the wave passes on
+    float prod[V], end[V], from[V];
 #pragma unroll
-    for (int u = K - 1; u >= 0; --u) {
-      if (t + u >= at.t1) continue;
-      const bool begin = now >> u & 1;
-      float ox[V], og[V];
+    for (int i = 0; i < V; ++i) {
+      prod[i] = 1.f;
+      end[i] = 0.f;
+    }
+    if (NW > 1 || !kWhole) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float s = gy[u][i] + l[i];
-        ox[i] = s * na[u][i];
-        og[i] = s * c[u][i];
-        l[i] = begin ? 0.f : a[u][i] * s;
-        if (!kWhole) prod[i] = begin ? -0.f : prod[i] * a[u][i];
-      }
-      if (kWhole) {
-        gated_store<ES, V>(dx + (t + u) * p.D * ES, ox, p.dt);
-        gated_store<ES, V>(dg + (t + u) * p.D * ES, og, p.dt);
+      for (int u = K - 1; u >= 0; --u) {
+        if (u < n) {
+          const bool begin = bits >> u & 1;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float s = gated_value(rd[u], i, p.dt) + end[i];
+            end[i] = begin ? 0.f : a[u][i] * s;
+            prod[i] = begin ? -0.f : prod[i] * a[u][i];
+          }
+        }
       }
     }
+    if constexpr (NW > 1) {
+      gated_store<4, V>(reinterpret_cast<char*>(&share.prod[turn][wave][lane * V]), prod, RP_F32);
+      gated_store<4, V>(reinterpret_cast<char*>(&share.end[turn][wave][lane * V]), end, RP_F32);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < V; ++i) from[i] = l[i];
+#pragma unroll
+      for (int w = NW - 1; w >= 0; --w) {
+        if (w == wave) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) from[i] = l[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float pw = share.prod[turn][w][lane * V + i];
+          l[i] = gated_join(pw, share.end[turn][w][lane * V + i], l[i]);
+          if (!kWhole) total[i] = gated_product(total[i], pw);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        from[i] = l[i];
+        if (!kWhole) {
+          l[i] = gated_join(prod[i], end[i], l[i]);
+          total[i] = gated_product(total[i], prod[i]);
+        }
+      }
+    }
+    if constexpr (kWhole) {
+#pragma unroll
+      for (int u = K - 1; u >= 0; --u) {
+        if (u < n) {
+          const bool begin = bits >> u & 1;
+          float ox[V], og[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float s = gated_value(rd[u], i, p.dt) + from[i];
+            ox[i] = s * na[u][i];
+            from[i] = begin ? 0.f : a[u][i] * s;
+            og[i] = s * (c[u][i] * (a[u][i] * na[u][i]));
+          }
+          gated_store<ES, V>(dx + (t + u) * p.D * ES, ox, p.dt);
+          gated_store<ES, V>(dg + (t + u) * p.D * ES, og, p.dt);
+        }
+      }
+      if constexpr (NW == 1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) l[i] = from[i];
+      }
+      if (d.dh0 != nullptr && t == 0)
+        gated_store<4, V>(reinterpret_cast<char*>(d.dh0 + at.b * p.D + at.ch), from, RP_F32);
+    }
   }
-  if (!kWhole) {
-    gated_store<4, V>(reinterpret_cast<char*>(slot), prod, RP_F32);
+  if (!kWhole && wave == 0) {
+    gated_store<4, V>(reinterpret_cast<char*>(slot), total, RP_F32);
     gated_store<4, V>(reinterpret_cast<char*>(slot + p.D), l, RP_F32);
-  } else if (d.dh0 != nullptr && at.c == 0) {
-    gated_store<4, V>(reinterpret_cast<char*>(d.dh0 + at.b * p.D + at.ch), l, RP_F32);
   }
 }
 
 namespace {
 
-template <int ES, int V>
+template <int ES, int V, int NW>
 hipError_t run(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * p.nchunk * ((p.D + kWave * V - 1) / (kWave * V))));
   if (p.nchunk > 1) {
-    hipLaunchKernelGGL((gated_bwd_kernel<ES, V, false>), grid, dim3(kWave), 0, st, p, g);
+    hipLaunchKernelGGL((gated_bwd_kernel<ES, V, NW, false>), grid, dim3(kWave * NW), 0, st, p, g);
     const hipError_t e = launch_gated_fold(p, g.dh, true, st);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((gated_bwd_kernel<ES, V, true>), grid, dim3(kWave), 0, st, p, g);
+  hipLaunchKernelGGL((gated_bwd_kernel<ES, V, NW, true>), grid, dim3(kWave * NW), 0, st, p, g);
   return hipGetLastError();
+}
+
+template <int ES, int V>
+hipError_t run_waves(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
+#define RP_CASE(NW) \
+  if (p.nw == NW) return run<ES, V, NW>(p, g, st);
+  RP_GATED_WAVES(RP_CASE)
+#undef RP_CASE
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
 
 hipError_t launch_gated_bwd(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
-  const int V = gated_lane_channels(p.B, p.D, true);
-  if (p.es == 4) return V == 2 ? run<4, 2>(p, g, st) : run<4, 1>(p, g, st);
-  return V == 2 ? run<2, 2>(p, g, st) : run<2, 1>(p, g, st);
+  if (p.es == 4) return run_waves<4, 1>(p, g, st);
+  return gated_lane_channels(2, p.D) == 2 ? run_waves<2, 2>(p, g, st) : run_waves<2, 1>(p, g, st);
 }
 
 }  // namespace rp

@@ -2,159 +2,267 @@
 //     h_t = a_t h_{t-1} + (1 - a_t) x_t,  y_t = h_t
 // and h_{t-1} taken as 0 where a sequence begins.  The state is fp32 in a register.
 //
-// The steps are a chain of one multiply-add each, so time goes by what is in flight:
-// each wave loads the next eight steps' inputs while it works on the present ones.
-// Where sequences times channels are too few waves for the card, the time axis is
-// split: a first launch takes each chunk's (product of gates, end state from 0), a
-// second joins them to the state that enters each chunk, and the main one starts from
-// those.  The inputs are read twice then.
+// Walked step by step a sequence goes by the latency of its loads.  So the waves of a
+// workgroup stand one behind the other in time: each loads 16 steps at once, forms the
+// product of their gates and the end state that they reach from 0, and leaves both in
+// LDS; the states that enter the waves follow from those (one multiply-add a wave),
+// and each wave goes over its 16 steps again, from registers.  The inputs are read
+// once.  Where sequences times channels are too few workgroups for the card, the time
+// axis is split among workgroups too: a launch takes each chunk's (product, end), a
+// second joins them, and the main one starts from there; the inputs are read twice
+// then.
 
 #include "gated.h"
 
 namespace rp {
 
-namespace {
-constexpr int kAhead = 8;
-}
-
 // kWhole: writes y (and the checkpoints); else only the chunks' (product, end).
-template <int ES, int V, bool kWhole>
-__global__ __launch_bounds__(kWave) void gated_fwd_kernel(GatedParams p) {
+template <int ES, int V, int NW, bool kWhole>
+__global__ __launch_bounds__(kWave* NW) void gated_fwd_kernel(GatedParams p) {
+  constexpr int K = kGatedK;
+  __shared__ GatedShare<V, NW> share;
   const GatedAt<V> at(p);
   if (!kWhole && at.c + 1 == p.nchunk) return;  // (nothing comes behind the last)
-  float h[V], prod[V];
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  float h[V], total[V];  // the state that enters the waves' steps; the chunk's product
   float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D + at.ch;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     h[i] = 0.f;
-    prod[i] = 1.f;
+    total[i] = 1.f;
     if (kWhole && p.nchunk > 1) h[i] = slot[i];
     if (kWhole && p.nchunk == 1 && p.h0 != nullptr) h[i] = p.h0[at.b * p.D + at.ch + i];
   }
   const char* x = static_cast<const char*>(p.x) + (at.b * p.xsb + at.ch) * ES;
   const char* g = static_cast<const char*>(p.g) + (at.b * p.gsb + at.ch) * ES;
   char* y = static_cast<char*>(p.y) + (at.b * p.L * p.D + at.ch) * ES;
-  GatedRaw<ES, V> rx[kAhead], rg[kAhead];
-  uint32_t bits = 0;
-  auto load = [&](int64_t t) {
+  int turn = 0;
+  for (int64_t t0 = at.t0; t0 < at.t1; t0 += K * NW, turn ^= 1) {
+    const int64_t t = t0 + wave * K;
+    const int n = at.t1 - t < K ? (int)(at.t1 - t) : K;  // (0 or less: no steps left)
+    GatedRaw<ES, V> rx[K], rg[K];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      // (past the chunk the last step again)
-      const int64_t s = t + u < at.t1 ? t + u : at.t1 - 1;
-      rx[u] = gated_load<ES, V>(x + s * p.xsl * ES);
-      rg[u] = gated_load<ES, V>(g + s * p.gsl * ES);
+    for (int u = 0; u < K; ++u) {
+      if (u < n) {
+        rx[u] = gated_load<ES, V>(x + (t + u) * p.xsl * ES);
+        rg[u] = gated_load<ES, V>(g + (t + u) * p.gsl * ES);
+      }
     }
-    bits = start_bits(p, at.b, t, (int)(at.t1 - t < kAhead ? at.t1 - t : kAhead));
-  };
-  load(at.t0);
-  for (int64_t t = at.t0; t < at.t1; t += kAhead) {
-    GatedRaw<ES, V> cx[kAhead], cg[kAhead];
-    const uint32_t now = bits;
+    const uint32_t bits = n > 0 ? start_bits(p, at.b, t, n) : 0;
+    float a[K][V], in[K][V], prod[V], end[V];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      cx[u] = rx[u];
-      cg[u] = rg[u];
-    }
-    if (t + kAhead < at.t1) load(t + kAhead);
-    if (kWhole && p.ckpt != nullptr && t % kGatedK == 0) {
-      float* to = p.ckpt + (at.b * ((p.L + kGatedK - 1) / kGatedK) + t / kGatedK) * p.D + at.ch;
-      gated_store<4, V>(reinterpret_cast<char*>(to), h, RP_F32);
+    for (int i = 0; i < V; ++i) {
+      prod[i] = 1.f;
+      end[i] = 0.f;
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (t + u >= at.t1) break;
-      const bool begin = now >> u & 1;
+    for (int u = 0; u < K; ++u) {
+      if (u < n) {
+        const bool begin = bits >> u & 1;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float na;
+          gate_of(gated_value(rg[u], i, p.dt), a[u][i], na);
+          in[u][i] = na * gated_value(rx[u], i, p.dt);
+          prod[i] = begin ? -0.f : prod[i] * a[u][i];
+          end[i] = ffma(a[u][i], begin ? 0.f : end[i], in[u][i]);
+        }
+      }
+    }
+    float from[V];
+    if constexpr (NW > 1) {
+      gated_store<4, V>(reinterpret_cast<char*>(&share.prod[turn][wave][lane * V]), prod, RP_F32);
+      gated_store<4, V>(reinterpret_cast<char*>(&share.end[turn][wave][lane * V]), end, RP_F32);
+      // (the next turn's stores go to the other half, and the one behind that waits for
+      // this turn's reads at the next turn's barrier)
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < V; ++i) from[i] = h[i];
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        if (w == wave) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) from[i] = h[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float pw = share.prod[turn][w][lane * V + i];
+          h[i] = gated_join(pw, share.end[turn][w][lane * V + i], h[i]);
+          if (!kWhole) total[i] = gated_product(total[i], pw);
+        }
+      }
+    } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float a, na;
-        gate_of(gated_value(cg[u], i, p.dt), a, na);
-        const float prev = begin ? 0.f : h[i];
-        h[i] = ffma(a, prev, na * gated_value(cx[u], i, p.dt));
-        if (!kWhole) prod[i] = begin ? -0.f : prod[i] * a;
+        from[i] = h[i];
+        h[i] = gated_join(prod[i], end[i], h[i]);
+        if (!kWhole) total[i] = gated_product(total[i], prod[i]);
       }
-      if (kWhole) gated_store<ES, V>(y + (t + u) * p.D * ES, h, p.dt);
+    }
+    if constexpr (kWhole) {
+      if (n > 0 && p.ckpt != nullptr) {
+        float* to = p.ckpt + (at.b * ((p.L + K - 1) / K) + t / K) * p.D + at.ch;
+        gated_store<4, V>(reinterpret_cast<char*>(to), from, RP_F32);
+      }
+#pragma unroll
+      for (int u = 0; u < K; ++u) {
+        if (u < n) {
+          const bool begin = bits >> u & 1;
+#pragma unroll
+          for (int i = 0; i < V; ++i) from[i] = ffma(a[u][i], begin ? 0.f : from[i], in[u][i]);
+          gated_store<ES, V>(y + (t + u) * p.D * ES, from, p.dt);
+        }
+      }
+      // the wave with the last step has the last state, as its own steps give it
+      if (p.h_last != nullptr && t < p.L && t + n == p.L)
+        gated_store<4, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D + at.ch), from, RP_F32);
     }
   }
-  if (!kWhole) {
-    gated_store<4, V>(reinterpret_cast<char*>(slot), prod, RP_F32);
+  if (!kWhole && wave == 0) {
+    gated_store<4, V>(reinterpret_cast<char*>(slot), total, RP_F32);
     gated_store<4, V>(reinterpret_cast<char*>(slot + p.D), h, RP_F32);
-  } else if (p.h_last != nullptr && at.c + 1 == p.nchunk) {
-    gated_store<4, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D + at.ch), h, RP_F32);
   }
 }
 
+// Few steps (a rollout's single token): no stretch to share, one thread for 16 bytes of
+// a row.
+template <int ES, int V>
+__global__ __launch_bounds__(kWave) void gated_few_kernel(GatedParams p) {
+  const GatedAt<V> at(p);
+  float h[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) h[i] = 0.f;
+  if (p.h0 != nullptr) {
+    const GatedRaw<4, V> r =
+        gated_load<4, V>(reinterpret_cast<const char*>(p.h0 + at.b * p.D + at.ch));
+#pragma unroll
+    for (int i = 0; i < V; ++i) h[i] = __uint_as_float(r.w[i]);
+  }
+  const char* x = static_cast<const char*>(p.x) + (at.b * p.xsb + at.ch) * ES;
+  const char* g = static_cast<const char*>(p.g) + (at.b * p.gsb + at.ch) * ES;
+  char* y = static_cast<char*>(p.y) + (at.b * p.L * p.D + at.ch) * ES;
+  if (p.ckpt != nullptr)
+    gated_store<4, V>(reinterpret_cast<char*>(p.ckpt + at.b * p.D + at.ch), h, RP_F32);
+  for (int64_t t = 0; t < p.L; ++t) {
+    const GatedRaw<ES, V> rx = gated_load<ES, V>(x + t * p.xsl * ES);
+    const GatedRaw<ES, V> rg = gated_load<ES, V>(g + t * p.gsl * ES);
+    const bool begin = start_bits(p, at.b, t, 1) != 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float a, na;
+      gate_of(gated_value(rg, i, p.dt), a, na);
+      h[i] = ffma(a, begin ? 0.f : h[i], na * gated_value(rx, i, p.dt));
+    }
+    gated_store<ES, V>(y + t * p.D * ES, h, p.dt);
+  }
+  if (p.h_last != nullptr)
+    gated_store<4, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D + at.ch), h, RP_F32);
+}
+
 // What enters each chunk, over its product: forwards from `in` (h0), or backwards from
-// the gradient of the last state.  One thread a channel.
-__global__ __launch_bounds__(kWave) void gated_fold_kernel(GatedParams p, const float* in,
-                                                           bool backward) {
+// the gradient of the last state.  16 waves take a sixteenth of the chunks of 64
+// channels each, as the waves above take steps.
+constexpr int kFoldWaves = 16;
+__global__ __launch_bounds__(kFoldWaves* kWave) void gated_fold_kernel(GatedParams p, const float* in,
+                                                                       bool backward) {
+  __shared__ float prods[kFoldWaves][kWave], ends[kFoldWaves][kWave];
   const uint32_t tiles = (uint32_t)((p.D + kWave - 1) / kWave);
   const int64_t b = blockIdx.x / tiles;
-  const int64_t ch = (int64_t)(blockIdx.x % tiles) * kWave + threadIdx.x;
-  if (ch >= p.D) return;
-  float h = in != nullptr ? in[b * p.D + ch] : 0.f;
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  int64_t ch = (int64_t)(blockIdx.x % tiles) * kWave + lane;
+  if (ch > p.D - 1) ch = p.D - 1;
   float* base = p.agg + b * p.nchunk * 2 * p.D + ch;
-  constexpr int kN = 8;
-  for (int k0 = 0; k0 < p.nchunk; k0 += kN) {
-    float a[kN], e[kN];
-#pragma unroll
-    for (int k = 0; k < kN; ++k) {
-      // (the last one's own product is never formed; nothing comes behind it)
-      const int64_t i = k0 + k < p.nchunk - 1 ? k0 + k : p.nchunk - 2;
-      const float* s = base + (backward ? p.nchunk - 1 - i : i) * 2 * p.D;
-      a[k] = s[0];
-      e[k] = s[p.D];
-    }
-#pragma unroll
-    for (int k = 0; k < kN; ++k) {
-      const int i = k0 + k;
-      if (i >= p.nchunk) break;
-      base[(int64_t)(backward ? p.nchunk - 1 - i : i) * 2 * p.D] = h;
-      h = gated_join(a[k], e[k], h);
-    }
+  auto slot = [&](int i) { return base + (int64_t)(backward ? p.nchunk - 1 - i : i) * 2 * p.D; };
+  // (the last chunk's own product is never formed; nothing comes behind it)
+  const int n = p.nchunk - 1, each = (n + kFoldWaves - 1) / kFoldWaves;
+  const int first = wave * each < n ? wave * each : n, last = first + each < n ? first + each : n;
+  float prod = 1.f, end = 0.f;
+#pragma unroll 8
+  for (int i = first; i < last; ++i) {
+    const float* s = slot(i);
+    end = gated_join(s[0], s[p.D], end);
+    prod = gated_product(prod, s[0]);
   }
+  prods[wave][lane] = prod;
+  ends[wave][lane] = end;
+  __syncthreads();
+  float h = in != nullptr ? in[b * p.D + ch] : 0.f;
+  for (int w = 0; w < wave; ++w) h = gated_join(prods[w][lane], ends[w][lane], h);
+#pragma unroll 8
+  for (int i = first; i < last; ++i) {
+    float* s = slot(i);
+    const float a = s[0], e = s[p.D];
+    s[0] = h;
+    h = gated_join(a, e, h);
+  }
+  // (the waves behind the last chunk have folded all of it)
+  if (wave == kFoldWaves - 1) *slot(n) = h;
 }
 
 hipError_t launch_gated_fold(const GatedParams& p, const float* in, bool backward, hipStream_t st) {
   hipLaunchKernelGGL(gated_fold_kernel, dim3((unsigned)(p.B * ((p.D + kWave - 1) / kWave))),
-                     dim3(kWave), 0, st, p, in, backward);
+                     dim3(kFoldWaves * kWave), 0, st, p, in, backward);
   return hipGetLastError();
 }
 
-int64_t gated_plan(GatedParams* p, bool backward) {
-  const int V = gated_lane_channels(p->B, p->D, backward);
-  const int64_t waves = p->B * ((p->D + kWave * V - 1) / (kWave * V));
-  p->nchunk = 1;
-  p->chunk = (p->L + kGatedK - 1) / kGatedK * kGatedK;
-  if (waves < 1024 && waves > 0 && p->L >= 128) {
-    int64_t n = (2048 + waves - 1) / waves;
-    if (n > (p->L + 63) / 64) n = (p->L + 63) / 64;
-    const int64_t each = (p->L + n - 1) / n;
-    p->chunk = (each + kGatedK - 1) / kGatedK * kGatedK;
-    p->nchunk = (int)((p->L + p->chunk - 1) / p->chunk);
+int64_t gated_plan(GatedParams* p) {
+  const int V = gated_lane_channels(p->es, p->D);
+  const int64_t tiles = p->B * ((p->D + kWave * V - 1) / (kWave * V));
+  // waves of a workgroup: until the card is full, or the sequence is
+  int nw = 1;
+  while (nw < 16 && nw * kGatedK < p->L && (tiles * nw < 8192 || nw < 4)) nw *= 2;
+  int64_t n = 1;
+  if (tiles * nw < 2048 && p->L > 2 * kGatedK * nw) {
+    nw = 4;
+    n = (8192 / nw + tiles - 1) / tiles;
+    const int64_t most = (p->L + kGatedK * nw - 1) / (kGatedK * nw);
+    if (n > most) n = most;
   }
+  const int64_t step = kGatedK * nw, each = (p->L + n - 1) / n;
+  p->nw = nw;
+  p->chunk = (each + step - 1) / step * step;
+  p->nchunk = (int)((p->L + p->chunk - 1) / p->chunk);
   return p->nchunk > 1 ? p->B * p->nchunk * 2 * p->D : 0;
 }
 
 namespace {
 
-template <int ES, int V>
+template <int ES, int V, int NW>
 hipError_t run(const GatedParams& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * p.nchunk * ((p.D + kWave * V - 1) / (kWave * V))));
   if (p.nchunk > 1) {
-    hipLaunchKernelGGL((gated_fwd_kernel<ES, V, false>), grid, dim3(kWave), 0, st, p);
+    hipLaunchKernelGGL((gated_fwd_kernel<ES, V, NW, false>), grid, dim3(kWave * NW), 0, st, p);
     const hipError_t e = launch_gated_fold(p, p.h0, false, st);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((gated_fwd_kernel<ES, V, true>), grid, dim3(kWave), 0, st, p);
+  hipLaunchKernelGGL((gated_fwd_kernel<ES, V, NW, true>), grid, dim3(kWave * NW), 0, st, p);
   return hipGetLastError();
+}
+
+template <int ES, int V>
+hipError_t run_few(const GatedParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)(p.B * ((p.D + kWave * V - 1) / (kWave * V))));
+  hipLaunchKernelGGL((gated_few_kernel<ES, V>), grid, dim3(kWave), 0, st, p);
+  return hipGetLastError();
+}
+
+template <int ES, int V>
+hipError_t run_waves(const GatedParams& p, hipStream_t st) {
+#define RP_CASE(NW) \
+  if (p.nw == NW) return run<ES, V, NW>(p, st);
+  RP_GATED_WAVES(RP_CASE)
+#undef RP_CASE
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
 
 hipError_t launch_gated_fwd(const GatedParams& p, hipStream_t st) {
-  const int V = gated_lane_channels(p.B, p.D, false);
-  if (p.es == 4) return V == 4 ? run<4, 4>(p, st) : V == 2 ? run<4, 2>(p, st) : run<4, 1>(p, st);
-  return V == 4 ? run<2, 4>(p, st) : V == 2 ? run<2, 2>(p, st) : run<2, 1>(p, st);
+  if (p.L <= 4 && p.D >= 4) return p.es == 4 ? run_few<4, 4>(p, st) : run_few<2, 4>(p, st);
+  if (p.es == 4) return run_waves<4, 1>(p, st);
+  return gated_lane_channels(2, p.D) == 2 ? run_waves<2, 2>(p, st) : run_waves<2, 1>(p, st);
 }
 
 }  // namespace rp

@@ -38,8 +38,8 @@ def _args(x, gate, starts):
     return a, (x, gate, starts)  # (copies live as long as the call)
 
 
-def _work(lib, a, backward, device):
-    a.work_bytes = lib.rp_gated_work_bytes(ctypes.byref(a), backward)
+def _work(lib, a, device):
+    a.work_bytes = lib.rp_gated_work_bytes(ctypes.byref(a))
     if a.work_bytes <= 0:
         return None
     work = torch.empty(a.work_bytes, dtype=torch.uint8, device=device)
@@ -61,7 +61,7 @@ def _forward(x, gate, h0, starts, keep):
         ckpt = torch.empty(lib.rp_gated_ckpt_bytes(ctypes.byref(a)) // 4, dtype=torch.float32,
                            device=x.device)
         a.ckpt = ckpt.data_ptr()
-    work = _work(lib, a, 0, x.device)  # noqa: F841  (held until the launch)
+    work = _work(lib, a, x.device)  # noqa: F841  (held until the launch)
     a.y, a.h_last = y.data_ptr(), last.data_ptr()
     _lib.call(lib.rp_gated_fwd, x.device, ctypes.byref(a))
     return y, last, ckpt
@@ -86,7 +86,7 @@ class _HipGatedScan(torch.autograd.Function):
         B, L, D = x.shape
         a, hold = _args(x, gate, starts)
         a.ckpt = ckpt.data_ptr()
-        work = _work(lib, a, 1, x.device)  # noqa: F841  (held until the launch)
+        work = _work(lib, a, x.device)  # noqa: F841  (held until the launch)
         dx = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
         dgate = torch.empty_like(dx)
         g = _lib.GatedGrad(dx=dx.data_ptr(), dgate=dgate.data_ptr())

@@ -1809,8 +1809,9 @@ int check_gated_inputs(const rp_gated_args* a) {
 int rp_gated_check(const rp_gated_args* a) {
   if (a == nullptr) return fail(RP_ERR_INVALID, "gated args: NULL");
   if (a->B < 0 || a->L < 0 || a->D < 0) return fail(RP_ERR_INVALID, "gated args: negative size");
-  if (a->B > kI32Max || a->L > kI32Max || a->D > kI32Max)
-    return fail(RP_ERR_UNSUPPORTED, "gated args: sizes must fit in int32");
+  // (a row's bytes are 32-bit offsets)
+  if (a->B > kI32Max || a->L > kI32Max || a->D > ((int64_t)1 << 28))
+    return fail(RP_ERR_UNSUPPORTED, "gated args: B and L must fit in int32, D up to 2^28");
   if (!known_dtype(a->dtype)) return fail(RP_ERR_INVALID, "gated args: unknown dtype code %d", a->dtype);
   if (a->B == 0 || a->L == 0 || a->D == 0) return RP_OK;
   // (the launches hold a wave for each 64 to 256 channels of a sequence's chunk)

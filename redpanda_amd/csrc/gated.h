@@ -11,6 +11,10 @@
 
 namespace rp {
 
+// The storage types are known when the kernels are compiled (T, an RP_* code): choosing
+// between the two of 16 bits for each value kept both forms in registers.
+constexpr int gated_es(int T) { return T == RP_F32 ? 4 : 2; }
+
 // V adjacent elements as stored.
 template <int ES, int V>
 struct GatedRaw {
@@ -18,8 +22,11 @@ struct GatedRaw {
   uint32_t w[kWords];
 };
 
+// (a row, the same in every lane, and the lane's bytes into it: one scalar address for
+// all lanes and no vector registers for the rows')
 template <int ES, int V>
-__device__ __forceinline__ GatedRaw<ES, V> gated_load(const char* p) {
+__device__ __forceinline__ GatedRaw<ES, V> gated_load(const char* row, uint32_t at) {
+  const char* p = row + at;
   GatedRaw<ES, V> r;
   if constexpr (ES * V == 2) {
     r.w[0] = *reinterpret_cast<const uint16_t*>(p);
@@ -38,20 +45,22 @@ __device__ __forceinline__ GatedRaw<ES, V> gated_load(const char* p) {
   return r;
 }
 
-template <int ES, int V>
-__device__ __forceinline__ float gated_value(const GatedRaw<ES, V>& r, int i, int dtype) {
-  if constexpr (ES == 4) {
+template <int T, int ES, int V>
+__device__ __forceinline__ float gated_value(const GatedRaw<ES, V>& r, int i) {
+  if constexpr (T == RP_F32) {
     return __uint_as_float(r.w[i]);
+  } else if constexpr (T == RP_BF16) {
+    return __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
   } else {
-    if (dtype == RP_BF16)
-      return __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
     return static_cast<float>(
         __builtin_bit_cast(_Float16, static_cast<uint16_t>(r.w[i / 2] >> (16 * (i & 1)))));
   }
 }
 
-template <int ES, int V>
-__device__ __forceinline__ void gated_store(char* p, const float (&v)[V], int dtype) {
+template <int T, int V>
+__device__ __forceinline__ void gated_store(char* row, uint32_t at, const float (&v)[V]) {
+  constexpr int ES = T == RP_F32 ? 4 : 2;
+  char* p = row + at;
   if constexpr (ES == 4) {
     if constexpr (V == 4) {
       u32x4_any w;
@@ -68,14 +77,14 @@ __device__ __forceinline__ void gated_store(char* p, const float (&v)[V], int dt
     }
   } else if constexpr (V == 4) {
     u32x2_any w;
-    w[0] = pack16(v[0], v[1], dtype);
-    w[1] = pack16(v[2], v[3], dtype);
+    w[0] = pack16(v[0], v[1], T);
+    w[1] = pack16(v[2], v[3], T);
     *reinterpret_cast<u32x2_any*>(p) = w;
   } else if constexpr (V == 2) {
     typedef uint32_t u32_any __attribute__((aligned(1)));
-    *reinterpret_cast<u32_any*>(p) = pack16(v[0], v[1], dtype);
+    *reinterpret_cast<u32_any*>(p) = pack16(v[0], v[1], T);
   } else {
-    *reinterpret_cast<uint16_t*>(p) = (uint16_t)pack16(v[0], 0.f, dtype);
+    *reinterpret_cast<uint16_t*>(p) = (uint16_t)pack16(v[0], 0.f, T);
   }
 }
 
@@ -99,14 +108,15 @@ __device__ __forceinline__ uint32_t start_bits(const GatedParams& p, int64_t b, 
 // A workgroup's place: its sequence, its time chunk and its lanes' first channels.
 template <int V>
 struct GatedAt {
-  int64_t b, c, ch, t0, t1;
+  int64_t b, c, t0, t1;
+  uint32_t ch;
   __device__ __forceinline__ GatedAt(const GatedParams& p) {
     const uint32_t tiles = (uint32_t)((p.D + kWave * V - 1) / (kWave * V));
     const uint32_t rest = blockIdx.x / tiles, tile = blockIdx.x - rest * tiles;
     b = rest / (uint32_t)p.nchunk;
     c = rest - (uint32_t)b * (uint32_t)p.nchunk;
-    ch = ((int64_t)tile * kWave + threadIdx.x % kWave) * V;
-    if (ch > p.D - V) ch = p.D - V;
+    ch = (tile * kWave + threadIdx.x % kWave) * V;
+    if (ch > (uint32_t)p.D - V) ch = (uint32_t)p.D - V;
     t0 = c * p.chunk;
     t1 = t0 + p.chunk < p.L ? t0 + p.chunk : p.L;
   }
@@ -136,6 +146,6 @@ inline int gated_lane_channels(int es, int64_t D) { return es == 2 && D >= 2 ? 2
 
 hipError_t launch_gated_fold(const GatedParams& p, const float* in, bool backward, hipStream_t st);
 
-#define RP_GATED_WAVES(X) X(1) X(2) X(4) X(8) X(16)
+#define RP_GATED_WAVES(X) X(1) X(2) X(4) X(8)
 
 }  // namespace rp

@@ -11,96 +11,107 @@
 
 namespace rp {
 
-template <int ES, int V, int NW, bool kWhole>
-__global__ __launch_bounds__(kWave* NW) void gated_bwd_kernel(GatedParams p, GatedGrad d) {
-  constexpr int K = kGatedK;
+template <int T, int V, int NW, bool kWhole>
+__global__ __launch_bounds__(kWave* NW)
+__attribute__((amdgpu_waves_per_eu(3))) void gated_bwd_kernel(GatedParams p, GatedGrad d) {
+  constexpr int K = kGatedK, ES = gated_es(T);
   __shared__ GatedShare<V, NW> share;
   const GatedAt<V> at(p);
   if (!kWhole && at.c == 0) return;  // (nothing comes before the first)
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   float l[V], total[V];  // what enters the waves' steps from behind; the chunk's product
-  float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D + at.ch;
+  float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     l[i] = 0.f;
     total[i] = 1.f;
-    if (kWhole && p.nchunk > 1) l[i] = slot[i];
+    if (kWhole && p.nchunk > 1) l[i] = slot[at.ch + i];
     if (kWhole && p.nchunk == 1 && d.dh != nullptr) l[i] = d.dh[at.b * p.D + at.ch + i];
   }
-  const char* x = static_cast<const char*>(p.x) + (at.b * p.xsb + at.ch) * ES;
-  const char* g = static_cast<const char*>(p.g) + (at.b * p.gsb + at.ch) * ES;
-  const char* dy = static_cast<const char*>(d.dy) + (d.dy != nullptr ? (at.b * d.dysb + at.ch) * ES : 0);
-  char* dx = static_cast<char*>(d.dx) + (at.b * p.L * p.D + at.ch) * ES;
-  char* dg = static_cast<char*>(d.dg) + (at.b * p.L * p.D + at.ch) * ES;
-  const float* ck = p.ckpt + at.b * ((p.L + K - 1) / K) * p.D + at.ch;
+  const char* x = static_cast<const char*>(p.x) + at.b * p.xsb * ES;
+  const char* g = static_cast<const char*>(p.g) + at.b * p.gsb * ES;
+  const char* dy = static_cast<const char*>(d.dy) + (d.dy != nullptr ? at.b * d.dysb * ES : 0);
+  char* dx = static_cast<char*>(d.dx) + at.b * p.L * p.D * ES;
+  char* dg = static_cast<char*>(d.dg) + at.b * p.L * p.D * ES;
+  const float* ck = p.ckpt + at.b * ((p.L + K - 1) / K) * p.D;
   int turn = 0;
   for (int64_t t0 = at.t0 + (at.t1 - at.t0 - 1) / (K * NW) * (K * NW); t0 >= at.t0;
        t0 -= K * NW, turn ^= 1) {
     const int64_t t = t0 + wave * K;
     const int n = at.t1 - t < K ? (int)(at.t1 - t) : K;  // (0 or less: no steps left)
-    GatedRaw<ES, V> rx[K], rg[K], rd[K];
-    float h[V] = {};
-#pragma unroll
-    for (int u = 0; u < K; ++u) {
-#pragma unroll
-      for (int i = 0; i < GatedRaw<ES, V>::kWords; ++i) rd[u].w[i] = 0;
-      if (u < n) {
-        if (kWhole) rx[u] = gated_load<ES, V>(x + (t + u) * p.xsl * ES);
-        rg[u] = gated_load<ES, V>(g + (t + u) * p.gsl * ES);
-        if (d.dy != nullptr) rd[u] = gated_load<ES, V>(dy + (t + u) * d.dysl * ES);
-      }
-    }
-    uint32_t bits = 0;
-    if (n > 0) {
-      bits = start_bits(p, at.b, t, n);
-      if (kWhole) {
-        const GatedRaw<4, V> r = gated_load<4, V>(reinterpret_cast<const char*>(ck + t / K * p.D));
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = __uint_as_float(r.w[i]);
-      }
-    }
-    // the states, of which h_{t-1} - x_t stays, and the gates
-    float a[K][V], na[K][V], c[K][V];
-#pragma unroll
-    for (int u = 0; u < K; ++u) {
-      if (u < n) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          gate_of(gated_value(rg[u], i, p.dt), a[u][i], na[u][i]);
-          if (kWhole) {
-            const float xv = gated_value(rx[u], i, p.dt);
-            const float prev = bits >> u & 1 ? 0.f : h[i];
-            c[u][i] = prev - xv;
-            h[i] = ffma(a[u][i], prev, na[u][i] * xv);
-          }
-        }
-      }
-    }
-    // the way back from 0, for what the wave passes on
-    float prod[V], end[V], from[V];
+    const uint32_t bits = n > 0 ? start_bits(p, at.b, t, n) : 0;
+    // 16 steps of one sequence, as nearly all are, go without a branch or a choice
+    const bool full = n == K && bits == 0 && d.dy != nullptr;
+    // the gates, and what turns a step's l_t into dz_t
+    GatedRaw<ES, V> rd[K];
+    float a[K][V], na[K][V], c[K][V], prod[V], end[V], from[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       prod[i] = 1.f;
       end[i] = 0.f;
     }
-    if (NW > 1 || !kWhole) {
+    auto there = [&](auto whole) {
+      GatedRaw<ES, V> rx[K], rg[K];
+      float h[V] = {};
+      if (kWhole && (whole() || n > 0)) {
+        const GatedRaw<4, V> r = gated_load<4, V>(reinterpret_cast<const char*>(ck + t / K * p.D), at.ch * 4);
 #pragma unroll
-      for (int u = K - 1; u >= 0; --u) {
-        if (u < n) {
-          const bool begin = bits >> u & 1;
+        for (int i = 0; i < V; ++i) h[i] = __uint_as_float(r.w[i]);
+      }
+#pragma unroll
+      for (int u = 0; u < K; ++u) {
+        if (!whole()) {
+#pragma unroll
+          for (int i = 0; i < GatedRaw<ES, V>::kWords; ++i) rd[u].w[i] = 0;
+        }
+        if (whole() || u < n) {
+          if (kWhole) rx[u] = gated_load<ES, V>(x + (t + u) * p.xsl * ES, at.ch * ES);
+          rg[u] = gated_load<ES, V>(g + (t + u) * p.gsl * ES, at.ch * ES);
+          if (whole() || d.dy != nullptr) rd[u] = gated_load<ES, V>(dy + (t + u) * d.dysl * ES, at.ch * ES);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < K; ++u) {
+        if (whole() || u < n) {
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            const float s = gated_value(rd[u], i, p.dt) + end[i];
-            end[i] = begin ? 0.f : a[u][i] * s;
-            prod[i] = begin ? -0.f : prod[i] * a[u][i];
+            gate_of(gated_value<T>(rg[u], i), a[u][i], na[u][i]);
+            if (kWhole) {
+              const float xv = gated_value<T>(rx[u], i);
+              const float prev = !whole() && bits >> u & 1 ? 0.f : h[i];
+              c[u][i] = (prev - xv) * (a[u][i] * na[u][i]);
+              h[i] = ffma(a[u][i], prev, na[u][i] * xv);
+            }
+          }
+          // (a scheduler free to work on all steps at once takes half as many registers
+          // again for it)
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      // the way back from 0, for what the wave passes on
+      if (NW > 1 || !kWhole) {
+#pragma unroll
+        for (int u = K - 1; u >= 0; --u) {
+          if (whole() || u < n) {
+            const bool begin = !whole() && bits >> u & 1;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float s = gated_value<T>(rd[u], i) + end[i];
+              end[i] = begin ? 0.f : a[u][i] * s;
+              prod[i] = begin ? -0.f : prod[i] * a[u][i];
+            }
           }
         }
       }
-    }
+    };
+    if (full)
+      there(std::true_type{});
+    else
+      there(std::false_type{});
     if constexpr (NW > 1) {
-      gated_store<4, V>(reinterpret_cast<char*>(&share.prod[turn][wave][lane * V]), prod, RP_F32);
-      gated_store<4, V>(reinterpret_cast<char*>(&share.end[turn][wave][lane * V]), end, RP_F32);
+      gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.prod[turn][wave]), lane * V * 4, prod);
+      gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.end[turn][wave]), lane * V * 4, end);
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < V; ++i) from[i] = l[i];
@@ -128,54 +139,60 @@ __global__ __launch_bounds__(kWave* NW) void gated_bwd_kernel(GatedParams p, Gat
       }
     }
     if constexpr (kWhole) {
+      auto again = [&](auto whole) {
 #pragma unroll
-      for (int u = K - 1; u >= 0; --u) {
-        if (u < n) {
-          const bool begin = bits >> u & 1;
-          float ox[V], og[V];
+        for (int u = K - 1; u >= 0; --u) {
+          if (whole() || u < n) {
+            const bool begin = !whole() && bits >> u & 1;
+            float ox[V], og[V];
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float s = gated_value(rd[u], i, p.dt) + from[i];
-            ox[i] = s * na[u][i];
-            from[i] = begin ? 0.f : a[u][i] * s;
-            og[i] = s * (c[u][i] * (a[u][i] * na[u][i]));
+            for (int i = 0; i < V; ++i) {
+              const float s = gated_value<T>(rd[u], i) + from[i];
+              ox[i] = s * na[u][i];
+              og[i] = s * c[u][i];
+              from[i] = begin ? 0.f : a[u][i] * s;
+            }
+            gated_store<T, V>(dx + (t + u) * p.D * ES, at.ch * ES, ox);
+            gated_store<T, V>(dg + (t + u) * p.D * ES, at.ch * ES, og);
           }
-          gated_store<ES, V>(dx + (t + u) * p.D * ES, ox, p.dt);
-          gated_store<ES, V>(dg + (t + u) * p.D * ES, og, p.dt);
         }
-      }
+      };
+      if (full)
+        again(std::true_type{});
+      else
+        again(std::false_type{});
       if constexpr (NW == 1) {
 #pragma unroll
         for (int i = 0; i < V; ++i) l[i] = from[i];
       }
       if (d.dh0 != nullptr && t == 0)
-        gated_store<4, V>(reinterpret_cast<char*>(d.dh0 + at.b * p.D + at.ch), from, RP_F32);
+        gated_store<RP_F32, V>(reinterpret_cast<char*>(d.dh0 + at.b * p.D), at.ch * 4, from);
     }
   }
   if (!kWhole && wave == 0) {
-    gated_store<4, V>(reinterpret_cast<char*>(slot), total, RP_F32);
-    gated_store<4, V>(reinterpret_cast<char*>(slot + p.D), l, RP_F32);
+    gated_store<RP_F32, V>(reinterpret_cast<char*>(slot), at.ch * 4, total);
+    gated_store<RP_F32, V>(reinterpret_cast<char*>(slot + p.D), at.ch * 4, l);
   }
 }
 
 namespace {
 
-template <int ES, int V, int NW>
+template <int T, int V, int NW>
 hipError_t run(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * p.nchunk * ((p.D + kWave * V - 1) / (kWave * V))));
   if (p.nchunk > 1) {
-    hipLaunchKernelGGL((gated_bwd_kernel<ES, V, NW, false>), grid, dim3(kWave * NW), 0, st, p, g);
+    hipLaunchKernelGGL((gated_bwd_kernel<T, V, NW, false>), grid, dim3(kWave * NW), 0, st, p, g);
     const hipError_t e = launch_gated_fold(p, g.dh, true, st);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((gated_bwd_kernel<ES, V, NW, true>), grid, dim3(kWave * NW), 0, st, p, g);
+  hipLaunchKernelGGL((gated_bwd_kernel<T, V, NW, true>), grid, dim3(kWave * NW), 0, st, p, g);
   return hipGetLastError();
 }
 
-template <int ES, int V>
+template <int T, int V>
 hipError_t run_waves(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
 #define RP_CASE(NW) \
-  if (p.nw == NW) return run<ES, V, NW>(p, g, st);
+  if (p.nw == NW) return run<T, V, NW>(p, g, st);
   RP_GATED_WAVES(RP_CASE)
 #undef RP_CASE
   return hipErrorInvalidValue;
@@ -184,8 +201,10 @@ hipError_t run_waves(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
 }  // namespace
 
 hipError_t launch_gated_bwd(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
-  if (p.es == 4) return run_waves<4, 1>(p, g, st);
-  return gated_lane_channels(2, p.D) == 2 ? run_waves<2, 2>(p, g, st) : run_waves<2, 1>(p, g, st);
+  if (p.dt == RP_F32) return run_waves<RP_F32, 1>(p, g, st);
+  if (gated_lane_channels(2, p.D) == 2)
+    return p.dt == RP_BF16 ? run_waves<RP_BF16, 2>(p, g, st) : run_waves<RP_F16, 2>(p, g, st);
+  return p.dt == RP_BF16 ? run_waves<RP_BF16, 1>(p, g, st) : run_waves<RP_F16, 1>(p, g, st);
 }
 
 }  // namespace rp

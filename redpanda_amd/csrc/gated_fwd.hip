@@ -17,63 +17,71 @@
 namespace rp {
 
 // kWhole: writes y (and the checkpoints); else only the chunks' (product, end).
-template <int ES, int V, int NW, bool kWhole>
+template <int T, int V, int NW, bool kWhole>
 __global__ __launch_bounds__(kWave* NW) void gated_fwd_kernel(GatedParams p) {
-  constexpr int K = kGatedK;
+  constexpr int K = kGatedK, ES = gated_es(T);
   __shared__ GatedShare<V, NW> share;
   const GatedAt<V> at(p);
   if (!kWhole && at.c + 1 == p.nchunk) return;  // (nothing comes behind the last)
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   float h[V], total[V];  // the state that enters the waves' steps; the chunk's product
-  float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D + at.ch;
+  float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     h[i] = 0.f;
     total[i] = 1.f;
-    if (kWhole && p.nchunk > 1) h[i] = slot[i];
+    if (kWhole && p.nchunk > 1) h[i] = slot[at.ch + i];
     if (kWhole && p.nchunk == 1 && p.h0 != nullptr) h[i] = p.h0[at.b * p.D + at.ch + i];
   }
-  const char* x = static_cast<const char*>(p.x) + (at.b * p.xsb + at.ch) * ES;
-  const char* g = static_cast<const char*>(p.g) + (at.b * p.gsb + at.ch) * ES;
-  char* y = static_cast<char*>(p.y) + (at.b * p.L * p.D + at.ch) * ES;
+  const char* x = static_cast<const char*>(p.x) + at.b * p.xsb * ES;
+  const char* g = static_cast<const char*>(p.g) + at.b * p.gsb * ES;
+  char* y = static_cast<char*>(p.y) + at.b * p.L * p.D * ES;
   int turn = 0;
   for (int64_t t0 = at.t0; t0 < at.t1; t0 += K * NW, turn ^= 1) {
     const int64_t t = t0 + wave * K;
     const int n = at.t1 - t < K ? (int)(at.t1 - t) : K;  // (0 or less: no steps left)
-    GatedRaw<ES, V> rx[K], rg[K];
-#pragma unroll
-    for (int u = 0; u < K; ++u) {
-      if (u < n) {
-        rx[u] = gated_load<ES, V>(x + (t + u) * p.xsl * ES);
-        rg[u] = gated_load<ES, V>(g + (t + u) * p.gsl * ES);
-      }
-    }
     const uint32_t bits = n > 0 ? start_bits(p, at.b, t, n) : 0;
+    // 16 steps of one sequence, as nearly all are, go without a branch or a choice
+    const bool full = n == K && bits == 0;
     float a[K][V], in[K][V], prod[V], end[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       prod[i] = 1.f;
       end[i] = 0.f;
     }
+    auto there = [&](auto whole) {
+      GatedRaw<ES, V> rx[K], rg[K];
 #pragma unroll
-    for (int u = 0; u < K; ++u) {
-      if (u < n) {
-        const bool begin = bits >> u & 1;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float na;
-          gate_of(gated_value(rg[u], i, p.dt), a[u][i], na);
-          in[u][i] = na * gated_value(rx[u], i, p.dt);
-          prod[i] = begin ? -0.f : prod[i] * a[u][i];
-          end[i] = ffma(a[u][i], begin ? 0.f : end[i], in[u][i]);
+      for (int u = 0; u < K; ++u) {
+        if (whole() || u < n) {
+          rx[u] = gated_load<ES, V>(x + (t + u) * p.xsl * ES, at.ch * ES);
+          rg[u] = gated_load<ES, V>(g + (t + u) * p.gsl * ES, at.ch * ES);
         }
       }
-    }
+#pragma unroll
+      for (int u = 0; u < K; ++u) {
+        if (whole() || u < n) {
+          const bool begin = !whole() && bits >> u & 1;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float na;
+            gate_of(gated_value<T>(rg[u], i), a[u][i], na);
+            in[u][i] = na * gated_value<T>(rx[u], i);
+            prod[i] = begin ? -0.f : prod[i] * a[u][i];
+            end[i] = ffma(a[u][i], begin ? 0.f : end[i], in[u][i]);
+          }
+        }
+      }
+    };
+    if (full)
+      there(std::true_type{});
+    else
+      there(std::false_type{});
     float from[V];
     if constexpr (NW > 1) {
-      gated_store<4, V>(reinterpret_cast<char*>(&share.prod[turn][wave][lane * V]), prod, RP_F32);
-      gated_store<4, V>(reinterpret_cast<char*>(&share.end[turn][wave][lane * V]), end, RP_F32);
+      gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.prod[turn][wave]), lane * V * 4, prod);
+      gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.end[turn][wave]), lane * V * 4, end);
       // (the next turn's stores go to the other half, and the one behind that waits for
       // this turn's reads at the next turn's barrier)
       __syncthreads();
@@ -102,62 +110,69 @@ __global__ __launch_bounds__(kWave* NW) void gated_fwd_kernel(GatedParams p) {
     }
     if constexpr (kWhole) {
       if (n > 0 && p.ckpt != nullptr) {
-        float* to = p.ckpt + (at.b * ((p.L + K - 1) / K) + t / K) * p.D + at.ch;
-        gated_store<4, V>(reinterpret_cast<char*>(to), from, RP_F32);
+        float* to = p.ckpt + (at.b * ((p.L + K - 1) / K) + t / K) * p.D;
+        gated_store<RP_F32, V>(reinterpret_cast<char*>(to), at.ch * 4, from);
       }
+      auto again = [&](auto whole) {
 #pragma unroll
-      for (int u = 0; u < K; ++u) {
-        if (u < n) {
-          const bool begin = bits >> u & 1;
+        for (int u = 0; u < K; ++u) {
+          if (whole() || u < n) {
+            const bool begin = !whole() && bits >> u & 1;
 #pragma unroll
-          for (int i = 0; i < V; ++i) from[i] = ffma(a[u][i], begin ? 0.f : from[i], in[u][i]);
-          gated_store<ES, V>(y + (t + u) * p.D * ES, from, p.dt);
+            for (int i = 0; i < V; ++i) from[i] = ffma(a[u][i], begin ? 0.f : from[i], in[u][i]);
+            gated_store<T, V>(y + (t + u) * p.D * ES, at.ch * ES, from);
+          }
         }
-      }
+      };
+      if (full)
+        again(std::true_type{});
+      else
+        again(std::false_type{});
       // the wave with the last step has the last state, as its own steps give it
       if (p.h_last != nullptr && t < p.L && t + n == p.L)
-        gated_store<4, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D + at.ch), from, RP_F32);
+        gated_store<RP_F32, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D), at.ch * 4, from);
     }
   }
   if (!kWhole && wave == 0) {
-    gated_store<4, V>(reinterpret_cast<char*>(slot), total, RP_F32);
-    gated_store<4, V>(reinterpret_cast<char*>(slot + p.D), h, RP_F32);
+    gated_store<RP_F32, V>(reinterpret_cast<char*>(slot), at.ch * 4, total);
+    gated_store<RP_F32, V>(reinterpret_cast<char*>(slot + p.D), at.ch * 4, h);
   }
 }
 
 // Few steps (a rollout's single token): no stretch to share, one thread for 16 bytes of
 // a row.
-template <int ES, int V>
+template <int T, int V>
 __global__ __launch_bounds__(kWave) void gated_few_kernel(GatedParams p) {
+  constexpr int ES = gated_es(T);
   const GatedAt<V> at(p);
   float h[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) h[i] = 0.f;
   if (p.h0 != nullptr) {
     const GatedRaw<4, V> r =
-        gated_load<4, V>(reinterpret_cast<const char*>(p.h0 + at.b * p.D + at.ch));
+        gated_load<4, V>(reinterpret_cast<const char*>(p.h0 + at.b * p.D), at.ch * 4);
 #pragma unroll
     for (int i = 0; i < V; ++i) h[i] = __uint_as_float(r.w[i]);
   }
-  const char* x = static_cast<const char*>(p.x) + (at.b * p.xsb + at.ch) * ES;
-  const char* g = static_cast<const char*>(p.g) + (at.b * p.gsb + at.ch) * ES;
-  char* y = static_cast<char*>(p.y) + (at.b * p.L * p.D + at.ch) * ES;
+  const char* x = static_cast<const char*>(p.x) + at.b * p.xsb * ES;
+  const char* g = static_cast<const char*>(p.g) + at.b * p.gsb * ES;
+  char* y = static_cast<char*>(p.y) + at.b * p.L * p.D * ES;
   if (p.ckpt != nullptr)
-    gated_store<4, V>(reinterpret_cast<char*>(p.ckpt + at.b * p.D + at.ch), h, RP_F32);
+    gated_store<RP_F32, V>(reinterpret_cast<char*>(p.ckpt + at.b * p.D), at.ch * 4, h);
   for (int64_t t = 0; t < p.L; ++t) {
-    const GatedRaw<ES, V> rx = gated_load<ES, V>(x + t * p.xsl * ES);
-    const GatedRaw<ES, V> rg = gated_load<ES, V>(g + t * p.gsl * ES);
+    const GatedRaw<ES, V> rx = gated_load<ES, V>(x + t * p.xsl * ES, at.ch * ES);
+    const GatedRaw<ES, V> rg = gated_load<ES, V>(g + t * p.gsl * ES, at.ch * ES);
     const bool begin = start_bits(p, at.b, t, 1) != 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       float a, na;
-      gate_of(gated_value(rg, i, p.dt), a, na);
-      h[i] = ffma(a, begin ? 0.f : h[i], na * gated_value(rx, i, p.dt));
+      gate_of(gated_value<T>(rg, i), a, na);
+      h[i] = ffma(a, begin ? 0.f : h[i], na * gated_value<T>(rx, i));
     }
-    gated_store<ES, V>(y + t * p.D * ES, h, p.dt);
+    gated_store<T, V>(y + t * p.D * ES, at.ch * ES, h);
   }
   if (p.h_last != nullptr)
-    gated_store<4, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D + at.ch), h, RP_F32);
+    gated_store<RP_F32, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D), at.ch * 4, h);
 }
 
 // What enters each chunk, over its product: forwards from `in` (h0), or backwards from
@@ -212,7 +227,7 @@ int64_t gated_plan(GatedParams* p) {
   const int64_t tiles = p->B * ((p->D + kWave * V - 1) / (kWave * V));
   // waves of a workgroup: until the card is full, or the sequence is
   int nw = 1;
-  while (nw < 16 && nw * kGatedK < p->L && (tiles * nw < 8192 || nw < 4)) nw *= 2;
+  while (nw < 8 && nw * kGatedK < p->L && (tiles * nw < 8192 || nw < 4)) nw *= 2;
   int64_t n = 1;
   if (tiles * nw < 2048 && p->L > 2 * kGatedK * nw) {
     nw = 4;
@@ -229,29 +244,29 @@ int64_t gated_plan(GatedParams* p) {
 
 namespace {
 
-template <int ES, int V, int NW>
+template <int T, int V, int NW>
 hipError_t run(const GatedParams& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * p.nchunk * ((p.D + kWave * V - 1) / (kWave * V))));
   if (p.nchunk > 1) {
-    hipLaunchKernelGGL((gated_fwd_kernel<ES, V, NW, false>), grid, dim3(kWave * NW), 0, st, p);
+    hipLaunchKernelGGL((gated_fwd_kernel<T, V, NW, false>), grid, dim3(kWave * NW), 0, st, p);
     const hipError_t e = launch_gated_fold(p, p.h0, false, st);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((gated_fwd_kernel<ES, V, NW, true>), grid, dim3(kWave * NW), 0, st, p);
+  hipLaunchKernelGGL((gated_fwd_kernel<T, V, NW, true>), grid, dim3(kWave * NW), 0, st, p);
   return hipGetLastError();
 }
 
-template <int ES, int V>
+template <int T, int V>
 hipError_t run_few(const GatedParams& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * ((p.D + kWave * V - 1) / (kWave * V))));
-  hipLaunchKernelGGL((gated_few_kernel<ES, V>), grid, dim3(kWave), 0, st, p);
+  hipLaunchKernelGGL((gated_few_kernel<T, V>), grid, dim3(kWave), 0, st, p);
   return hipGetLastError();
 }
 
-template <int ES, int V>
+template <int T, int V>
 hipError_t run_waves(const GatedParams& p, hipStream_t st) {
 #define RP_CASE(NW) \
-  if (p.nw == NW) return run<ES, V, NW>(p, st);
+  if (p.nw == NW) return run<T, V, NW>(p, st);
   RP_GATED_WAVES(RP_CASE)
 #undef RP_CASE
   return hipErrorInvalidValue;
@@ -260,9 +275,15 @@ hipError_t run_waves(const GatedParams& p, hipStream_t st) {
 }  // namespace
 
 hipError_t launch_gated_fwd(const GatedParams& p, hipStream_t st) {
-  if (p.L <= 4 && p.D >= 4) return p.es == 4 ? run_few<4, 4>(p, st) : run_few<2, 4>(p, st);
-  if (p.es == 4) return run_waves<4, 1>(p, st);
-  return gated_lane_channels(2, p.D) == 2 ? run_waves<2, 2>(p, st) : run_waves<2, 1>(p, st);
+  if (p.L <= 4 && p.D >= 4) {
+    return p.dt == RP_F32    ? run_few<RP_F32, 4>(p, st)
+           : p.dt == RP_BF16 ? run_few<RP_BF16, 4>(p, st)
+                             : run_few<RP_F16, 4>(p, st);
+  }
+  if (p.dt == RP_F32) return run_waves<RP_F32, 1>(p, st);
+  if (gated_lane_channels(2, p.D) == 2)
+    return p.dt == RP_BF16 ? run_waves<RP_BF16, 2>(p, st) : run_waves<RP_F16, 2>(p, st);
+  return p.dt == RP_BF16 ? run_waves<RP_BF16, 1>(p, st) : run_waves<RP_F16, 1>(p, st);
 }
 
 }  // namespace rp

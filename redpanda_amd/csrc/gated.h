@@ -141,11 +141,38 @@ struct GatedShare {
   float end[2][NW][kWave * V];
 };
 
-// Channels a lane takes: four bytes of them.
-inline int gated_lane_channels(int es, int64_t D) { return es == 2 && D >= 2 ? 2 : 1; }
+// The waves' (product, end) of a chunk, joined in order (from behind: the last wave's
+// first), to the chunk's slot.
+template <int V, int NW>
+__device__ __forceinline__ void gated_leave(const GatedParams& p, int64_t b, int64_t c, uint32_t ch,
+                                            int lane, int wave, bool behind, float (&prod)[V],
+                                            float (&end)[V], GatedShare<V, NW>& share) {
+  gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.prod[0][wave]), lane * V * 4, prod);
+  gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.end[0][wave]), lane * V * 4, end);
+  __syncthreads();
+  if (wave > 0) return;
+  float total[V], out[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    total[i] = 1.f;
+    out[i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      const int w = behind ? NW - 1 - k : k;
+      const float pw = share.prod[0][w][lane * V + i];
+      out[i] = gated_join(pw, share.end[0][w][lane * V + i], out[i]);
+      total[i] = gated_product(total[i], pw);
+    }
+  }
+  float* slot = p.agg + (b * p.nchunk + c) * 2 * p.D;
+  gated_store<RP_F32, V>(reinterpret_cast<char*>(slot), ch * 4, total);
+  gated_store<RP_F32, V>(reinterpret_cast<char*>(slot + p.D), ch * 4, out);
+}
 
 hipError_t launch_gated_fold(const GatedParams& p, const float* in, bool backward, hipStream_t st);
 
+// Waves of a workgroup, and where the time axis is split among workgroups.
+constexpr int kSplitWaves = 4;
 #define RP_GATED_WAVES(X) X(1) X(2) X(4) X(8)
 
 }  // namespace rp

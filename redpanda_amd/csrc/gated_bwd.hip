@@ -11,23 +11,21 @@
 
 namespace rp {
 
-template <int T, int V, int NW, bool kWhole>
+template <int T, int V, int NW>
 __global__ __launch_bounds__(kWave* NW)
 __attribute__((amdgpu_waves_per_eu(3))) void gated_bwd_kernel(GatedParams p, GatedGrad d) {
   constexpr int K = kGatedK, ES = gated_es(T);
   __shared__ GatedShare<V, NW> share;
   const GatedAt<V> at(p);
-  if (!kWhole && at.c == 0) return;  // (nothing comes before the first)
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  float l[V], total[V];  // what enters the waves' steps from behind; the chunk's product
-  float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D;
+  float l[V];  // what enters the waves' steps from behind
+  const float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     l[i] = 0.f;
-    total[i] = 1.f;
-    if (kWhole && p.nchunk > 1) l[i] = slot[at.ch + i];
-    if (kWhole && p.nchunk == 1 && d.dh != nullptr) l[i] = d.dh[at.b * p.D + at.ch + i];
+    if (p.nchunk > 1) l[i] = slot[at.ch + i];
+    if (p.nchunk == 1 && d.dh != nullptr) l[i] = d.dh[at.b * p.D + at.ch + i];
   }
   const char* x = static_cast<const char*>(p.x) + at.b * p.xsb * ES;
   const char* g = static_cast<const char*>(p.g) + at.b * p.gsb * ES;
@@ -54,7 +52,7 @@ __attribute__((amdgpu_waves_per_eu(3))) void gated_bwd_kernel(GatedParams p, Gat
     auto there = [&](auto whole) {
       GatedRaw<ES, V> rx[K], rg[K];
       float h[V] = {};
-      if (kWhole && (whole() || n > 0)) {
+      if (whole() || n > 0) {
         const GatedRaw<4, V> r = gated_load<4, V>(reinterpret_cast<const char*>(ck + t / K * p.D), at.ch * 4);
 #pragma unroll
         for (int i = 0; i < V; ++i) h[i] = __uint_as_float(r.w[i]);
@@ -66,7 +64,7 @@ __attribute__((amdgpu_waves_per_eu(3))) void gated_bwd_kernel(GatedParams p, Gat
           for (int i = 0; i < GatedRaw<ES, V>::kWords; ++i) rd[u].w[i] = 0;
         }
         if (whole() || u < n) {
-          if (kWhole) rx[u] = gated_load<ES, V>(x + (t + u) * p.xsl * ES, at.ch * ES);
+          rx[u] = gated_load<ES, V>(x + (t + u) * p.xsl * ES, at.ch * ES);
           rg[u] = gated_load<ES, V>(g + (t + u) * p.gsl * ES, at.ch * ES);
           if (whole() || d.dy != nullptr) rd[u] = gated_load<ES, V>(dy + (t + u) * d.dysl * ES, at.ch * ES);
         }
@@ -77,12 +75,10 @@ __attribute__((amdgpu_waves_per_eu(3))) void gated_bwd_kernel(GatedParams p, Gat
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             gate_of(gated_value<T>(rg[u], i), a[u][i], na[u][i]);
-            if (kWhole) {
-              const float xv = gated_value<T>(rx[u], i);
-              const float prev = !whole() && bits >> u & 1 ? 0.f : h[i];
-              c[u][i] = (prev - xv) * (a[u][i] * na[u][i]);
-              h[i] = ffma(a[u][i], prev, na[u][i] * xv);
-            }
+            const float xv = gated_value<T>(rx[u], i);
+            const float prev = !whole() && bits >> u & 1 ? 0.f : h[i];
+            c[u][i] = (prev - xv) * (a[u][i] * na[u][i]);
+            h[i] = ffma(a[u][i], prev, na[u][i] * xv);
           }
           // (a scheduler free to work on all steps at once takes half as many registers
           // again for it)
@@ -90,7 +86,7 @@ __attribute__((amdgpu_waves_per_eu(3))) void gated_bwd_kernel(GatedParams p, Gat
         }
       }
       // the way back from 0, for what the wave passes on
-      if (NW > 1 || !kWhole) {
+      if constexpr (NW > 1) {
 #pragma unroll
         for (int u = K - 1; u >= 0; --u) {
           if (whole() || u < n) {
@@ -123,56 +119,114 @@ __attribute__((amdgpu_waves_per_eu(3))) void gated_bwd_kernel(GatedParams p, Gat
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float pw = share.prod[turn][w][lane * V + i];
-          l[i] = gated_join(pw, share.end[turn][w][lane * V + i], l[i]);
-          if (!kWhole) total[i] = gated_product(total[i], pw);
+          l[i] = gated_join(share.prod[turn][w][lane * V + i], share.end[turn][w][lane * V + i], l[i]);
         }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        from[i] = l[i];
-        if (!kWhole) {
-          l[i] = gated_join(prod[i], end[i], l[i]);
-          total[i] = gated_product(total[i], prod[i]);
+      for (int i = 0; i < V; ++i) from[i] = l[i];
+    }
+    auto again = [&](auto whole) {
+#pragma unroll
+      for (int u = K - 1; u >= 0; --u) {
+        if (whole() || u < n) {
+          const bool begin = !whole() && bits >> u & 1;
+          float ox[V], og[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float s = gated_value<T>(rd[u], i) + from[i];
+            ox[i] = s * na[u][i];
+            og[i] = s * c[u][i];
+            from[i] = begin ? 0.f : a[u][i] * s;
+          }
+          gated_store<T, V>(dx + (t + u) * p.D * ES, at.ch * ES, ox);
+          gated_store<T, V>(dg + (t + u) * p.D * ES, at.ch * ES, og);
         }
       }
+    };
+    if (full)
+      again(std::true_type{});
+    else
+      again(std::false_type{});
+    if constexpr (NW == 1) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) l[i] = from[i];
     }
-    if constexpr (kWhole) {
-      auto again = [&](auto whole) {
+    if (d.dh0 != nullptr && t == 0)
+      gated_store<RP_F32, V>(reinterpret_cast<char*>(d.dh0 + at.b * p.D), at.ch * 4, from);
+  }
+}
+
+// A chunk's (product, what it passes on) from behind: each wave walks its share of the
+// steps backwards.
+template <int T, int V, int NW>
+__global__ __launch_bounds__(kWave* NW) void gated_bwd_sum_kernel(GatedParams p, GatedGrad d) {
+  constexpr int K = kGatedK, ES = gated_es(T);
+  __shared__ GatedShare<V, NW> share;
+  const GatedAt<V> at(p);
+  if (at.c == 0) return;  // (nothing comes before the first)
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const char* g = static_cast<const char*>(p.g) + at.b * p.gsb * ES;
+  const char* dy = static_cast<const char*>(d.dy) + (d.dy != nullptr ? at.b * d.dysb * ES : 0);
+  const int64_t first = at.t0 + wave * (p.chunk / NW);
+  int64_t last = first + p.chunk / NW;
+  if (last > at.t1) last = at.t1;  // (the last chunk's shares are cut, or empty)
+  float prod[V], end[V];
 #pragma unroll
-        for (int u = K - 1; u >= 0; --u) {
-          if (whole() || u < n) {
-            const bool begin = !whole() && bits >> u & 1;
-            float ox[V], og[V];
+  for (int i = 0; i < V; ++i) {
+    prod[i] = 1.f;
+    end[i] = 0.f;
+  }
+  GatedRaw<ES, V> rg[K], rd[K];
+  uint32_t bits = 0;
+  int n = 0;
+  auto load = [&](int64_t t) {
+    n = last - t < K ? (int)(last - t) : K;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float s = gated_value<T>(rd[u], i) + from[i];
-              ox[i] = s * na[u][i];
-              og[i] = s * c[u][i];
-              from[i] = begin ? 0.f : a[u][i] * s;
-            }
-            gated_store<T, V>(dx + (t + u) * p.D * ES, at.ch * ES, ox);
-            gated_store<T, V>(dg + (t + u) * p.D * ES, at.ch * ES, og);
+    for (int u = 0; u < K; ++u) {
+      const int64_t s = u < n ? t + u : t;  // (past the end the first step again)
+      rg[u] = gated_load<ES, V>(g + s * p.gsl * ES, at.ch * ES);
+#pragma unroll
+      for (int i = 0; i < GatedRaw<ES, V>::kWords; ++i) rd[u].w[i] = 0;
+      if (d.dy != nullptr) rd[u] = gated_load<ES, V>(dy + s * d.dysl * ES, at.ch * ES);
+    }
+    bits = start_bits(p, at.b, t, n);
+  };
+  int64_t t = first + (last - first - 1) / K * K;
+  if (first < last) load(t);
+  for (; first < last && t >= first; t -= K) {
+    GatedRaw<ES, V> cg[K], cd[K];
+    const uint32_t now = bits;
+    const int m = n;
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+      cg[u] = rg[u];
+      cd[u] = rd[u];
+    }
+    if (t - K >= first) load(t - K);
+    auto walk = [&](auto whole) {
+#pragma unroll
+      for (int u = K - 1; u >= 0; --u) {
+        if (whole() || u < m) {
+          const bool begin = !whole() && now >> u & 1;
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float a, na;
+            gate_of(gated_value<T>(cg[u], i), a, na);
+            const float s = gated_value<T>(cd[u], i) + end[i];
+            end[i] = begin ? 0.f : a * s;
+            prod[i] = begin ? -0.f : prod[i] * a;
           }
         }
-      };
-      if (full)
-        again(std::true_type{});
-      else
-        again(std::false_type{});
-      if constexpr (NW == 1) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) l[i] = from[i];
       }
-      if (d.dh0 != nullptr && t == 0)
-        gated_store<RP_F32, V>(reinterpret_cast<char*>(d.dh0 + at.b * p.D), at.ch * 4, from);
-    }
+    };
+    if (now == 0 && m == K)
+      walk(std::true_type{});
+    else
+      walk(std::false_type{});
   }
-  if (!kWhole && wave == 0) {
-    gated_store<RP_F32, V>(reinterpret_cast<char*>(slot), at.ch * 4, total);
-    gated_store<RP_F32, V>(reinterpret_cast<char*>(slot + p.D), at.ch * 4, l);
-  }
+  gated_leave<V, NW>(p, at.b, at.c, at.ch, lane, wave, true, prod, end, share);
 }
 
 namespace {
@@ -181,11 +235,15 @@ template <int T, int V, int NW>
 hipError_t run(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * p.nchunk * ((p.D + kWave * V - 1) / (kWave * V))));
   if (p.nchunk > 1) {
-    hipLaunchKernelGGL((gated_bwd_kernel<T, V, NW, false>), grid, dim3(kWave * NW), 0, st, p, g);
-    const hipError_t e = launch_gated_fold(p, g.dh, true, st);
-    if (e != hipSuccess) return e;
+    if constexpr (NW == kSplitWaves) {
+      hipLaunchKernelGGL((gated_bwd_sum_kernel<T, V, NW>), grid, dim3(kWave * NW), 0, st, p, g);
+      const hipError_t e = launch_gated_fold(p, g.dh, true, st);
+      if (e != hipSuccess) return e;
+    } else {
+      return hipErrorInvalidValue;
+    }
   }
-  hipLaunchKernelGGL((gated_bwd_kernel<T, V, NW, true>), grid, dim3(kWave * NW), 0, st, p, g);
+  hipLaunchKernelGGL((gated_bwd_kernel<T, V, NW>), grid, dim3(kWave * NW), 0, st, p, g);
   return hipGetLastError();
 }
 
@@ -194,6 +252,7 @@ hipError_t run_waves(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
 #define RP_CASE(NW) \
   if (p.nw == NW) return run<T, V, NW>(p, g, st);
   RP_GATED_WAVES(RP_CASE)
+  if constexpr (V == 1) RP_CASE(16)
 #undef RP_CASE
   return hipErrorInvalidValue;
 }
@@ -202,7 +261,7 @@ hipError_t run_waves(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
 
 hipError_t launch_gated_bwd(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
   if (p.dt == RP_F32) return run_waves<RP_F32, 1>(p, g, st);
-  if (gated_lane_channels(2, p.D) == 2)
+  if (p.v == 2)
     return p.dt == RP_BF16 ? run_waves<RP_BF16, 2>(p, g, st) : run_waves<RP_F16, 2>(p, g, st);
   return p.dt == RP_BF16 ? run_waves<RP_BF16, 1>(p, g, st) : run_waves<RP_F16, 1>(p, g, st);
 }

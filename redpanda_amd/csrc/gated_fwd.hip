@@ -16,23 +16,20 @@
 
 namespace rp {
 
-// kWhole: writes y (and the checkpoints); else only the chunks' (product, end).
-template <int T, int V, int NW, bool kWhole>
+template <int T, int V, int NW>
 __global__ __launch_bounds__(kWave* NW) void gated_fwd_kernel(GatedParams p) {
   constexpr int K = kGatedK, ES = gated_es(T);
   __shared__ GatedShare<V, NW> share;
   const GatedAt<V> at(p);
-  if (!kWhole && at.c + 1 == p.nchunk) return;  // (nothing comes behind the last)
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  float h[V], total[V];  // the state that enters the waves' steps; the chunk's product
-  float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D;
+  float h[V];  // the state that enters the waves' steps
+  const float* slot = p.agg + ((at.b * p.nchunk + at.c) * 2) * p.D;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     h[i] = 0.f;
-    total[i] = 1.f;
-    if (kWhole && p.nchunk > 1) h[i] = slot[at.ch + i];
-    if (kWhole && p.nchunk == 1 && p.h0 != nullptr) h[i] = p.h0[at.b * p.D + at.ch + i];
+    if (p.nchunk > 1) h[i] = slot[at.ch + i];
+    if (p.nchunk == 1 && p.h0 != nullptr) h[i] = p.h0[at.b * p.D + at.ch + i];
   }
   const char* x = static_cast<const char*>(p.x) + at.b * p.xsb * ES;
   const char* g = static_cast<const char*>(p.g) + at.b * p.gsb * ES;
@@ -95,9 +92,7 @@ __global__ __launch_bounds__(kWave* NW) void gated_fwd_kernel(GatedParams p) {
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float pw = share.prod[turn][w][lane * V + i];
-          h[i] = gated_join(pw, share.end[turn][w][lane * V + i], h[i]);
-          if (!kWhole) total[i] = gated_product(total[i], pw);
+          h[i] = gated_join(share.prod[turn][w][lane * V + i], share.end[turn][w][lane * V + i], h[i]);
         }
       }
     } else {
@@ -105,38 +100,92 @@ __global__ __launch_bounds__(kWave* NW) void gated_fwd_kernel(GatedParams p) {
       for (int i = 0; i < V; ++i) {
         from[i] = h[i];
         h[i] = gated_join(prod[i], end[i], h[i]);
-        if (!kWhole) total[i] = gated_product(total[i], prod[i]);
       }
     }
-    if constexpr (kWhole) {
-      if (n > 0 && p.ckpt != nullptr) {
-        float* to = p.ckpt + (at.b * ((p.L + K - 1) / K) + t / K) * p.D;
-        gated_store<RP_F32, V>(reinterpret_cast<char*>(to), at.ch * 4, from);
-      }
-      auto again = [&](auto whole) {
+    if (n > 0 && p.ckpt != nullptr) {
+      float* to = p.ckpt + (at.b * ((p.L + K - 1) / K) + t / K) * p.D;
+      gated_store<RP_F32, V>(reinterpret_cast<char*>(to), at.ch * 4, from);
+    }
+    auto again = [&](auto whole) {
 #pragma unroll
-        for (int u = 0; u < K; ++u) {
-          if (whole() || u < n) {
-            const bool begin = !whole() && bits >> u & 1;
+      for (int u = 0; u < K; ++u) {
+        if (whole() || u < n) {
+          const bool begin = !whole() && bits >> u & 1;
 #pragma unroll
-            for (int i = 0; i < V; ++i) from[i] = ffma(a[u][i], begin ? 0.f : from[i], in[u][i]);
-            gated_store<T, V>(y + (t + u) * p.D * ES, at.ch * ES, from);
-          }
+          for (int i = 0; i < V; ++i) from[i] = ffma(a[u][i], begin ? 0.f : from[i], in[u][i]);
+          gated_store<T, V>(y + (t + u) * p.D * ES, at.ch * ES, from);
         }
-      };
-      if (full)
-        again(std::true_type{});
-      else
-        again(std::false_type{});
-      // the wave with the last step has the last state, as its own steps give it
-      if (p.h_last != nullptr && t < p.L && t + n == p.L)
-        gated_store<RP_F32, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D), at.ch * 4, from);
+      }
+    };
+    if (full)
+      again(std::true_type{});
+    else
+      again(std::false_type{});
+    // the wave with the last step has the last state, as its own steps give it
+    if (p.h_last != nullptr && t < p.L && t + n == p.L)
+      gated_store<RP_F32, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D), at.ch * 4, from);
+  }
+}
+
+// A chunk's (product, end): each wave walks its share of the steps, the next 16 loaded
+// while it works on the present ones.
+template <int T, int V, int NW>
+__global__ __launch_bounds__(kWave* NW) void gated_fwd_sum_kernel(GatedParams p) {
+  constexpr int K = kGatedK, ES = gated_es(T);
+  __shared__ GatedShare<V, NW> share;
+  const GatedAt<V> at(p);
+  if (at.c + 1 == p.nchunk) return;  // (nothing comes behind the last)
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const char* x = static_cast<const char*>(p.x) + at.b * p.xsb * ES;
+  const char* g = static_cast<const char*>(p.g) + at.b * p.gsb * ES;
+  // (every chunk but the last is whole: its shares are multiples of 16 steps)
+  const int64_t first = at.t0 + wave * (p.chunk / NW), last = first + p.chunk / NW;
+  float prod[V], end[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    prod[i] = 1.f;
+    end[i] = 0.f;
+  }
+  GatedRaw<ES, V> rx[K], rg[K];
+  uint32_t bits = 0;
+  auto load = [&](int64_t t) {
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+      rx[u] = gated_load<ES, V>(x + (t + u) * p.xsl * ES, at.ch * ES);
+      rg[u] = gated_load<ES, V>(g + (t + u) * p.gsl * ES, at.ch * ES);
     }
+    bits = start_bits(p, at.b, t, K);
+  };
+  load(first);
+  for (int64_t t = first; t < last; t += K) {
+    GatedRaw<ES, V> cx[K], cg[K];
+    const uint32_t now = bits;
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+      cx[u] = rx[u];
+      cg[u] = rg[u];
+    }
+    if (t + K < last) load(t + K);
+    auto walk = [&](auto whole) {
+#pragma unroll
+      for (int u = 0; u < K; ++u) {
+        const bool begin = !whole() && now >> u & 1;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float a, na;
+          gate_of(gated_value<T>(cg[u], i), a, na);
+          prod[i] = begin ? -0.f : prod[i] * a;
+          end[i] = ffma(a, begin ? 0.f : end[i], na * gated_value<T>(cx[u], i));
+        }
+      }
+    };
+    if (now == 0)
+      walk(std::true_type{});
+    else
+      walk(std::false_type{});
   }
-  if (!kWhole && wave == 0) {
-    gated_store<RP_F32, V>(reinterpret_cast<char*>(slot), at.ch * 4, total);
-    gated_store<RP_F32, V>(reinterpret_cast<char*>(slot + p.D), at.ch * 4, h);
-  }
+  gated_leave<V, NW>(p, at.b, at.c, at.ch, lane, wave, false, prod, end, share);
 }
 
 // Few steps (a rollout's single token): no stretch to share, one thread for 16 bytes of
@@ -223,14 +272,19 @@ hipError_t launch_gated_fold(const GatedParams& p, const float* in, bool backwar
 }
 
 int64_t gated_plan(GatedParams* p) {
-  const int V = gated_lane_channels(p->es, p->D);
-  const int64_t tiles = p->B * ((p->D + kWave * V - 1) / (kWave * V));
+  const int V = p->v = p->es == 2 && p->D >= 2 ? 2 : 1;
+  int64_t tiles = p->B * ((p->D + kWave * V - 1) / (kWave * V));
   // waves of a workgroup: until the card is full, or the sequence is
   int nw = 1;
   while (nw < 8 && nw * kGatedK < p->L && (tiles * nw < 8192 || nw < 4)) nw *= 2;
   int64_t n = 1;
-  if (tiles * nw < 2048 && p->L > 2 * kGatedK * nw) {
-    nw = 4;
+  if (tiles * nw < 2048 && p->L <= 16 * kGatedK) {
+    // few channels and few steps: as many waves as there are stretches of 16, and as
+    // many lanes as channels
+    p->v = 1;
+    while (nw < 16 && nw * kGatedK < p->L) nw *= 2;
+  } else if (tiles * nw < 2048) {
+    nw = kSplitWaves;
     n = (8192 / nw + tiles - 1) / tiles;
     const int64_t most = (p->L + kGatedK * nw - 1) / (kGatedK * nw);
     if (n > most) n = most;
@@ -248,11 +302,15 @@ template <int T, int V, int NW>
 hipError_t run(const GatedParams& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * p.nchunk * ((p.D + kWave * V - 1) / (kWave * V))));
   if (p.nchunk > 1) {
-    hipLaunchKernelGGL((gated_fwd_kernel<T, V, NW, false>), grid, dim3(kWave * NW), 0, st, p);
-    const hipError_t e = launch_gated_fold(p, p.h0, false, st);
-    if (e != hipSuccess) return e;
+    if constexpr (NW == kSplitWaves) {
+      hipLaunchKernelGGL((gated_fwd_sum_kernel<T, V, NW>), grid, dim3(kWave * NW), 0, st, p);
+      const hipError_t e = launch_gated_fold(p, p.h0, false, st);
+      if (e != hipSuccess) return e;
+    } else {
+      return hipErrorInvalidValue;
+    }
   }
-  hipLaunchKernelGGL((gated_fwd_kernel<T, V, NW, true>), grid, dim3(kWave * NW), 0, st, p);
+  hipLaunchKernelGGL((gated_fwd_kernel<T, V, NW>), grid, dim3(kWave * NW), 0, st, p);
   return hipGetLastError();
 }
 
@@ -268,6 +326,7 @@ hipError_t run_waves(const GatedParams& p, hipStream_t st) {
 #define RP_CASE(NW) \
   if (p.nw == NW) return run<T, V, NW>(p, st);
   RP_GATED_WAVES(RP_CASE)
+  if constexpr (V == 1) RP_CASE(16)
 #undef RP_CASE
   return hipErrorInvalidValue;
 }
@@ -281,7 +340,7 @@ hipError_t launch_gated_fwd(const GatedParams& p, hipStream_t st) {
                              : run_few<RP_F16, 4>(p, st);
   }
   if (p.dt == RP_F32) return run_waves<RP_F32, 1>(p, st);
-  if (gated_lane_channels(2, p.D) == 2)
+  if (p.v == 2)
     return p.dt == RP_BF16 ? run_waves<RP_BF16, 2>(p, st) : run_waves<RP_F16, 2>(p, st);
   return p.dt == RP_BF16 ? run_waves<RP_BF16, 1>(p, st) : run_waves<RP_F16, 1>(p, st);
 }

@@ -97,6 +97,7 @@ struct GatedParams {
   float* h_last;     // (B, D) or null
   float* ckpt;       // (B, ceil(L / kGatedK), D) or null: the state before every 16th step
   float* agg;        // workspace of gated_work_floats
+  int v;             // channels of a lane
   int nw;            // waves of a workgroup
   int nchunk;        // time chunks, each of `chunk` steps (a multiple of 16 nw)
   int64_t chunk;
@@ -109,7 +110,7 @@ struct GatedGrad {
   void* dg;
   float* dh0;        // (B, D) or null
 };
-// Sets p.nw, p.nchunk and p.chunk; the floats of workspace that p.agg needs.
+// Sets p.v, p.nw, p.nchunk and p.chunk; the floats of workspace that p.agg needs.
 int64_t gated_plan(GatedParams* p);
 hipError_t launch_gated_fwd(const GatedParams& p, hipStream_t st);
 hipError_t launch_gated_bwd(const GatedParams& p, const GatedGrad& g, hipStream_t st);

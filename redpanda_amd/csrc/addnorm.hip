@@ -202,26 +202,27 @@ namespace {
 
 unsigned row_grid(int64_t rows) { return (unsigned)(rows < (1 << 20) ? rows : (1 << 20)); }
 
-// Workgroups of a launch whose groups of G lanes walk rows.
+// Workgroups of a launch whose groups of G lanes walk rows: as few as walk as many rows
+// each as `most` would.
 unsigned walk_grid(int64_t rows, int G, int most) {
   const int groups = norm_threads(G) / G;
-  const int64_t n = (rows + groups - 1) / groups;
-  return (unsigned)(n < most ? n : most);
+  const int64_t n = (rows + groups - 1) / groups, turns = (n + most - 1) / most;
+  return (unsigned)(turns > 0 ? (n + turns - 1) / turns : 0);
 }
 
 }  // namespace
 
-int addnorm_parts(int64_t rows, int64_t d, int es_s, int es_out) {
+static int addnorm_parts(int64_t rows, int64_t d) {
   const int G = addnorm_group(d);
-  if (G != 0) return (int)walk_grid(rows, G, addnorm_workgroups_bwd(d, es_s, es_out));
+  if (G != 0) return (int)walk_grid(rows, G, addnorm_workgroups_bwd(d));
   const int64_t tiles = (d + 8 * kWave - 1) / (8 * kWave);
   const int64_t n = (rows + 4 * kWaves - 1) / (4 * kWaves);
   const int64_t most = (2048 + tiles - 1) / tiles;
   return (int)(n < most ? n : most);
 }
 
-int64_t addnorm_work_floats(int64_t rows, int64_t d, int es_s, int es_out) {
-  return (int64_t)addnorm_parts(rows, d, es_s, es_out) * d + (addnorm_group(d) == 0 ? rows : 0);
+int64_t addnorm_work_floats(int64_t rows, int64_t d) {
+  return (int64_t)addnorm_parts(rows, d) * d + (addnorm_group(d) == 0 ? rows : 0);
 }
 
 hipError_t launch_addnorm_fwd(const AddNormParams& p, hipStream_t st) {
@@ -229,8 +230,10 @@ hipError_t launch_addnorm_fwd(const AddNormParams& p, hipStream_t st) {
   const int G = addnorm_group(p.d);
   if (G != 0) {
     const unsigned wg = walk_grid(p.rows, G, addnorm_workgroups_fwd(p.d));
-    if (p.x == nullptr) return launch_addnorm_fwd1(p, wg, st);
-    return p.es_x == 4 ? launch_addnorm_fwd4(p, wg, st) : launch_addnorm_fwd2(p, wg, st);
+    if (p.x == nullptr) return launch_addnorm_fwd12(p, wg, st);
+    auto* launch = p.es_x == 4 ? (p.es_add == 4 ? launch_addnorm_fwd44 : launch_addnorm_fwd42)
+                               : (p.es_add == 4 ? launch_addnorm_fwd24 : launch_addnorm_fwd22);
+    return launch(p, wg, st);
   }
   hipLaunchKernelGGL(addnorm_fwd_kernel, dim3(row_grid(p.rows)), dim3(kThreads), 0, st, p);
   return hipGetLastError();
@@ -238,11 +241,12 @@ hipError_t launch_addnorm_fwd(const AddNormParams& p, hipStream_t st) {
 
 hipError_t launch_addnorm_bwd(const AddNormParams& p, const AddNormGrad& g, hipStream_t st) {
   const int es_s = p.x == nullptr ? 1 : p.es_sum;
-  const int n = addnorm_parts(p.rows, p.d, es_s, p.es_out);
+  const int n = addnorm_parts(p.rows, p.d);
   if (p.rows > 0 && addnorm_group(p.d) != 0) {
-    auto* launch = es_s == 4   ? (p.es_out == 4 ? launch_addnorm_bwd44 : launch_addnorm_bwd42)
-                   : es_s == 2 ? (p.es_out == 4 ? launch_addnorm_bwd24 : launch_addnorm_bwd22)
-                               : (p.es_out == 4 ? launch_addnorm_bwd14 : launch_addnorm_bwd12);
+    auto* launch = es_s == 4   ? (p.es_out == 4 ? launch_addnorm_bwd444 : launch_addnorm_bwd424)
+                   : es_s == 2 ? (p.es_out == 4 ? launch_addnorm_bwd242 : launch_addnorm_bwd222)
+                   : p.es_sum == 4 ? (p.es_out == 4 ? launch_addnorm_bwd144 : launch_addnorm_bwd124)
+                                   : (p.es_out == 4 ? launch_addnorm_bwd142 : launch_addnorm_bwd122);
     const hipError_t e = launch(p, g, (unsigned)n, st);
     if (e != hipSuccess) return e;
   } else if (p.rows > 0) {

@@ -45,32 +45,6 @@ __device__ __forceinline__ void load_kept(const NormCols<G, NB>& c, const int8_t
   }
 }
 
-// Rows whose element size is known when the kernel runs, in the wider form.
-template <int G, int NB>
-__device__ __forceinline__ void load_either(const NormCols<G, NB>& c, const char* row, int es,
-                                            Raw8<4> (&r)[NB]) {
-  if (es == 4) {
-    c.template load<4>(row, r);
-  } else {
-    Raw8<2> h[NB];
-    c.template load<2>(row, h);
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[j].w[i] = h[j].w[i];
-  }
-}
-__device__ __forceinline__ void either_floats(const Raw8<4>& r, int dtype, float (&v)[8]) {
-  if (dtype == RP_F32) {
-    to_floats(r, dtype, v);
-  } else {
-    Raw8<2> h;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h.w[i] = r.w[i];
-    to_floats(h, dtype, v);
-  }
-}
-
 // v rounded to a type and back.
 __device__ __forceinline__ void round_to(int dtype, float (&v)[8]) {
   if (dtype == RP_F32) return;
@@ -80,8 +54,8 @@ __device__ __forceinline__ void round_to(int dtype, float (&v)[8]) {
   to_floats(h, dtype, v);
 }
 
-// ES: bytes of an element of x; 1: the rows are held in 8 bits.
-template <int ES, int G, int NB>
+// ES: bytes of an element of x (1: the rows are held in 8 bits), EA: of add.
+template <int ES, int EA, int G, int NB>
 __global__ __launch_bounds__(norm_threads(G)) void addnorm_fwd_rows_kernel(AddNormParams p) {
   constexpr int kW = G > kWave ? G / kWave : 1;
   __shared__ float buf[2][kW][1];
@@ -93,14 +67,14 @@ __global__ __launch_bounds__(norm_threads(G)) void addnorm_fwd_rows_kernel(AddNo
   float w[NB][8];
   cols.load_weight(p.w, 1.f, 1.f, w);
   AnyRow<ES> rx[NB];
-  Raw8<4> ra[NB];
+  Raw8<EA> ra[NB];
   auto load = [&](int64_t row) {
     if constexpr (ES == 1)
       load_kept(cols, p.q8 + row * p.d, p.e8 + row * ne, rx);
     else
       load_any<ES>(cols, static_cast<const char*>(p.x) + row * p.xsr * ES, rx);
     if (ES != 1 && p.add != nullptr)
-      load_either(cols, static_cast<const char*>(p.add) + row * p.asr * p.es_add, p.es_add, ra);
+      cols.template load<EA>(static_cast<const char*>(p.add) + row * p.asr * EA, ra);
   };
   load(at.row);
   for (int it = 0; at.row < p.rows; at.row += at.step, it ^= 1) {
@@ -112,7 +86,7 @@ __global__ __launch_bounds__(norm_threads(G)) void addnorm_fwd_rows_kernel(AddNo
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           float a[8];
-          either_floats(ra[j], p.dt_add, a);
+          to_floats(ra[j], p.dt_add, a);
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[j][i] += a[i];
           round_to(p.dt_sum, v[j]);
@@ -153,8 +127,9 @@ __global__ __launch_bounds__(norm_threads(G)) void addnorm_fwd_rows_kernel(AddNo
 }
 
 // ds to dx and dadd, and the workgroup's sums of g xh over its rows to
-// part[workgroup].  ES: bytes of an element of the rows s (1: in 8 bits), EO: of dout.
-template <int ES, int EO, int G, int NB>
+// part[workgroup].  ES: bytes of an element of the rows s (1: in 8 bits), EO: of dout,
+// ED: of dsum (ES, but for rows in 8 bits).
+template <int ES, int EO, int ED, int G, int NB>
 __global__ __launch_bounds__(norm_threads(G)) void addnorm_bwd_rows_kernel(AddNormParams p,
                                                                            AddNormGrad g) {
   constexpr int kW = G > kWave ? G / kWave : 1;
@@ -164,11 +139,20 @@ __global__ __launch_bounds__(norm_threads(G)) void addnorm_bwd_rows_kernel(AddNo
   const NormCols<G, NB> cols(at.g, p.d);
   const float invd = 1.f / (float)cols.d;
   const int64_t ne = (p.d + kPackBlock - 1) / kPackBlock;
+  // 1024 threads have 128 registers each: there the weights are read for each row, no
+  // row is read ahead, and the columns' sums are in LDS
+  constexpr bool kAhead = G < 1024;
+  __shared__ float dw_lds[kAhead ? 1 : 8 * NB][kAhead ? 1 : G];
   float w[NB][8], dw[NB][8] = {};
-  cols.load_weight(p.w, 1.f, 1.f, w);
+  if constexpr (kAhead) {
+    cols.load_weight(p.w, 1.f, 1.f, w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8 * NB; ++i) dw_lds[i][at.g] = 0.f;
+  }
   AnyRow<ES> rx[NB];
   Raw8<EO> rg[NB];
-  Raw8<4> rd[NB];
+  Raw8<ED> rd[NB];
   auto load = [&](int64_t row) {
     if constexpr (ES == 1)
       load_kept(cols, p.q8 + row * p.d, p.e8 + row * ne, rx);
@@ -176,23 +160,29 @@ __global__ __launch_bounds__(norm_threads(G)) void addnorm_bwd_rows_kernel(AddNo
       load_any<ES>(cols, static_cast<const char*>(p.x) + row * p.xsr * ES, rx);
     cols.template load<EO>(static_cast<const char*>(g.dout) + row * g.dosr * EO, rg);
     if (g.dsum != nullptr)
-      load_either(cols, static_cast<const char*>(g.dsum) + row * g.dssr * p.es_sum, p.es_sum, rd);
+      cols.template load<ED>(static_cast<const char*>(g.dsum) + row * g.dssr * ED, rd);
   };
-  if (at.row < p.rows) load(at.row);
+  if (kAhead && at.row < p.rows) load(at.row);
   for (int it = 0; at.row < p.rows; at.row += at.step, it ^= 1) {
+    if constexpr (!kAhead) {
+      load(at.row);
+      const float* pw = p.w;
+      asm volatile("" : "+s"(pw));  // (or the weights would be read once, and kept)
+      cols.load_weight(pw, 1.f, 1.f, w);
+    }
     float v[NB][8], q[NB][8], d[NB][8];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       rx[j].floats(p.dt_sum, v[j]);
       to_floats(rg[j], p.dt_out, q[j]);
       if (g.dsum != nullptr) {
-        either_floats(rd[j], p.dt_sum, d[j]);
+        to_floats(rd[j], p.dt_sum, d[j]);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) d[j][i] = 0.f;
       }
     }
-    if (at.row + at.step < p.rows) load(at.row + at.step);
+    if (kAhead && at.row + at.step < p.rows) load(at.row + at.step);
     // mean(q xh) = r sum(q s) / d, so that one look at the row gives r and it
     float s[2] = {0.f, 0.f};
 #pragma unroll
@@ -210,7 +200,10 @@ __global__ __launch_bounds__(norm_threads(G)) void addnorm_bwd_rows_kernel(AddNo
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float xh = v[j][i] * r;
-        dw[j][i] = ffma(q[j][i], xh, dw[j][i]);
+        if constexpr (kAhead)
+          dw[j][i] = ffma(q[j][i], xh, dw[j][i]);
+        else
+          dw_lds[j * 8 + i][at.g] = ffma(q[j][i], xh, dw_lds[j * 8 + i][at.g]);
         d[j][i] = ffma(ffma(-xh, m, q[j][i] * w[j][i]), r, d[j][i]);
       }
     if (g.dx != nullptr)
@@ -219,6 +212,12 @@ __global__ __launch_bounds__(norm_threads(G)) void addnorm_bwd_rows_kernel(AddNo
       cols.store(static_cast<char*>(g.dadd) + at.row * p.d * p.es_add, p.dt_add, d);
   }
   if (g.dw == nullptr) return;
+  if constexpr (!kAhead) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dw[j][i] = dw_lds[j * 8 + i][at.g];
+  }
   // the groups' sums: over a wave's groups by lane exchanges, then wave by wave
   // through LDS in order
   float* part = g.part + (int64_t)blockIdx.x * p.d;
@@ -263,21 +262,26 @@ inline int addnorm_group(int64_t d) {
   return 0;
 }
 
-// Workgroups that a launch fills the card with.
+// Workgroups that a launch fills the card with: as many as its registers let be
+// resident.
 inline int addnorm_workgroups_fwd(int64_t d) {
   const int G = addnorm_group(d);
-  return G > 256 ? (G == 1024 ? 256 : 512) : 1024;
+  if (G > 256) return G == 1024 ? 256 : 512;
+  const int nb = (int)((d + 8 * G - 1) / (8 * G));
+  return 256 * (nb == 1 ? 7 : nb == 2 ? 5 : G < kWave ? 3 : 4);
 }
-inline int addnorm_workgroups_bwd(int64_t d, int es_s, int es_out) {
+inline int addnorm_workgroups_bwd(int64_t d) {
   const int G = addnorm_group(d);
-  return G > 256 ? 256 : 512;
+  if (G > 256) return 256;
+  const int nb = (int)((d + 8 * G - 1) / (8 * G));
+  return 256 * (nb == 1 ? 5 : nb == 2 ? 3 : 2);
 }
 
-template <int ES>
+template <int ES, int EA>
 hipError_t launch_addnorm_fwd_rows(const AddNormParams& p, unsigned wg, hipStream_t st) {
 #define RP_CASE(G, NB)                                                                          \
   if (p.d <= G * NB * 8) {                                                                      \
-    hipLaunchKernelGGL((addnorm_fwd_rows_kernel<ES, G, NB>), dim3(wg), dim3(norm_threads(G)), 0, \
+    hipLaunchKernelGGL((addnorm_fwd_rows_kernel<ES, EA, G, NB>), dim3(wg), dim3(norm_threads(G)), 0, \
                        st, p);                                                                  \
     return hipGetLastError();                                                                   \
   }
@@ -286,12 +290,12 @@ hipError_t launch_addnorm_fwd_rows(const AddNormParams& p, unsigned wg, hipStrea
   return hipErrorInvalidValue;
 }
 
-template <int ES, int EO>
+template <int ES, int EO, int ED>
 hipError_t launch_addnorm_bwd_rows(const AddNormParams& p, const AddNormGrad& g, unsigned wg,
                                    hipStream_t st) {
 #define RP_CASE(G, NB)                                                                    \
   if (p.d <= G * NB * 8) {                                                                \
-    hipLaunchKernelGGL((addnorm_bwd_rows_kernel<ES, EO, G, NB>), dim3(wg),                \
+    hipLaunchKernelGGL((addnorm_bwd_rows_kernel<ES, EO, ED, G, NB>), dim3(wg),                \
                        dim3(norm_threads(G)), 0, st, p, g);                               \
     return hipGetLastError();                                                             \
   }
@@ -300,19 +304,25 @@ hipError_t launch_addnorm_bwd_rows(const AddNormParams& p, const AddNormGrad& g,
   return hipErrorInvalidValue;
 }
 
-// The instantiations, one file each (element sizes of the rows and of the gradient).
-#define RP_ADDNORM_FWD(ES) hipError_t launch_addnorm_fwd##ES(const AddNormParams& p, unsigned wg, hipStream_t st)
-#define RP_ADDNORM_BWD(ES, EO)                                                                     \
-  hipError_t launch_addnorm_bwd##ES##EO(const AddNormParams& p, const AddNormGrad& g, unsigned wg, \
-                                        hipStream_t st)
-RP_ADDNORM_FWD(4);
-RP_ADDNORM_FWD(2);
-RP_ADDNORM_FWD(1);
-RP_ADDNORM_BWD(4, 4);
-RP_ADDNORM_BWD(4, 2);
-RP_ADDNORM_BWD(2, 4);
-RP_ADDNORM_BWD(2, 2);
-RP_ADDNORM_BWD(1, 4);
-RP_ADDNORM_BWD(1, 2);
+// The instantiations, one file each: element sizes of the rows and of add; of the rows,
+// of dout and of dsum.
+#define RP_ADDNORM_FWD(ES, EA) \
+  hipError_t launch_addnorm_fwd##ES##EA(const AddNormParams& p, unsigned wg, hipStream_t st)
+#define RP_ADDNORM_BWD(ES, EO, ED)                                                                 \
+  hipError_t launch_addnorm_bwd##ES##EO##ED(const AddNormParams& p, const AddNormGrad& g, unsigned wg, \
+                                            hipStream_t st)
+RP_ADDNORM_FWD(4, 4);
+RP_ADDNORM_FWD(4, 2);
+RP_ADDNORM_FWD(2, 4);
+RP_ADDNORM_FWD(2, 2);
+RP_ADDNORM_FWD(1, 2);
+RP_ADDNORM_BWD(4, 4, 4);
+RP_ADDNORM_BWD(4, 2, 4);
+RP_ADDNORM_BWD(2, 4, 2);
+RP_ADDNORM_BWD(2, 2, 2);
+RP_ADDNORM_BWD(1, 4, 4);
+RP_ADDNORM_BWD(1, 4, 2);
+RP_ADDNORM_BWD(1, 2, 4);
+RP_ADDNORM_BWD(1, 2, 2);
 
 }  // namespace rp

@@ -1502,24 +1502,30 @@ rp::EmbedParams embed_params(const rp_embedding_args* a) {
 }
 
 struct EmbedWork {
-  int64_t start, place, sorted, part, bytes;
+  int64_t start, place, sorted, part, pairs, segs, bytes;
 };
 
-EmbedWork embed_work(const rp_embedding_args* a) {
+EmbedWork embed_work(const rp_embedding_args* a, const rp::EmbedPlan& plan) {
   EmbedWork w;
   w.start = 0;
-  w.place = round_up((a->V + 1) * 4, 256);
+  w.place = round_up((plan.slots + 1) * 4, 256);
   w.sorted = w.place + round_up(a->N * 4, 256);
   w.part = w.sorted + round_up(a->N * 4, 256);
-  w.bytes = w.part + round_up(rp::embed_chunks(a->N) * 2 * a->d * 4, 256);
+  w.pairs = w.part + round_up(plan.shares * 2 * a->d * 4, 256);
+  w.segs = w.pairs + round_up(plan.parts * rp::kSplitPart * (int64_t)sizeof(rp::EmbedPair), 256);
+  w.bytes = w.segs + round_up(plan.parts * 17 * 4, 256);
   return w;
+}
+
+rp::EmbedPlan plan_of(const rp_embedding_args* a) {
+  return rp::embed_plan(a->N, a->V, a->d, (int)elem_size(a->dtype_out));
 }
 
 }  // namespace
 
 int64_t rp_embedding_work_bytes(const rp_embedding_args* a) {
   if (rp_embedding_check(a) != RP_OK) return -1;
-  return embed_work(a).bytes;
+  return embed_work(a, plan_of(a)).bytes;
 }
 
 int rp_embedding_fwd(const rp_embedding_args* a, void* stream) {
@@ -1549,7 +1555,8 @@ int rp_embedding_bwd(const rp_embedding_args* a, const rp_embedding_grad* g, voi
     return fail(RP_ERR_INVALID, "embedding grad: NULL or misaligned dw");
   if (a->N > 0 && !good_rows(g->dout, a->N, a->d, g->dout_sr, eo))
     return fail(RP_ERR_INVALID, "embedding grad: NULL or misaligned dout, or a row stride below d");
-  const EmbedWork at = embed_work(a);
+  const rp::EmbedPlan plan = plan_of(a);
+  const EmbedWork at = embed_work(a, plan);
   st = check_work(g->work, g->work_bytes, at.bytes, "embedding bwd");
   if (st != RP_OK) return st;
   const Span outs[2] = {{g->dw, a->V * a->d * ew}, {g->work, at.bytes}};
@@ -1561,11 +1568,14 @@ int rp_embedding_bwd(const rp_embedding_args* a, const rp_embedding_grad* g, voi
   char* work = static_cast<char*>(g->work);
   eg.dout = g->dout;
   eg.dosr = g->dout_sr;
+  eg.plan = plan;
   eg.dw = g->dw;
   eg.start = reinterpret_cast<int32_t*>(work + at.start);
   eg.place = reinterpret_cast<int32_t*>(work + at.place);
   eg.sorted = reinterpret_cast<int32_t*>(work + at.sorted);
   eg.part = reinterpret_cast<float*>(work + at.part);
+  eg.pairs = reinterpret_cast<rp::EmbedPair*>(work + at.pairs);
+  eg.segs = reinterpret_cast<int32_t*>(work + at.segs);
   hipError_t e = rp::launch_embed_bwd(embed_params(a), eg, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "embedding bwd launch");
   return RP_OK;
@@ -1666,8 +1676,7 @@ rp::AddNormParams addnorm_params(const rp_addnorm_args* a) {
 
 int64_t rp_addnorm_work_bytes(const rp_addnorm_args* a) {
   if (rp_addnorm_check(a) != RP_OK) return -1;
-  return round_up(4 * rp::addnorm_work_floats(a->rows, a->d, a->x ? (int)elem_size(a->dtype_sum) : 1,
-                                              (int)elem_size(a->dtype_out)), 256);
+  return round_up(4 * rp::addnorm_work_floats(a->rows, a->d), 256);
 }
 
 int rp_addnorm_fwd(const rp_addnorm_args* a, void* stream) {

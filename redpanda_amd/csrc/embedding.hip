@@ -1,20 +1,24 @@
 // Embedding: out[i] = scale w[ids[i]], and the table's gradient
 //     dw[v] = scale sum of dout[i] over the places i with ids[i] = v.
 //
-// Forward: one thread per eight columns of a place; the places' rows are written
-// once and the table's come from L2 where ids repeat.
+// Forward: eight columns of four places a thread, loads before stores; the places' rows
+// are written once and the table's come from L2 where ids repeat.
 //
 // Backward.  Tokens are far from uniform (a board's empty square is a quarter of
 // them), so the places are sorted by id first and the sums run over equal shares of
-// the sorted places, whatever the ids are; nothing is added by atomics, and the sums'
-// order is fixed:
-//   sort   workgroup g owns a range of ids and looks at all of them: how many lie
-//          below its range is where its places begin, its own are counted by id and
-//          written in order of id, then of place.  No workgroup waits for another.
-//   sum    a wave takes 32 sorted places and 256 columns, and adds rows while the
-//          id stays the same.  An id whose places end inside is written to dw, what
-//          may go on in the next share, or began in one before, to `part`.  Ids that
-//          do not occur get zeros.
+// the sorted places, whatever the ids are; no float is added by an atomic, and the
+// sums' order is fixed:
+//   split  (more than 8192 places) each 2048 places are put in order of their ids' low
+//          four bits, so that what follows looks at a sixteenth of them.
+//   sort   a workgroup owns a bucket, the ids of the same low bits (so that frequent ids
+//          next to each other fall to different ones), and looks at all ids, or those of
+//          its sixteenth: how many belong to buckets below it is where its places begin,
+//          its own are counted and written together, id by id.  No workgroup waits for
+//          another.
+//   sum    a wave takes a share of the sorted places and 16 bytes a lane of their rows,
+//          and adds while the id stays the same.  An id whose places end inside is
+//          written to dw, what may go on in the next share, or began in one before, to
+//          `part`.  Ids that do not occur get zeros.
 //   join   the share in which a divided id begins adds its pieces in order.
 
 #include "rp_rows.h"
@@ -25,67 +29,227 @@ namespace rp {
 namespace {
 
 constexpr int kSortWaves = 16;
-constexpr int kSortRange = 512;   // most ids of a workgroup's range
-constexpr int kChunk = 32;        // sorted places of a wave's share
-constexpr int kCols = 4 * kWave;  // columns of a wave's share
+constexpr int kSortRange = 512;  // most ids of a bucket
+constexpr int kSortList = 256;   // places that a wave remembers from its first look
+constexpr int kZeroRows = 32;    // ids that a wave looks at for absent ones
 
 template <typename Id>
 __device__ __forceinline__ int64_t id_at(const void* ids, int64_t i) {
   return static_cast<const Id*>(ids)[i];
 }
 
+// Buckets are the ids' low lg bits, ordered by the lowest four of them first.
+__device__ __forceinline__ int32_t bucket_of(const EmbedPlan& plan, int32_t id) {
+  return (id & 15) << (plan.lg - 4) | (id >> 4 & ((1 << (plan.lg - 4)) - 1));
+}
+__device__ __forceinline__ int32_t low_bits(const EmbedPlan& plan, int32_t bucket) {
+  return (bucket & ((1 << (plan.lg - 4)) - 1)) << 4 | bucket >> (plan.lg - 4);
+}
+__device__ __forceinline__ int64_t slot_of(const EmbedPlan& plan, int32_t id) {
+  return (int64_t)bucket_of(plan, id) * plan.range + (id >> plan.lg);
+}
+
 }  // namespace
 
-template <typename Id>
-__global__ __launch_bounds__(kThreads) void embed_fwd_kernel(EmbedParams p) {
-  const int64_t nb = (p.d + 7) / 8, n = p.N * nb;
-  for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < n;
-       e += (int64_t)gridDim.x * kThreads) {
-    // (32-bit division where it fits: a 64-bit one costs more than the row)
-    const int64_t i = n <= 0xffffffffll ? (int64_t)((uint32_t)e / (uint32_t)nb) : e / nb;
-    const int64_t col = (e - i * nb) * 8;
-    const int64_t id = id_at<Id>(p.ids, i);
-    float v[8] = {};
-    if (id >= 0 && id < p.V)
-      load8(static_cast<const char*>(p.w) + id * p.wsr * p.es_w, col, p.d, p.dt_w, v);
+template <typename Id, int ES>
+__global__ __launch_bounds__(kThreads) void embed_fwd_kernel(EmbedParams p, FastDiv blocks) {
+  constexpr int kRows = 4;
+  const int64_t n = p.N * (int64_t)blocks.n, step = (int64_t)gridDim.x * kThreads;
+  for (int64_t e0 = (int64_t)blockIdx.x * kThreads + threadIdx.x; e0 < n; e0 += kRows * step) {
+    int64_t at[kRows], id[kRows];
+    uint32_t col[kRows];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= p.scale;
-    store8(static_cast<char*>(p.out) + i * p.d * p.es_out, col, p.d, p.dt_out, v);
+    for (int k = 0; k < kRows; ++k) {
+      const int64_t e = e0 + k * step;
+      at[k] = -1;
+      if (e < n) {
+        at[k] = n <= 0x7fffffff ? (int64_t)blocks.div((uint32_t)e) : e / blocks.n;
+        col[k] = (uint32_t)(e - at[k] * blocks.n) * 8;
+        id[k] = id_at<Id>(p.ids, at[k]);
+      }
+    }
+    Raw8<ES> r[kRows];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+#pragma unroll
+      for (int i = 0; i < 2 * ES; ++i) r[k].w[i] = 0;
+      if (at[k] >= 0 && id[k] >= 0 && id[k] < p.V)
+        r[k] = load_raw8<ES>(static_cast<const char*>(p.w) + id[k] * p.wsr * ES, col[k], p.d);
+    }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (at[k] < 0) continue;
+      float v[8];
+      to_floats(r[k], p.dt_w, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= p.scale;
+      store8(static_cast<char*>(p.out) + at[k] * p.d * p.es_out, col[k], p.d, p.dt_out, v);
+    }
   }
 }
 
+// Workgroup: 2048 places to pairs[2048 workgroup ..], ordered by the ids' low four bits;
+// where each of the sixteen begins (and the last ends) to segs[workgroup].
 template <typename Id>
-__global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedParams p, EmbedGrad g,
-                                                                       int range) {
+__global__ __launch_bounds__(kThreads) void embed_split_kernel(EmbedParams p, EmbedGrad g) {
+  constexpr int kGroups = kSplitPart / kThreads;
+  __shared__ int32_t cnt[kWaves][16];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t part0 = (int64_t)blockIdx.x * kSplitPart, first = part0 + wave * (kSplitPart / kWaves);
+  if (lane < 16) cnt[wave][lane] = 0;
+  int32_t id[kGroups];
+#pragma unroll
+  for (int u = 0; u < kGroups; ++u) {
+    const int64_t i = first + u * kWave + lane;
+    const int64_t v = i < p.N ? id_at<Id>(p.ids, i) : -1;
+    id[u] = v >= 0 && v < p.V && v != p.pad ? (int32_t)v : -1;
+  }
+  // the lanes of the same low bits; and a lane's place among them
+  auto same = [&](int32_t v, int& rank) {
+    uint64_t m = __ballot(v >= 0);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const uint64_t set = __ballot(v >> b & 1);
+      m &= v >> b & 1 ? set : ~set;
+    }
+    rank = __popcll(m & ((1ull << lane) - 1));
+    return v >= 0 ? m : 0;
+  };
+#pragma unroll
+  for (int u = 0; u < kGroups; ++u) {
+    int rank;
+    const uint64_t m = same(id[u], rank);
+    if (m != 0 && rank == 0) atomicAdd(&cnt[wave][id[u] & 15], (int32_t)__popcll(m));
+  }
+  __syncthreads();
+  // wave 0's lanes 0 .. 63 are (low bits, wave) in order
+  if (threadIdx.x < kWave) {
+    const int32_t mine = cnt[lane % kWaves][lane / kWaves];
+    int32_t inc = mine;
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+      const int32_t o = __shfl_up(inc, m);
+      if (lane >= m) inc += o;
+    }
+    cnt[lane % kWaves][lane / kWaves] = inc - mine;
+    int32_t* segs = g.segs + (int64_t)blockIdx.x * 17;
+    if (lane % kWaves == 0) segs[lane / kWaves] = inc - mine;
+    if (lane == kWave - 1) segs[16] = inc;
+  }
+  __syncthreads();
+  EmbedPair* out = g.pairs + part0;
+#pragma unroll
+  for (int u = 0; u < kGroups; ++u) {
+    int rank;
+    const uint64_t m = same(id[u], rank);
+    if (m != 0) out[cnt[wave][id[u] & 15] + rank] = {id[u], (int32_t)(first + u * kWave + lane)};
+    // (read by all of its lanes before the first of them moves it on)
+    __builtin_amdgcn_wave_barrier();
+    if (m != 0 && rank == 0) atomicAdd(&cnt[wave][id[u] & 15], (int32_t)__popcll(m));
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Src: the ids' type, or EmbedPair behind the split.
+template <typename Src>
+__global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedParams p, EmbedGrad g) {
+  constexpr bool kSplit = std::is_same<Src, EmbedPair>::value;
   __shared__ int32_t cnt[kSortWaves][kSortRange];
-  __shared__ int32_t below[kSortWaves];
-  __shared__ int32_t scan[kSortWaves];
+  __shared__ int32_t list_at[kSortWaves][kSortList];
+  __shared__ uint16_t list_key[kSortWaves][kSortList];
+  __shared__ int32_t below[kSortWaves], scan[kSortWaves];
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t lo = (int64_t)blockIdx.x * range;
-  const int64_t hi = lo + range < p.V ? lo + range : p.V;
-  // each wave looks at its own stretch of places, in order
-  const int64_t stretch = ((p.N + kSortWaves * kWave - 1) / (kSortWaves * kWave)) * kWave;
-  const int64_t first = wave * stretch;
-  const int64_t last = first + stretch < p.N ? first + stretch : p.N;
+  const int range = g.plan.range, lg = g.plan.lg;
+  const int32_t bucket = (int32_t)blockIdx.x, sixteenth = bucket >> (lg - 4);
   for (int i = lane; i < range; i += kWave) cnt[wave][i] = 0;
-  int32_t under = 0;
-#pragma unroll 4
-  for (int64_t i = first + lane; i < last; i += kWave) {
-    const int64_t id = id_at<Id>(p.ids, i);
-    if (id >= lo && id < hi && id != p.pad) atomicAdd(&cnt[wave][id - lo], 1);
-    under += id >= 0 && id < lo && id != p.pad;
+  int32_t under = 0, listed = 0;
+
+  // f(each lane's id or -1, its place) for the places of the wave, 64 at a time, the
+  // loads of several groups together
+  auto look = [&](auto f) {
+    if constexpr (kSplit) {
+      constexpr int kParts = 4;
+      const int64_t each = (g.plan.parts + kSortWaves - 1) / kSortWaves;
+      const int64_t last = (wave + 1) * each < g.plan.parts ? (wave + 1) * each : g.plan.parts;
+      for (int64_t q0 = wave * each; q0 < last; q0 += kParts) {
+        int from[kParts], n[kParts], most = 0;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+          from[k] = n[k] = 0;
+          if (q0 + k < last) {
+            from[k] = g.segs[(q0 + k) * 17 + sixteenth];
+            n[k] = g.segs[(q0 + k) * 17 + sixteenth + 1] - from[k];
+          }
+          most = n[k] > most ? n[k] : most;
+        }
+        for (int j = 0; j < most; j += kWave) {
+          EmbedPair e[kParts];
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) {
+            e[k] = {-1, 0};
+            if (j + lane < n[k]) e[k] = g.pairs[(q0 + k) * kSplitPart + from[k] + j + lane];
+          }
+#pragma unroll
+          for (int k = 0; k < kParts; ++k)
+            if (j < n[k]) f(e[k].id, e[k].at);
+        }
+      }
+    } else {
+      constexpr int kGroups = 8;
+      const int64_t stretch = ((p.N + kSortWaves * kWave - 1) / (kSortWaves * kWave)) * kWave;
+      const int64_t first = wave * stretch;
+      const int64_t last = first + stretch < p.N ? first + stretch : p.N;
+      for (int64_t i0 = first; i0 < last; i0 += kGroups * kWave) {
+        int32_t id[kGroups];
+#pragma unroll
+        for (int u = 0; u < kGroups; ++u) {
+          const int64_t i = i0 + u * kWave + lane;
+          const int64_t v = i < last ? id_at<Src>(p.ids, i) : -1;
+          id[u] = v >= 0 && v < p.V && v != p.pad ? (int32_t)v : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kGroups; ++u) f(id[u], (int32_t)(i0 + u * kWave) + lane);
+      }
+    }
+  };
+
+  if constexpr (kSplit) {
+    // the sixteenths below come first
+    for (int64_t q = threadIdx.x; q < g.plan.parts; q += kSortWaves * kWave)
+      under += g.segs[q * 17 + sixteenth];
   }
+  look([&](int32_t id, int32_t at) {
+    const int32_t b = bucket_of(g.plan, id);
+    under += id >= 0 && b < bucket;
+    const bool in = id >= 0 && b == bucket;
+    uint64_t left = __ballot(in);
+    if (left == 0) return;
+    const int key = id >> lg;
+    const int to = listed + __popcll(left & ((1ull << lane) - 1));
+    if (in && to < kSortList) {
+      list_at[wave][to] = at;
+      list_key[wave][to] = (uint16_t)key;
+    }
+    listed += __popcll(left);
+    while (left != 0) {  // one turn for each id of the bucket among the 64
+      const int lead = __builtin_ctzll(left);
+      const int k = __builtin_amdgcn_readlane(key, lead);
+      const uint64_t those = __ballot(in && key == k);
+      if (lane == 0) cnt[wave][k] += __popcll(those);
+      left &= ~those;
+    }
+  });
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) under += __shfl_xor(under, m);
   if (lane == 0) below[wave] = under;
   __syncthreads();
-  // where each id's places begin: the places below the range, then the ids of the
-  // range in order (an inclusive scan over them, a thread each)
-  int32_t mine = 0;
+  // where each id's places begin: behind the buckets below, then id by id (an inclusive
+  // scan over them, a thread each)
+  int32_t count = 0;
   if ((int)threadIdx.x < range)
-    for (int w = 0; w < kSortWaves; ++w) mine += cnt[w][threadIdx.x];
-  int32_t inc = mine;
+    for (int w = 0; w < kSortWaves; ++w) count += cnt[w][threadIdx.x];
+  int32_t inc = count;
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) {
     const int32_t o = __shfl_up(inc, m);
@@ -98,10 +262,11 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
     base += below[w];
     if (w < wave) base += scan[w];
   }
-  int32_t at = base + inc - mine;
   if ((int)threadIdx.x < range) {
-    if (lo + threadIdx.x < hi) g.start[lo + threadIdx.x] = at;
-    if (lo + threadIdx.x == p.V - 1) g.start[p.V] = at + mine;
+    int32_t at = base + inc - count;
+    const int64_t slot = (int64_t)bucket * range + threadIdx.x;
+    g.start[slot] = at;
+    if (slot == g.plan.slots - 1) g.start[slot + 1] = at + count;
     for (int w = 0; w < kSortWaves; ++w) {
       const int32_t c = cnt[w][threadIdx.x];
       cnt[w][threadIdx.x] = at;
@@ -109,89 +274,100 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
     }
   }
   __syncthreads();
-  for (int64_t i0 = first; i0 < last; i0 += kWave) {
-    const int64_t i = i0 + lane;
-    const int64_t id = i < last ? id_at<Id>(p.ids, i) : -1;
-    const bool in = id >= lo && id < hi && id != p.pad;
+  // each wave's places, from its list or, where that was too short, by another look; the
+  // running place of the last id is kept in a register
+  const int32_t low = low_bits(g.plan, bucket);
+  int last_key = -1, next = 0;
+  auto place = [&](int32_t i, int key, bool in) {
     uint64_t left = __ballot(in);
-    while (left != 0) {  // one turn for each id of the range among the 64
+    while (left != 0) {
       const int lead = __builtin_ctzll(left);
-      const int key = __builtin_amdgcn_readlane((int)(id - lo), lead);
-      const bool same = in && (int)(id - lo) == key;
-      const uint64_t those = __ballot(same);
-      const int32_t to = cnt[wave][key];
-      if (same) {
-        const int32_t pos = to + __popcll(those & ((1ull << lane) - 1));
-        g.place[pos] = (int32_t)i;
-        g.sorted[pos] = (int32_t)id;
+      const int k = __builtin_amdgcn_readlane(key, lead);
+      const uint64_t those = __ballot(in && key == k);
+      if (k != last_key) {
+        if (lane == 0 && last_key >= 0) cnt[wave][last_key] = next;
+        last_key = k;
+        next = __builtin_amdgcn_readfirstlane(cnt[wave][k]);
       }
-      if (lane == lead) cnt[wave][key] = to + __popcll(those);
+      if (in && key == k) {
+        const int32_t pos = next + __popcll(those & ((1ull << lane) - 1));
+        g.place[pos] = i;
+        g.sorted[pos] = (k << lg) | low;
+      }
+      next += __popcll(those);
       left &= ~those;
     }
+  };
+  if (listed <= kSortList) {
+    for (int j = 0; j < listed; j += kWave) {
+      const bool in = j + lane < listed;
+      place(in ? list_at[wave][j + lane] : 0, in ? list_key[wave][j + lane] : 0, in);
+    }
+  } else {
+    look([&](int32_t id, int32_t at) {
+      place(at, id >> lg, id >= 0 && bucket_of(g.plan, id) == bucket);
+    });
   }
 }
 
 namespace {
 
-// Four elements at `col` of a row of d (zeros at and past d), as stored.
+// 16 bytes of a row as stored, C columns, from `col` on (zeros at and past d).
 template <int ES>
-struct Raw4 {
-  uint32_t w[ES];
+struct Row16 {
+  static constexpr int kCols = 16 / ES;
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const char* row, int64_t col, int64_t d) {
+    if (col + kCols <= d) {
+      const u32x4_any v = *reinterpret_cast<const u32x4_any*>(row + col * ES);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = 0;
+#pragma unroll
+      for (int i = 0; i < kCols - 1; ++i) {
+        if (col + i >= d) break;
+        if constexpr (ES == 4)
+          w[i] = reinterpret_cast<const uint32_t*>(row)[col + i];
+        else
+          w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[col + i] << (16 * (i & 1));
+      }
+    }
+  }
+  __device__ __forceinline__ void add_to(float (&v)[kCols], int dtype) const {
+    if constexpr (ES == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(w[i]);
+    } else {
+      Raw8<2> r;
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.w[i] = w[i];
+      to_floats(r, dtype, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += f[i];
+    }
+  }
 };
 
-template <int ES>
-__device__ __forceinline__ Raw4<ES> load4(const char* row, int64_t col, int64_t d) {
-  Raw4<ES> r;
-  if (col + 4 <= d) {
-    if constexpr (ES == 4) {
-      const u32x4_any v = *reinterpret_cast<const u32x4_any*>(row + col * 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r.w[i] = v[i];
-    } else {
-      const u32x2_any v = *reinterpret_cast<const u32x2_any*>(row + col * 2);
-      r.w[0] = v[0];
-      r.w[1] = v[1];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < ES; ++i) r.w[i] = 0;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      if (col + i >= d) break;
-      if constexpr (ES == 4)
-        r.w[i] = reinterpret_cast<const uint32_t*>(row)[col + i];
-      else
-        r.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[col + i] << (16 * (i & 1));
-    }
-  }
-  return r;
+__device__ __forceinline__ void store_cols(void* row, int64_t col, int64_t d, int dtype,
+                                           const float (&v)[8]) {
+  store8(row, col, d, dtype, v);
 }
-
-template <int ES>
-__device__ __forceinline__ void add4(const Raw4<ES>& r, int dtype, float (&v)[4]) {
-  if constexpr (ES == 4) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(r.w[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] += cvt_raw(r.w[i / 2] >> (16 * (i & 1)) & 0xffff, dtype);
-  }
-}
-
-__device__ __forceinline__ void store4(char* row, int64_t col, int64_t d, int dtype,
-                                       const float (&v)[4]) {
+__device__ __forceinline__ void store_cols(void* row, int64_t col, int64_t d, int dtype,
+                                           const float (&v)[4]) {
   if (col + 4 <= d) {
     if (dtype == RP_F32) {
       u32x4_any w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
-      *reinterpret_cast<u32x4_any*>(row + col * 4) = w;
+      *reinterpret_cast<u32x4_any*>(static_cast<char*>(row) + col * 4) = w;
     } else {
       u32x2_any w;
       w[0] = pack16(v[0], v[1], dtype);
       w[1] = pack16(v[2], v[3], dtype);
-      *reinterpret_cast<u32x2_any*>(row + col * 2) = w;
+      *reinterpret_cast<u32x2_any*>(static_cast<char*>(row) + col * 2) = w;
     }
     return;
   }
@@ -199,157 +375,175 @@ __device__ __forceinline__ void store4(char* row, int64_t col, int64_t d, int dt
   for (int i = 0; i < 3; ++i) {
     if (col + i >= d) break;
     if (dtype == RP_F32)
-      reinterpret_cast<float*>(row)[col + i] = v[i];
+      static_cast<float*>(row)[col + i] = v[i];
     else
-      reinterpret_cast<uint16_t*>(row)[col + i] = (uint16_t)pack16(v[i], 0.f, dtype);
+      static_cast<uint16_t*>(row)[col + i] = (uint16_t)pack16(v[i], 0.f, dtype);
   }
 }
 
 }  // namespace
 
-// Workgroups of four waves: blockIdx.x below `chunks` are shares of the sorted
-// places, the ones behind them ids that may be absent, 32 each; blockIdx.y takes four
-// waves' columns.
+// Workgroups of four waves: blockIdx.x below `shares` are shares of the sorted places,
+// the ones behind them ids that may be absent; blockIdx.y takes four waves' columns.
 template <int EO>
-__global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, EmbedGrad g,
-                                                             int64_t chunks) {
+__global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, EmbedGrad g) {
+  constexpr int C = Row16<EO>::kCols;
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t col = ((int64_t)blockIdx.y * kWaves + wave) * kCols + 4 * lane;
+  const int64_t col = (((int64_t)blockIdx.y * kWaves + wave) * kWave + lane) * C;
   const bool mine = col < p.d;
-  float acc[4] = {};
-  if ((int64_t)blockIdx.x >= chunks) {
-    const int64_t v0 = ((int64_t)blockIdx.x - chunks) * kChunk;
-    const int64_t v = v0 + lane;
-    const bool none = lane < kChunk && v < p.V && g.start[v] == g.start[v + 1];
+  float acc[C] = {};
+  if ((int64_t)blockIdx.x >= g.plan.shares) {
+    const int64_t v0 = ((int64_t)blockIdx.x - g.plan.shares) * kZeroRows;
+    const int64_t v = v0 + lane, slot = slot_of(g.plan, (int32_t)v);
+    const bool none = lane < kZeroRows && v < p.V && g.start[slot] == g.start[slot + 1];
     for (uint64_t m = __ballot(none); m != 0; m &= m - 1) {
       const int64_t row = v0 + __builtin_ctzll(m);
-      if (mine) store4(static_cast<char*>(g.dw) + row * p.d * p.es_w, col, p.d, p.dt_w, acc);
+      if (mine) store_cols(static_cast<char*>(g.dw) + row * p.d * p.es_w, col, p.d, p.dt_w, acc);
     }
     return;
   }
-  const int32_t total = g.start[p.V];
-  const int64_t pos0 = (int64_t)blockIdx.x * kChunk;
+  const int32_t total = g.start[g.plan.slots];
+  const int64_t pos0 = (int64_t)blockIdx.x * g.plan.share;
   if (pos0 >= total) return;
-  const int n = (int)(total - pos0 < kChunk ? total - pos0 : kChunk);
-  int32_t place = 0, id = -1;
-  if (lane < n) {
-    place = g.place[pos0 + lane];
-    id = g.sorted[pos0 + lane];
-  }
-  // the ids next to the share: whether its first and last id go on there
-  int32_t cur = __builtin_amdgcn_readlane(id, 0);
+  const int64_t pos1 = pos0 + g.plan.share < total ? pos0 + g.plan.share : total;
+  // whether the share's first and last id go on outside of it
+  int32_t cur = g.sorted[pos0];
   bool head = pos0 > 0 && g.sorted[pos0 - 1] == cur;
-  const bool tail = pos0 + n < total && g.sorted[pos0 + n] == __builtin_amdgcn_readlane(id, n - 1);
+  const bool tail = pos1 < total && g.sorted[pos1] == g.sorted[pos1 - 1];
   float* part = g.part + (int64_t)blockIdx.x * 2 * p.d;
   const char* rows = static_cast<const char*>(g.dout);
   auto flush = [&](bool last) {
     if (mine) {
       if (head || (last && tail)) {
         // unscaled, in fp32
-        store4(reinterpret_cast<char*>(part + (head ? 0 : p.d)), col, p.d, RP_F32, acc);
+        store_cols(part + (head ? 0 : p.d), col, p.d, RP_F32, acc);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= p.scale;
-        store4(static_cast<char*>(g.dw) + (int64_t)cur * p.d * p.es_w, col, p.d, p.dt_w, acc);
+        for (int i = 0; i < C; ++i) acc[i] *= p.scale;
+        store_cols(static_cast<char*>(g.dw) + (int64_t)cur * p.d * p.es_w, col, p.d, p.dt_w, acc);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = 0.f;
+    for (int i = 0; i < C; ++i) acc[i] = 0.f;
     head = false;
   };
   constexpr int kAhead = 8;
-  for (int j0 = 0; j0 < n; j0 += kAhead) {
-    Raw4<EO> r[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      // (a share's end reads its last row again)
-      const int64_t row = __builtin_amdgcn_readlane(place, j0 + j < n ? j0 + j : n - 1);
-      if (mine) r[j] = load4<EO>(rows + row * g.dosr * EO, col, p.d);
+  for (int64_t pos = pos0; pos < pos1; pos += kWave) {
+    const int n = (int)(pos1 - pos < kWave ? pos1 - pos : kWave);
+    int32_t place = 0, id = 0;
+    if (lane < n) {
+      place = g.place[pos + lane];
+      id = g.sorted[pos + lane];
     }
+    for (int j0 = 0; j0 < n; j0 += kAhead) {
+      Row16<EO> r[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (j0 + j >= n) break;
-      const int32_t next = __builtin_amdgcn_readlane(id, j0 + j);
-      if (next != cur) {
-        flush(false);
-        cur = next;
+      for (int j = 0; j < kAhead; ++j) {
+        // (a share's end reads its last row again)
+        const int64_t row = __builtin_amdgcn_readlane(place, j0 + j < n ? j0 + j : n - 1);
+        if (mine) r[j].load(rows + row * g.dosr * EO, col, p.d);
       }
-      if (mine) add4(r[j], p.dt_out, acc);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (j0 + j >= n) break;
+        const int32_t next = __builtin_amdgcn_readlane(id, j0 + j);
+        if (next != cur) {
+          flush(false);
+          cur = next;
+        }
+        if (mine) r[j].add_to(acc, p.dt_out);
+      }
     }
   }
   flush(true);
 }
 
-// One workgroup for each share: if an id begins in it and goes on behind it, its
-// pieces, which 16 waves add a sixteenth each.
-__global__ __launch_bounds__(kSortWaves* kWave) void embed_join_kernel(EmbedParams p, EmbedGrad g) {
-  __shared__ float buf[kSortWaves][4][kWave];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int32_t total = g.start[p.V];
-  const int64_t c = blockIdx.x, end = (c + 1) * kChunk;
+// One workgroup for each share and 64 columns: if an id begins in the share and goes on
+// behind it, its pieces, which 16 groups of 16 lanes add a sixteenth each.
+constexpr int kJoinGroups = 16;
+__global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedParams p, EmbedGrad g) {
+  __shared__ float buf[kJoinGroups][4][16];
+  const int32_t total = g.start[g.plan.slots];
+  const int64_t c = blockIdx.x, end = (c + 1) * g.plan.share;
   if (end >= total) return;
   const int32_t id = g.sorted[end];
-  const int64_t first = g.start[id];
+  const int64_t slot = slot_of(g.plan, id), first = g.start[slot];
   // (one that ends with the share, or began before it, is another's or none)
-  if (first >= end || first < c * kChunk) return;
-  const int64_t pieces = ((int64_t)g.start[id + 1] - 1) / kChunk - c + 1;
-  const int64_t each = (pieces + kSortWaves - 1) / kSortWaves;
-  const int64_t col = (int64_t)blockIdx.y * kCols + 4 * lane;
-  const int64_t k1 = (wave + 1) * each < pieces ? (wave + 1) * each : pieces;
+  if (first >= end || first < c * g.plan.share) return;
+  const int64_t pieces = ((int64_t)g.start[slot + 1] - 1) / g.plan.share - c + 1;
+  const int64_t each = (pieces + kJoinGroups - 1) / kJoinGroups;
+  const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
+  const int64_t col = (int64_t)blockIdx.y * 64 + 4 * lane;
+  const int64_t k1 = (group + 1) * each < pieces ? (group + 1) * each : pieces;
   float acc[4] = {};
   if (col < p.d) {
 #pragma unroll 8
-    for (int64_t k = wave * each; k < k1; ++k)
-      add4(load4<4>(reinterpret_cast<const char*>(g.part + ((c + k) * 2 + (k == 0)) * p.d), col, p.d),
-           RP_F32, acc);
+    for (int64_t k = group * each; k < k1; ++k) {
+      Row16<4> r;
+      r.load(reinterpret_cast<const char*>(g.part + ((c + k) * 2 + (k == 0)) * p.d), col, p.d);
+      r.add_to(acc, RP_F32);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) buf[wave][i][lane] = acc[i];
+  for (int i = 0; i < 4; ++i) buf[group][i][lane] = acc[i];
   __syncthreads();
-  if (wave > 0 || col >= p.d) return;
+  if (group > 0 || col >= p.d) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    for (int w = 1; w < kSortWaves; ++w) acc[i] += buf[w][i][lane];
+    for (int w = 1; w < kJoinGroups; ++w) acc[i] += buf[w][i][lane];
     acc[i] *= p.scale;
   }
-  store4(static_cast<char*>(g.dw) + (int64_t)id * p.d * p.es_w, col, p.d, p.dt_w, acc);
+  store_cols(static_cast<char*>(g.dw) + (int64_t)id * p.d * p.es_w, col, p.d, p.dt_w, acc);
 }
 
-int64_t embed_chunks(int64_t N) { return (N + kChunk - 1) / kChunk; }
+EmbedPlan embed_plan(int64_t N, int64_t V, int64_t d, int es_out) {
+  EmbedPlan plan;
+  plan.lg = 8;  // a workgroup a CU
+  while (((V + (1ll << plan.lg) - 1) >> plan.lg) > kSortRange) ++plan.lg;
+  plan.range = (int)((V + (1ll << plan.lg) - 1) >> plan.lg);
+  plan.slots = (int64_t)plan.range << plan.lg;
+  // shares as long as leave 4096 waves: each writes up to two rows of `part`
+  const int64_t tiles = (d * es_out + 16 * kWave - 1) / (16 * kWave);
+  plan.share = 32;
+  while (plan.share < 128 && N * tiles >= 4096 * 2 * plan.share) plan.share *= 2;
+  plan.shares = (N + plan.share - 1) / plan.share;
+  // (where every workgroup looks at all ids: 16384 of them 15 us, 131072 88)
+  plan.parts = N > 8192 ? (N + kSplitPart - 1) / kSplitPart : 0;
+  return plan;
+}
 
 hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st) {
-  const int64_t n = p.N * ((p.d + 7) / 8);
+  const int64_t nb = (p.d + 7) / 8, n = p.N * nb;
   if (n == 0) return hipSuccess;
-  const int64_t wg = (n + kThreads - 1) / kThreads;
+  const int64_t wg = (n + 4 * kThreads - 1) / (4 * kThreads);
   const dim3 grid((unsigned)(wg < (1 << 20) ? wg : (1 << 20)));
-  if (p.ids64)
-    hipLaunchKernelGGL(embed_fwd_kernel<int64_t>, grid, dim3(kThreads), 0, st, p);
-  else
-    hipLaunchKernelGGL(embed_fwd_kernel<int32_t>, grid, dim3(kThreads), 0, st, p);
+  const FastDiv blocks((uint32_t)nb);
+  auto* launch = p.ids64 ? (p.es_w == 4 ? embed_fwd_kernel<int64_t, 4> : embed_fwd_kernel<int64_t, 2>)
+                         : (p.es_w == 4 ? embed_fwd_kernel<int32_t, 4> : embed_fwd_kernel<int32_t, 2>);
+  hipLaunchKernelGGL(launch, grid, dim3(kThreads), 0, st, p, blocks);
   return hipGetLastError();
 }
 
 hipError_t launch_embed_bwd(const EmbedParams& p, const EmbedGrad& g, hipStream_t st) {
   if (p.V * p.d == 0) return hipSuccess;
-  // about one workgroup a CU, more where the ids would not fit their counters
-  int64_t range = (p.V + 255) / 256;
-  if (range > kSortRange) range = kSortRange;
-  const dim3 grid((unsigned)((p.V + range - 1) / range));
-  if (p.ids64)
-    hipLaunchKernelGGL(embed_sort_kernel<int64_t>, grid, dim3(kSortWaves * kWave), 0, st, p, g, (int)range);
-  else
-    hipLaunchKernelGGL(embed_sort_kernel<int32_t>, grid, dim3(kSortWaves * kWave), 0, st, p, g, (int)range);
-  const int64_t chunks = embed_chunks(p.N);
-  const dim3 sums((unsigned)(chunks + (p.V + kChunk - 1) / kChunk),
-                  (unsigned)((p.d + kCols * kWaves - 1) / (kCols * kWaves)));
-  if (p.es_out == 4)
-    hipLaunchKernelGGL(embed_sum_kernel<4>, sums, dim3(kThreads), 0, st, p, g, chunks);
-  else
-    hipLaunchKernelGGL(embed_sum_kernel<2>, sums, dim3(kThreads), 0, st, p, g, chunks);
-  if (chunks > 1)
-    hipLaunchKernelGGL(embed_join_kernel, dim3((unsigned)(chunks - 1), (unsigned)((p.d + kCols - 1) / kCols)),
-                       dim3(kSortWaves * kWave), 0, st, p, g);
+  if (g.plan.parts > 0)
+    hipLaunchKernelGGL((p.ids64 ? embed_split_kernel<int64_t> : embed_split_kernel<int32_t>),
+                       dim3((unsigned)g.plan.parts), dim3(kThreads), 0, st, p, g);
+  auto* sort = g.plan.parts > 0 ? embed_sort_kernel<EmbedPair>
+               : p.ids64        ? embed_sort_kernel<int64_t>
+                                : embed_sort_kernel<int32_t>;
+  hipLaunchKernelGGL(sort, dim3(1u << g.plan.lg), dim3(kSortWaves * kWave), 0, st, p, g);
+  const int es = p.es_out;
+  const int64_t wide = 16 * kWave * kWaves;  // bytes of four waves' columns
+  const dim3 sums((unsigned)(g.plan.shares + (p.V + kZeroRows - 1) / kZeroRows),
+                  (unsigned)((p.d * es + wide - 1) / wide));
+  hipLaunchKernelGGL((es == 4 ? embed_sum_kernel<4> : embed_sum_kernel<2>), sums, dim3(kThreads), 0, st,
+                     p, g);
+  if (g.plan.shares > 1)
+    hipLaunchKernelGGL(embed_join_kernel,
+                       dim3((unsigned)(g.plan.shares - 1), (unsigned)((p.d + 63) / 64)),
+                       dim3(kThreads), 0, st, p, g);
   return hipGetLastError();
 }
 

@@ -7,6 +7,21 @@
 
 namespace rp {
 
+// e / n for 0 <= e < 2^31 by one product: m = ceil(2^(31 + s) / n) with 2^s >= n
+// fits 32 bits and is off by less than n <= 2^s, which e < 2^31 does not let reach the
+// quotient.
+struct FastDiv {
+  uint32_t m, s, n;
+  FastDiv() : m(0), s(0), n(1) {}
+  explicit FastDiv(uint32_t d) : s(0), n(d) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t e) const {
+    return (uint32_t)(((uint64_t)e * m) >> (31 + s));
+  }
+};
+
 // Embedding (embedding.hip).
 struct EmbedParams {
   int64_t N, V, d;
@@ -20,17 +35,36 @@ struct EmbedParams {
   void* out;        // (N, d) contiguous
 };
 
+// How a backward is laid out.
+struct EmbedPlan {
+  int lg;         // ids are sorted in 2^lg buckets by their low bits
+  int range;      // ids of a bucket
+  int share;      // sorted places of a wave of the sums
+  int64_t slots;  // 2^lg range
+  int64_t shares;
+  int64_t parts;  // of the split before the sort, or 0
+};
+constexpr int64_t kSplitPart = 2048;  // places of a part
+EmbedPlan embed_plan(int64_t N, int64_t V, int64_t d, int es_out);
+
+// A place and its id, as the split leaves them.
+struct EmbedPair {
+  int32_t id, at;
+};
+
 struct EmbedGrad {
   const void* dout;  // (N, d) in dt_out, row stride dosr
   int64_t dosr;
   void* dw;          // (V, d) contiguous in dt_w
-  int32_t* start;    // (V + 1,) workspace: where each id's places begin in `place`
-  int32_t* place;    // (N,) workspace: the places 0 .. N - 1 in order of their ids
-  int32_t* sorted;   // (N,) workspace: the ids in order
-  float* part;       // (chunks, 2, d) workspace
+  int32_t* start;    // (slots + 1,) workspace: where each id's places begin in `place`
+  int32_t* place;    // (N,) workspace: the places 0 .. N - 1 with equal ids together
+  int32_t* sorted;   // (N,) workspace: their ids
+  float* part;       // (shares, 2, d) workspace
+  EmbedPair* pairs;  // (parts, 2048) workspace
+  int32_t* segs;     // (parts, 17) workspace: where the sixteen low bits begin in a part
+  EmbedPlan plan;
 };
 
-int64_t embed_chunks(int64_t N);
 hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st);
 hipError_t launch_embed_bwd(const EmbedParams& p, const EmbedGrad& g, hipStream_t st);
 
@@ -62,9 +96,8 @@ struct AddNormGrad {
   float* part;       // addnorm_work_floats of workspace
 };
 
-// Floats of workspace that a backward needs (es_s: bytes of an
-// element of the rows it reads, 1 for those in 8 bits).
-int64_t addnorm_work_floats(int64_t rows, int64_t d, int es_s, int es_out);
+// Floats of workspace that a backward needs.
+int64_t addnorm_work_floats(int64_t rows, int64_t d);
 hipError_t launch_addnorm_fwd(const AddNormParams& p, hipStream_t st);
 // The backward's rows are p.x (row stride p.xsr, in dt_sum), or p.q8 and p.e8.
 hipError_t launch_addnorm_bwd(const AddNormParams& p, const AddNormGrad& g, hipStream_t st);

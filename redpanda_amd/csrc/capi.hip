@@ -1502,7 +1502,7 @@ rp::EmbedParams embed_params(const rp_embedding_args* a) {
 }
 
 struct EmbedWork {
-  int64_t start, place, sorted, part, pairs, segs, bytes;
+  int64_t start, place, sorted, part, divided, pairs, segs, bytes;
 };
 
 EmbedWork embed_work(const rp_embedding_args* a, const rp::EmbedPlan& plan) {
@@ -1511,7 +1511,8 @@ EmbedWork embed_work(const rp_embedding_args* a, const rp::EmbedPlan& plan) {
   w.place = round_up((plan.slots + 1) * 4, 256);
   w.sorted = w.place + round_up(a->N * 4, 256);
   w.part = w.sorted + round_up(a->N * 4, 256);
-  w.pairs = w.part + round_up(plan.shares * 2 * a->d * 4, 256);
+  w.divided = w.part + round_up(plan.shares * 2 * a->d * 4, 256);
+  w.pairs = w.divided + round_up(plan.shares * (int64_t)sizeof(rp::EmbedPair), 256);
   w.segs = w.pairs + round_up(plan.parts * rp::kSplitPart * (int64_t)sizeof(rp::EmbedPair), 256);
   w.bytes = w.segs + round_up(plan.parts * 17 * 4, 256);
   return w;
@@ -1574,6 +1575,7 @@ int rp_embedding_bwd(const rp_embedding_args* a, const rp_embedding_grad* g, voi
   eg.place = reinterpret_cast<int32_t*>(work + at.place);
   eg.sorted = reinterpret_cast<int32_t*>(work + at.sorted);
   eg.part = reinterpret_cast<float*>(work + at.part);
+  eg.divided = reinterpret_cast<rp::EmbedPair*>(work + at.divided);
   eg.pairs = reinterpret_cast<rp::EmbedPair*>(work + at.pairs);
   eg.segs = reinterpret_cast<int32_t*>(work + at.segs);
   hipError_t e = rp::launch_embed_bwd(embed_params(a), eg, (hipStream_t)stream);

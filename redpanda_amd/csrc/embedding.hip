@@ -8,7 +8,7 @@
 // them), so the places are sorted by id first and the sums run over equal shares of
 // the sorted places, whatever the ids are; no float is added by an atomic, and the
 // sums' order is fixed:
-//   split  (more than 8192 places) each 2048 places are put in order of their ids' low
+//   split  (more than 32768 places) each 2048 places are put in order of their ids' low
 //          four bits, so that what follows looks at a sixteenth of them.
 //   sort   a workgroup owns a bucket, the ids of the same low bits (so that frequent ids
 //          next to each other fall to different ones), and looks at all ids, or those of
@@ -54,13 +54,13 @@ __device__ __forceinline__ int64_t slot_of(const EmbedPlan& plan, int32_t id) {
 template <typename Id, int ES>
 __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(EmbedParams p, FastDiv blocks) {
   constexpr int kRows = 4;
-  const int64_t n = p.N * (int64_t)blocks.n, step = (int64_t)gridDim.x * kThreads;
-  for (int64_t e0 = (int64_t)blockIdx.x * kThreads + threadIdx.x; e0 < n; e0 += kRows * step) {
+  const int64_t n = p.N * (int64_t)blocks.n, step = (int64_t)gridDim.x * kRows * kThreads;
+  for (int64_t e0 = (int64_t)blockIdx.x * kRows * kThreads + threadIdx.x; e0 < n; e0 += step) {
     int64_t at[kRows], id[kRows];
     uint32_t col[kRows];
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      const int64_t e = e0 + k * step;
+      const int64_t e = e0 + k * kThreads;
       at[k] = -1;
       if (e < n) {
         at[k] = n <= 0x7fffffff ? (int64_t)blocks.div((uint32_t)e) : e / blocks.n;
@@ -164,6 +164,8 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
   const int32_t bucket = (int32_t)blockIdx.x, sixteenth = bucket >> (lg - 4);
   for (int i = lane; i < range; i += kWave) cnt[wave][i] = 0;
   int32_t under = 0, listed = 0;
+  // (the running value of the last id is kept in a register)
+  int last_key = -1, running = 0;
 
   // f(each lane's id or -1, its place) for the places of the wave, 64 at a time, the
   // loads of several groups together
@@ -183,16 +185,22 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
           }
           most = n[k] > most ? n[k] : most;
         }
-        for (int j = 0; j < most; j += kWave) {
-          EmbedPair e[kParts];
+        constexpr int kGroups = 4;
+        for (int j0 = 0; j0 < most; j0 += kGroups * kWave) {
+          EmbedPair e[kGroups][kParts];
 #pragma unroll
-          for (int k = 0; k < kParts; ++k) {
-            e[k] = {-1, 0};
-            if (j + lane < n[k]) e[k] = g.pairs[(q0 + k) * kSplitPart + from[k] + j + lane];
-          }
+          for (int u = 0; u < kGroups; ++u)
 #pragma unroll
-          for (int k = 0; k < kParts; ++k)
-            if (j < n[k]) f(e[k].id, e[k].at);
+            for (int k = 0; k < kParts; ++k) {
+              const int j = j0 + u * kWave + lane;
+              e[u][k] = {-1, 0};
+              if (j < n[k]) e[u][k] = g.pairs[(q0 + k) * kSplitPart + from[k] + j];
+            }
+#pragma unroll
+          for (int u = 0; u < kGroups; ++u)
+#pragma unroll
+            for (int k = 0; k < kParts; ++k)
+              if (j0 + u * kWave < n[k]) f(e[u][k].id, e[u][k].at);
         }
       }
     } else {
@@ -236,10 +244,16 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
       const int lead = __builtin_ctzll(left);
       const int k = __builtin_amdgcn_readlane(key, lead);
       const uint64_t those = __ballot(in && key == k);
-      if (lane == 0) cnt[wave][k] += __popcll(those);
+      if (k != last_key) {
+        if (lane == 0 && last_key >= 0) cnt[wave][last_key] += running;
+        last_key = k;
+        running = 0;
+      }
+      running += __popcll(those);
       left &= ~those;
     }
   });
+  if (lane == 0 && last_key >= 0) cnt[wave][last_key] += running;
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) under += __shfl_xor(under, m);
   if (lane == 0) below[wave] = under;
@@ -274,10 +288,9 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
     }
   }
   __syncthreads();
-  // each wave's places, from its list or, where that was too short, by another look; the
-  // running place of the last id is kept in a register
+  // each wave's places, from its list or, where that was too short, by another look
   const int32_t low = low_bits(g.plan, bucket);
-  int last_key = -1, next = 0;
+  last_key = -1;
   auto place = [&](int32_t i, int key, bool in) {
     uint64_t left = __ballot(in);
     while (left != 0) {
@@ -285,16 +298,16 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
       const int k = __builtin_amdgcn_readlane(key, lead);
       const uint64_t those = __ballot(in && key == k);
       if (k != last_key) {
-        if (lane == 0 && last_key >= 0) cnt[wave][last_key] = next;
+        if (lane == 0 && last_key >= 0) cnt[wave][last_key] = running;
         last_key = k;
-        next = __builtin_amdgcn_readfirstlane(cnt[wave][k]);
+        running = __builtin_amdgcn_readfirstlane(cnt[wave][k]);
       }
       if (in && key == k) {
-        const int32_t pos = next + __popcll(those & ((1ull << lane) - 1));
+        const int32_t pos = running + __popcll(those & ((1ull << lane) - 1));
         g.place[pos] = i;
         g.sorted[pos] = (k << lg) | low;
       }
-      next += __popcll(those);
+      running += __popcll(those);
       left &= ~those;
     }
   };
@@ -335,7 +348,8 @@ struct Row16 {
       }
     }
   }
-  __device__ __forceinline__ void add_to(float (&v)[kCols], int dtype) const {
+  template <int T>
+  __device__ __forceinline__ void add_to(float (&v)[kCols]) const {
     if constexpr (ES == 4) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(w[i]);
@@ -344,7 +358,7 @@ struct Row16 {
       float f[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) r.w[i] = w[i];
-      to_floats(r, dtype, f);
+      to_floats(r, T, f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += f[i];
     }
@@ -385,9 +399,10 @@ __device__ __forceinline__ void store_cols(void* row, int64_t col, int64_t d, in
 
 // Workgroups of four waves: blockIdx.x below `shares` are shares of the sorted places,
 // the ones behind them ids that may be absent; blockIdx.y takes four waves' columns.
-template <int EO>
+// T: the type of dout.
+template <int T>
 __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, EmbedGrad g) {
-  constexpr int C = Row16<EO>::kCols;
+  constexpr int EO = T == RP_F32 ? 4 : 2, C = Row16<EO>::kCols;
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t col = (((int64_t)blockIdx.y * kWaves + wave) * kWave + lane) * C;
@@ -405,12 +420,23 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, Embe
   }
   const int32_t total = g.start[g.plan.slots];
   const int64_t pos0 = (int64_t)blockIdx.x * g.plan.share;
-  if (pos0 >= total) return;
+  if (pos0 >= total) {
+    if (blockIdx.y == 0 && threadIdx.x == 0) g.divided[blockIdx.x] = {0, 0};
+    return;
+  }
   const int64_t pos1 = pos0 + g.plan.share < total ? pos0 + g.plan.share : total;
   // whether the share's first and last id go on outside of it
   int32_t cur = g.sorted[pos0];
   bool head = pos0 > 0 && g.sorted[pos0 - 1] == cur;
   const bool tail = pos1 < total && g.sorted[pos1] == g.sorted[pos1 - 1];
+  // the pieces of an id that begins here and goes on, for the join
+  if (blockIdx.y == 0 && threadIdx.x == 0) {
+    const int32_t id = g.sorted[pos1 - 1];
+    const int64_t slot = slot_of(g.plan, id);
+    const bool owner = tail && g.start[slot] >= pos0;
+    const int32_t pieces = (g.start[slot + 1] - 1) / g.plan.share - (int32_t)blockIdx.x + 1;
+    g.divided[blockIdx.x] = {id, owner ? pieces : 0};
+  }
   float* part = g.part + (int64_t)blockIdx.x * 2 * p.d;
   const char* rows = static_cast<const char*>(g.dout);
   auto flush = [&](bool last) {
@@ -428,6 +454,7 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, Embe
     for (int i = 0; i < C; ++i) acc[i] = 0.f;
     head = false;
   };
+  // the next eight rows are loaded while the present ones are added
   constexpr int kAhead = 8;
   for (int64_t pos = pos0; pos < pos1; pos += kWave) {
     const int n = (int)(pos1 - pos < kWave ? pos1 - pos : kWave);
@@ -436,14 +463,21 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, Embe
       place = g.place[pos + lane];
       id = g.sorted[pos + lane];
     }
-    for (int j0 = 0; j0 < n; j0 += kAhead) {
-      Row16<EO> r[kAhead];
+    Row16<EO> r[kAhead];
+    auto load = [&](int j0) {
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        // (a share's end reads its last row again)
+        // (past the end the last row again)
         const int64_t row = __builtin_amdgcn_readlane(place, j0 + j < n ? j0 + j : n - 1);
         if (mine) r[j].load(rows + row * g.dosr * EO, col, p.d);
       }
+    };
+    load(0);
+    for (int j0 = 0; j0 < n; j0 += kAhead) {
+      Row16<EO> now[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) now[j] = r[j];
+      if (j0 + kAhead < n) load(j0 + kAhead);
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         if (j0 + j >= n) break;
@@ -452,49 +486,69 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, Embe
           flush(false);
           cur = next;
         }
-        if (mine) r[j].add_to(acc, p.dt_out);
+        if (mine) now[j].template add_to<T>(acc);
       }
     }
   }
   flush(true);
 }
 
-// One workgroup for each share and 64 columns: if an id begins in the share and goes on
-// behind it, its pieces, which 16 groups of 16 lanes add a sixteenth each.
-constexpr int kJoinGroups = 16;
-__global__ __launch_bounds__(kThreads) void embed_join_kernel(EmbedParams p, EmbedGrad g) {
-  __shared__ float buf[kJoinGroups][4][16];
-  const int32_t total = g.start[g.plan.slots];
-  const int64_t c = blockIdx.x, end = (c + 1) * g.plan.share;
-  if (end >= total) return;
-  const int32_t id = g.sorted[end];
-  const int64_t slot = slot_of(g.plan, id), first = g.start[slot];
-  // (one that ends with the share, or began before it, is another's or none)
-  if (first >= end || first < c * g.plan.share) return;
-  const int64_t pieces = ((int64_t)g.start[slot + 1] - 1) / g.plan.share - c + 1;
-  const int64_t each = (pieces + kJoinGroups - 1) / kJoinGroups;
-  const int lane = threadIdx.x % 16, group = threadIdx.x / 16;
-  const int64_t col = (int64_t)blockIdx.y * 64 + 4 * lane;
-  const int64_t k1 = (group + 1) * each < pieces ? (group + 1) * each : pieces;
-  float acc[4] = {};
-  if (col < p.d) {
+// A workgroup takes 16 shares and 256 columns: for each share in which an id begins that
+// goes on behind it, the id's pieces, a wave for those of up to eight, and all waves (a
+// sixteenth each) for those of more, of which there are two at most.
+__global__ __launch_bounds__(kSortWaves* kWave) void embed_join_kernel(EmbedParams p, EmbedGrad g) {
+  constexpr int kFew = 8;
+  __shared__ float buf[kSortWaves][4][kWave];
+  const int64_t c0 = (int64_t)blockIdx.x * kSortWaves;
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t col = ((int64_t)blockIdx.y * kWave + lane) * 4;
+  auto piece = [&](int64_t c, int64_t k) {
+    Row16<4> r;
+    r.load(reinterpret_cast<const char*>(g.part + ((c + k) * 2 + (k == 0)) * p.d), col, p.d);
+    return r;
+  };
+  auto finish = [&](int32_t id, float (&acc)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= p.scale;
+    store_cols(static_cast<char*>(g.dw) + (int64_t)id * p.d * p.es_w, col, p.d, p.dt_w, acc);
+  };
+  // lane l of every wave knows share c0 + l's
+  EmbedPair divided = {0, 0};
+  if (lane < kSortWaves && c0 + lane < g.plan.shares) divided = g.divided[c0 + lane];
+  const int32_t pieces = __builtin_amdgcn_readlane(divided.at, wave);
+  if (pieces > 0 && pieces <= kFew && col < p.d) {
+    Row16<4> r[kFew];
+#pragma unroll
+    for (int k = 0; k < kFew; ++k)
+      if (k < pieces) r[k] = piece(c0 + wave, k);
+    float acc[4] = {};
+#pragma unroll
+    for (int k = 0; k < kFew; ++k)
+      if (k < pieces) r[k].add_to<RP_F32>(acc);
+    finish(__builtin_amdgcn_readlane(divided.id, wave), acc);
+  }
+  for (uint64_t many = __ballot(divided.at > kFew); many != 0; many &= many - 1) {
+    const int s = __builtin_ctzll(many);
+    const int32_t n = __builtin_amdgcn_readlane(divided.at, s);
+    const int32_t each = (n + kSortWaves - 1) / kSortWaves;
+    const int32_t last = (wave + 1) * each < n ? (wave + 1) * each : n;
+    float acc[4] = {};
+    if (col < p.d) {
 #pragma unroll 8
-    for (int64_t k = group * each; k < k1; ++k) {
-      Row16<4> r;
-      r.load(reinterpret_cast<const char*>(g.part + ((c + k) * 2 + (k == 0)) * p.d), col, p.d);
-      r.add_to(acc, RP_F32);
+      for (int64_t k = wave * each; k < last; ++k) piece(c0 + s, k).add_to<RP_F32>(acc);
     }
-  }
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) buf[group][i][lane] = acc[i];
-  __syncthreads();
-  if (group > 0 || col >= p.d) return;
+    for (int i = 0; i < 4; ++i) buf[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave > 0 || col >= p.d) continue;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    for (int w = 1; w < kJoinGroups; ++w) acc[i] += buf[w][i][lane];
-    acc[i] *= p.scale;
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 1; w < kSortWaves; ++w) acc[i] += buf[w][i][lane];
+    finish(__builtin_amdgcn_readlane(divided.id, s), acc);
   }
-  store_cols(static_cast<char*>(g.dw) + (int64_t)id * p.d * p.es_w, col, p.d, p.dt_w, acc);
 }
 
 EmbedPlan embed_plan(int64_t N, int64_t V, int64_t d, int es_out) {
@@ -508,8 +562,9 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int64_t d, int es_out) {
   plan.share = 32;
   while (plan.share < 128 && N * tiles >= 4096 * 2 * plan.share) plan.share *= 2;
   plan.shares = (N + plan.share - 1) / plan.share;
-  // (where every workgroup looks at all ids: 16384 of them 15 us, 131072 88)
-  plan.parts = N > 8192 ? (N + kSplitPart - 1) / kSplitPart : 0;
+  // (every workgroup looking at all ids takes 15 us for 16384 of them and 88 for 131072;
+  // behind a split of 5 us it takes 14 and 39)
+  plan.parts = N > 32768 ? (N + kSplitPart - 1) / kSplitPart : 0;
   return plan;
 }
 
@@ -538,12 +593,15 @@ hipError_t launch_embed_bwd(const EmbedParams& p, const EmbedGrad& g, hipStream_
   const int64_t wide = 16 * kWave * kWaves;  // bytes of four waves' columns
   const dim3 sums((unsigned)(g.plan.shares + (p.V + kZeroRows - 1) / kZeroRows),
                   (unsigned)((p.d * es + wide - 1) / wide));
-  hipLaunchKernelGGL((es == 4 ? embed_sum_kernel<4> : embed_sum_kernel<2>), sums, dim3(kThreads), 0, st,
-                     p, g);
+  auto* sum = p.dt_out == RP_F32    ? embed_sum_kernel<RP_F32>
+              : p.dt_out == RP_BF16 ? embed_sum_kernel<RP_BF16>
+                                    : embed_sum_kernel<RP_F16>;
+  hipLaunchKernelGGL(sum, sums, dim3(kThreads), 0, st, p, g);
   if (g.plan.shares > 1)
     hipLaunchKernelGGL(embed_join_kernel,
-                       dim3((unsigned)(g.plan.shares - 1), (unsigned)((p.d + 63) / 64)),
-                       dim3(kThreads), 0, st, p, g);
+                       dim3((unsigned)((g.plan.shares + kSortWaves - 1) / kSortWaves),
+                            (unsigned)((p.d + 4 * kWave - 1) / (4 * kWave))),
+                       dim3(kSortWaves * kWave), 0, st, p, g);
   return hipGetLastError();
 }
 

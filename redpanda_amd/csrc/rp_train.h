@@ -60,6 +60,8 @@ struct EmbedGrad {
   int32_t* place;    // (N,) workspace: the places 0 .. N - 1 with equal ids together
   int32_t* sorted;   // (N,) workspace: their ids
   float* part;       // (shares, 2, d) workspace
+  EmbedPair* divided;  // (shares,) workspace: the id that begins in a share and goes on
+                       //   behind it, and the number of its pieces (or 0)
   EmbedPair* pairs;  // (parts, 2048) workspace
   int32_t* segs;     // (parts, 17) workspace: where the sixteen low bits begin in a part
   EmbedPlan plan;

@@ -58,8 +58,8 @@ def make(N, V, d, tw, tout, seed, skew=True):
 
 @pytest.mark.parametrize("tw,tout", PAIRS)
 @pytest.mark.parametrize("N,V,d", [(1, 1, 1), (5, 3, 7), (31, 40, 64), (32, 40, 100), (33, 7, 257),
-                                   (64, 5, 33), (300, 50, 384),(700, 1000, 1001), (65, 4, 1030), (8193, 70, 6),
-                                   (20000, 300, 12)])
+                                   (64, 5, 33), (300, 50, 384), (700, 1000, 1001), (65, 4, 1030), (8193, 70, 6),
+                                   (33000, 300, 12)])
 def test_rows_and_gradient(gpu_lib, N, V, d, tw, tout):
     ids, w, dy = make(N, V, d, tw, tout, N * 100 + d)
     check(ids, w, 1.0, tout, dy)

@@ -234,10 +234,12 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
     uint64_t left = __ballot(in);
     if (left == 0) return;
     const int key = id >> lg;
-    const int to = listed + __popcll(left & ((1ull << lane) - 1));
-    if (in && to < kSortList) {
-      list_at[wave][to] = at;
-      list_key[wave][to] = (uint16_t)key;
+    if (listed < kSortList) {
+      const int to = listed + __popcll(left & ((1ull << lane) - 1));
+      if (in && to < kSortList) {
+        list_at[wave][to] = at;
+        list_key[wave][to] = (uint16_t)key;
+      }
     }
     listed += __popcll(left);
     while (left != 0) {  // one turn for each id of the bucket among the 64
@@ -418,30 +420,28 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, Embe
     }
     return;
   }
+  // the first 64 places, and the ids next to the share, are asked for before it is known
+  // whether there are so many (those behind the last are never used)
+  const int64_t pos0 = (int64_t)blockIdx.x * g.plan.share, back = p.N - 1;
+  const int64_t ahead = pos0 + lane < back ? pos0 + lane : back;
+  const int64_t next0 = pos0 + g.plan.share < back ? pos0 + g.plan.share : back;
+  int32_t place = g.place[ahead], id = g.sorted[ahead];
+  const int32_t before = g.sorted[pos0 > 0 ? pos0 - 1 : 0], behind = g.sorted[next0];
   const int32_t total = g.start[g.plan.slots];
-  const int64_t pos0 = (int64_t)blockIdx.x * g.plan.share;
   if (pos0 >= total) {
     if (blockIdx.y == 0 && threadIdx.x == 0) g.divided[blockIdx.x] = {0, 0};
     return;
   }
   const int64_t pos1 = pos0 + g.plan.share < total ? pos0 + g.plan.share : total;
-  // whether the share's first and last id go on outside of it
-  int32_t cur = g.sorted[pos0];
-  bool head = pos0 > 0 && g.sorted[pos0 - 1] == cur;
-  const bool tail = pos1 < total && g.sorted[pos1] == g.sorted[pos1 - 1];
-  // the pieces of an id that begins here and goes on, for the join
-  if (blockIdx.y == 0 && threadIdx.x == 0) {
-    const int32_t id = g.sorted[pos1 - 1];
-    const int64_t slot = slot_of(g.plan, id);
-    const bool owner = tail && g.start[slot] >= pos0;
-    const int32_t pieces = (g.start[slot + 1] - 1) / g.plan.share - (int32_t)blockIdx.x + 1;
-    g.divided[blockIdx.x] = {id, owner ? pieces : 0};
-  }
+  // whether the share's first id began before it
+  int32_t cur = __builtin_amdgcn_readfirstlane(id);
+  bool head = pos0 > 0 && before == cur;
   float* part = g.part + (int64_t)blockIdx.x * 2 * p.d;
   const char* rows = static_cast<const char*>(g.dout);
   auto flush = [&](bool last) {
     if (mine) {
-      if (head || (last && tail)) {
+      // (at the end: whether the last id goes on behind)
+      if (head || (last && pos1 < total && behind == cur)) {
         // unscaled, in fp32
         store_cols(part + (head ? 0 : p.d), col, p.d, RP_F32, acc);
       } else {
@@ -458,8 +458,7 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, Embe
   constexpr int kAhead = 8;
   for (int64_t pos = pos0; pos < pos1; pos += kWave) {
     const int n = (int)(pos1 - pos < kWave ? pos1 - pos : kWave);
-    int32_t place = 0, id = 0;
-    if (lane < n) {
+    if (pos > pos0 && lane < n) {
       place = g.place[pos + lane];
       id = g.sorted[pos + lane];
     }
@@ -491,6 +490,16 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, Embe
     }
   }
   flush(true);
+  // the pieces of an id that begins here and goes on, for the join
+  if (blockIdx.y == 0 && threadIdx.x == 0) {
+    int32_t pieces = 0;
+    if (pos1 < total && behind == cur) {
+      const int64_t slot = slot_of(g.plan, cur);
+      if (g.start[slot] >= pos0)
+        pieces = (g.start[slot + 1] - 1) / g.plan.share - (int32_t)blockIdx.x + 1;
+    }
+    g.divided[blockIdx.x] = {cur, pieces};
+  }
 }
 
 // A workgroup takes 16 shares and 256 columns: for each share in which an id begins that

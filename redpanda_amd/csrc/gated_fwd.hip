@@ -243,24 +243,35 @@ __global__ __launch_bounds__(kFoldWaves* kWave) void gated_fold_kernel(GatedPara
   const int n = p.nchunk - 1, each = (n + kFoldWaves - 1) / kFoldWaves;
   const int first = wave * each < n ? wave * each : n, last = first + each < n ? first + each : n;
   float prod = 1.f, end = 0.f;
-#pragma unroll 8
-  for (int i = first; i < last; ++i) {
-    const float* s = slot(i);
-    end = gated_join(s[0], s[p.D], end);
-    prod = gated_product(prod, s[0]);
-  }
+  // (16 chunks at a time: all of their loads before the first use, and before the stores)
+  constexpr int kN = 16;
+  auto walk = [&](auto f) {
+    for (int i0 = first; i0 < last; i0 += kN) {
+      float a[kN], e[kN];
+#pragma unroll
+      for (int k = 0; k < kN; ++k) {
+        const float* s = slot(i0 + k < last ? i0 + k : last - 1);
+        a[k] = s[0];
+        e[k] = s[p.D];
+      }
+#pragma unroll
+      for (int k = 0; k < kN; ++k)
+        if (i0 + k < last) f(i0 + k, a[k], e[k]);
+    }
+  };
+  walk([&](int, float a, float e) {
+    end = gated_join(a, e, end);
+    prod = gated_product(prod, a);
+  });
   prods[wave][lane] = prod;
   ends[wave][lane] = end;
   __syncthreads();
   float h = in != nullptr ? in[b * p.D + ch] : 0.f;
   for (int w = 0; w < wave; ++w) h = gated_join(prods[w][lane], ends[w][lane], h);
-#pragma unroll 8
-  for (int i = first; i < last; ++i) {
-    float* s = slot(i);
-    const float a = s[0], e = s[p.D];
-    s[0] = h;
+  walk([&](int i, float a, float e) {
+    *slot(i) = h;
     h = gated_join(a, e, h);
-  }
+  });
   // (the waves behind the last chunk have folded all of it)
   if (wave == kFoldWaves - 1) *slot(n) = h;
 }

@@ -101,7 +101,8 @@ class _HipCheckpoint8(torch.autograd.Function):
             with torch.enable_grad(), torch.autocast("cuda", dtype=dtype, enabled=on,
                                                      cache_enabled=cache):
                 out = ctx.fn(normed)
-            dnorm, *got = torch.autograd.grad(out, (normed, *wanted), dout, allow_unused=True)
+            if out.requires_grad:  # (fn may detach)
+                dnorm, *got = torch.autograd.grad(out, (normed, *wanted), dout, allow_unused=True)
         dx, dadd, dw = norm_backward(None, (q, e), w, ctx.args, ctx.dtypes, dsum, dnorm, need[1:4])
         it = iter(got)
         return (None, dx, dadd, dw, None, None, *(next(it) if n else None for n in need[6:]))

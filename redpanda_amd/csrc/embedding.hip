@@ -1,8 +1,9 @@
 // Embedding: out[i] = scale w[ids[i]], and the table's gradient
 //     dw[v] = scale sum of dout[i] over the places i with ids[i] = v.
 //
-// Forward: eight columns of four places a thread, loads before stores; the places' rows
-// are written once and the table's come from L2 where ids repeat.
+// Forward: a wave takes eight places and 16 bytes a lane of their rows, all loads before
+// the stores (short rows: eight columns of four places a thread); the places' rows are
+// written once and the table's come from L2 where ids repeat.
 //
 // Backward.  Tokens are far from uniform (a board's empty square is a quarter of
 // them), so the places are sorted by id first and the sums run over equal shares of
@@ -85,6 +86,112 @@ __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(EmbedParams p, Fast
       for (int i = 0; i < 8; ++i) v[i] *= p.scale;
       store8(static_cast<char*>(p.out) + at[k] * p.d * p.es_out, col[k], p.d, p.dt_out, v);
     }
+  }
+}
+
+namespace {
+
+// 16 bytes of a row as stored, C columns, from `col` on (zeros at and past d).
+template <int ES>
+struct Row16 {
+  static constexpr int kCols = 16 / ES;
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const char* row, int64_t col, int64_t d) {
+    if (col + kCols <= d) {
+      const u32x4_any v = *reinterpret_cast<const u32x4_any*>(row + col * ES);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = 0;
+#pragma unroll
+      for (int i = 0; i < kCols - 1; ++i) {
+        if (col + i >= d) break;
+        if constexpr (ES == 4)
+          w[i] = reinterpret_cast<const uint32_t*>(row)[col + i];
+        else
+          w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[col + i] << (16 * (i & 1));
+      }
+    }
+  }
+  template <int T>
+  __device__ __forceinline__ void floats(float (&v)[kCols]) const {
+    if constexpr (ES == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+      Raw8<2> r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r.w[i] = w[i];
+      to_floats(r, T, v);
+    }
+  }
+  template <int T>
+  __device__ __forceinline__ void add_to(float (&v)[kCols]) const {
+    float f[kCols];
+    floats<T>(f);
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) v[i] += f[i];
+  }
+};
+
+__device__ __forceinline__ void store_cols(void* row, int64_t col, int64_t d, int dtype,
+                                           const float (&v)[8]) {
+  store8(row, col, d, dtype, v);
+}
+__device__ __forceinline__ void store_cols(void* row, int64_t col, int64_t d, int dtype,
+                                           const float (&v)[4]) {
+  if (col + 4 <= d) {
+    if (dtype == RP_F32) {
+      u32x4_any w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
+      *reinterpret_cast<u32x4_any*>(static_cast<char*>(row) + col * 4) = w;
+    } else {
+      u32x2_any w;
+      w[0] = pack16(v[0], v[1], dtype);
+      w[1] = pack16(v[2], v[3], dtype);
+      *reinterpret_cast<u32x2_any*>(static_cast<char*>(row) + col * 2) = w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    if (col + i >= d) break;
+    if (dtype == RP_F32)
+      static_cast<float*>(row)[col + i] = v[i];
+    else
+      static_cast<uint16_t*>(row)[col + i] = (uint16_t)pack16(v[i], 0.f, dtype);
+  }
+}
+
+}  // namespace
+
+// Rows of half a kilobyte on: their addresses and ids are the wave's.
+template <typename Id, int T>
+__global__ __launch_bounds__(kThreads) void embed_rows_kernel(EmbedParams p) {
+  constexpr int ES = T == RP_F32 ? 4 : 2, C = Row16<ES>::kCols, kRows = 8;
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t col = ((int64_t)blockIdx.y * kWave + lane) * C;
+  const int64_t row0 = ((int64_t)blockIdx.x * kWaves + wave) * kRows;
+  if (col >= p.d) return;
+  Row16<ES> r[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[k].w[i] = 0;
+    const int64_t id = row0 + k < p.N ? id_at<Id>(p.ids, row0 + k) : -1;
+    if (id >= 0 && id < p.V) r[k].load(static_cast<const char*>(p.w) + id * p.wsr * ES, col, p.d);
+  }
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    if (row0 + k >= p.N) break;
+    float v[C];
+    r[k].template floats<T>(v);
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] *= p.scale;
+    store_cols(static_cast<char*>(p.out) + (row0 + k) * p.d * p.es_out, col, p.d, p.dt_out, v);
   }
 }
 
@@ -325,80 +432,6 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
   }
 }
 
-namespace {
-
-// 16 bytes of a row as stored, C columns, from `col` on (zeros at and past d).
-template <int ES>
-struct Row16 {
-  static constexpr int kCols = 16 / ES;
-  uint32_t w[4];
-  __device__ __forceinline__ void load(const char* row, int64_t col, int64_t d) {
-    if (col + kCols <= d) {
-      const u32x4_any v = *reinterpret_cast<const u32x4_any*>(row + col * ES);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = v[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = 0;
-#pragma unroll
-      for (int i = 0; i < kCols - 1; ++i) {
-        if (col + i >= d) break;
-        if constexpr (ES == 4)
-          w[i] = reinterpret_cast<const uint32_t*>(row)[col + i];
-        else
-          w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[col + i] << (16 * (i & 1));
-      }
-    }
-  }
-  template <int T>
-  __device__ __forceinline__ void add_to(float (&v)[kCols]) const {
-    if constexpr (ES == 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += __uint_as_float(w[i]);
-    } else {
-      Raw8<2> r;
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r.w[i] = w[i];
-      to_floats(r, T, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += f[i];
-    }
-  }
-};
-
-__device__ __forceinline__ void store_cols(void* row, int64_t col, int64_t d, int dtype,
-                                           const float (&v)[8]) {
-  store8(row, col, d, dtype, v);
-}
-__device__ __forceinline__ void store_cols(void* row, int64_t col, int64_t d, int dtype,
-                                           const float (&v)[4]) {
-  if (col + 4 <= d) {
-    if (dtype == RP_F32) {
-      u32x4_any w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
-      *reinterpret_cast<u32x4_any*>(static_cast<char*>(row) + col * 4) = w;
-    } else {
-      u32x2_any w;
-      w[0] = pack16(v[0], v[1], dtype);
-      w[1] = pack16(v[2], v[3], dtype);
-      *reinterpret_cast<u32x2_any*>(static_cast<char*>(row) + col * 2) = w;
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    if (col + i >= d) break;
-    if (dtype == RP_F32)
-      static_cast<float*>(row)[col + i] = v[i];
-    else
-      static_cast<uint16_t*>(row)[col + i] = (uint16_t)pack16(v[i], 0.f, dtype);
-  }
-}
-
-}  // namespace
-
 // Workgroups of four waves: blockIdx.x below `shares` are shares of the sorted places,
 // the ones behind them ids that may be absent; blockIdx.y takes four waves' columns.
 // T: the type of dout.
@@ -577,9 +610,30 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int64_t d, int es_out) {
   return plan;
 }
 
+namespace {
+
+template <int T>
+void launch_embed_rows(const EmbedParams& p, hipStream_t st) {
+  const int64_t wide = 16 * kWave;  // bytes of a wave's columns
+  const dim3 grid((unsigned)((p.N + 8 * kWaves - 1) / (8 * kWaves)),
+                  (unsigned)((p.d * p.es_w + wide - 1) / wide));
+  if (p.ids64)
+    hipLaunchKernelGGL((embed_rows_kernel<int64_t, T>), grid, dim3(kThreads), 0, st, p);
+  else
+    hipLaunchKernelGGL((embed_rows_kernel<int32_t, T>), grid, dim3(kThreads), 0, st, p);
+}
+
+}  // namespace
+
 hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st) {
   const int64_t nb = (p.d + 7) / 8, n = p.N * nb;
   if (n == 0) return hipSuccess;
+  if (p.d * p.es_w >= 512) {
+    p.dt_w == RP_F32 ? launch_embed_rows<RP_F32>(p, st)
+    : p.dt_w == RP_BF16 ? launch_embed_rows<RP_BF16>(p, st)
+                        : launch_embed_rows<RP_F16>(p, st);
+    return hipGetLastError();
+  }
   const int64_t wg = (n + 4 * kThreads - 1) / (4 * kThreads);
   const dim3 grid((unsigned)(wg < (1 << 20) ? wg : (1 << 20)));
   const FastDiv blocks((uint32_t)nb);

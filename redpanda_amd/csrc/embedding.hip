@@ -9,13 +9,13 @@
 // them), so the places are sorted by id first and the sums run over equal shares of
 // the sorted places, whatever the ids are; no float is added by an atomic, and the
 // sums' order is fixed:
-//   split  (more than 32768 places) each 2048 places are put in order of their ids' low
-//          four bits, so that what follows looks at a sixteenth of them.
-//   sort   a workgroup owns a bucket, the ids of the same low bits (so that frequent ids
-//          next to each other fall to different ones), and looks at all ids, or those of
-//          its sixteenth: how many belong to buckets below it is where its places begin,
-//          its own are counted and written together, id by id.  No workgroup waits for
-//          another.
+//   sort   ids of the same low bits are a bucket (so that frequent ids next to each other
+//          fall to different ones).  Up to 4096 places: a workgroup a bucket looks at all
+//          ids; how many belong to buckets below is where its places begin, its own are
+//          counted and written together, id by id.  More: each 2048 places are put in
+//          order of their ids' low eight bits (split), several workgroups a bucket count
+//          what that put together for it (count), and write it (place).  No workgroup
+//          waits for another.
 //   sum    a wave takes a share of the sorted places and 16 bytes a lane of their rows,
 //          and adds while the id stays the same.  An id whose places end inside is
 //          written to dw, what may go on in the next share, or began in one before, to
@@ -30,8 +30,7 @@ namespace rp {
 namespace {
 
 constexpr int kSortWaves = 16;
-constexpr int kSortRange = 512;  // most ids of a bucket
-constexpr int kSortList = 256;   // places that a wave remembers from its first look
+constexpr int kSortRange = 256;  // most ids of a bucket
 constexpr int kZeroRows = 32;    // ids that a wave looks at for absent ones
 
 template <typename Id>
@@ -39,12 +38,9 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int64_t i) {
   return static_cast<const Id*>(ids)[i];
 }
 
-// Buckets are the ids' low lg bits, ordered by the lowest four of them first.
+// Buckets are the ids' low lg bits (8 or more), ordered by the lowest eight first.
 __device__ __forceinline__ int32_t bucket_of(const EmbedPlan& plan, int32_t id) {
-  return (id & 15) << (plan.lg - 4) | (id >> 4 & ((1 << (plan.lg - 4)) - 1));
-}
-__device__ __forceinline__ int32_t low_bits(const EmbedPlan& plan, int32_t bucket) {
-  return (bucket & ((1 << (plan.lg - 4)) - 1)) << 4 | bucket >> (plan.lg - 4);
+  return (id & 255) << (plan.lg - 8) | (id >> 8 & ((1 << (plan.lg - 8)) - 1));
 }
 __device__ __forceinline__ int64_t slot_of(const EmbedPlan& plan, int32_t id) {
   return (int64_t)bucket_of(plan, id) * plan.range + (id >> plan.lg);
@@ -195,15 +191,18 @@ __global__ __launch_bounds__(kThreads) void embed_rows_kernel(EmbedParams p) {
   }
 }
 
-// Workgroup: 2048 places to pairs[2048 workgroup ..], ordered by the ids' low four bits;
-// where each of the sixteen begins (and the last ends) to segs[workgroup].
+// Workgroup: 2048 places to pairs[2048 workgroup ..], ordered by the ids' low eight bits;
+// where each of the 256 begins (and the last ends) to segs[workgroup].
 template <typename Id>
 __global__ __launch_bounds__(kThreads) void embed_split_kernel(EmbedParams p, EmbedGrad g) {
+  static_assert(kThreads == 256, "a thread for each value of the low bits");
   constexpr int kGroups = kSplitPart / kThreads;
-  __shared__ int32_t cnt[kWaves][16];
+  __shared__ int32_t cnt[kWaves][256];
+  __shared__ int32_t scan[kWaves];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int64_t part0 = (int64_t)blockIdx.x * kSplitPart, first = part0 + wave * (kSplitPart / kWaves);
-  if (lane < 16) cnt[wave][lane] = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) cnt[w][threadIdx.x] = 0;
   int32_t id[kGroups];
 #pragma unroll
   for (int u = 0; u < kGroups; ++u) {
@@ -211,158 +210,283 @@ __global__ __launch_bounds__(kThreads) void embed_split_kernel(EmbedParams p, Em
     const int64_t v = i < p.N ? id_at<Id>(p.ids, i) : -1;
     id[u] = v >= 0 && v < p.V && v != p.pad ? (int32_t)v : -1;
   }
-  // the lanes of the same low bits; and a lane's place among them
-  auto same = [&](int32_t v, int& rank) {
-    uint64_t m = __ballot(v >= 0);
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const uint64_t set = __ballot(v >> b & 1);
-      m &= v >> b & 1 ? set : ~set;
-    }
-    rank = __popcll(m & ((1ull << lane) - 1));
-    return v >= 0 ? m : 0;
-  };
+  __syncthreads();
+  // the lanes of the same low bits (none for a lane without an id)
+  uint64_t same[kGroups];
 #pragma unroll
   for (int u = 0; u < kGroups; ++u) {
-    int rank;
-    const uint64_t m = same(id[u], rank);
-    if (m != 0 && rank == 0) atomicAdd(&cnt[wave][id[u] & 15], (int32_t)__popcll(m));
+    uint64_t m = __ballot(id[u] >= 0);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const uint64_t set = __ballot(id[u] >> b & 1);
+      m &= id[u] >> b & 1 ? set : ~set;
+    }
+    same[u] = id[u] >= 0 ? m : 0;
+    if (same[u] != 0 && __builtin_ctzll(same[u]) == lane)
+      atomicAdd(&cnt[wave][id[u] & 255], (int32_t)__popcll(same[u]));
   }
   __syncthreads();
-  // wave 0's lanes 0 .. 63 are (low bits, wave) in order
-  if (threadIdx.x < kWave) {
-    const int32_t mine = cnt[lane % kWaves][lane / kWaves];
-    int32_t inc = mine;
+  // a thread each: an inclusive scan over the low bits, then wave by wave
+  int32_t c[kWaves], mine = 0;
 #pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) {
-      const int32_t o = __shfl_up(inc, m);
-      if (lane >= m) inc += o;
-    }
-    cnt[lane % kWaves][lane / kWaves] = inc - mine;
-    int32_t* segs = g.segs + (int64_t)blockIdx.x * 17;
-    if (lane % kWaves == 0) segs[lane / kWaves] = inc - mine;
-    if (lane == kWave - 1) segs[16] = inc;
+  for (int w = 0; w < kWaves; ++w) mine += c[w] = cnt[w][threadIdx.x];
+  int32_t inc = mine;
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) {
+    const int32_t o = __shfl_up(inc, m);
+    if (lane >= m) inc += o;
+  }
+  if (lane == kWave - 1) scan[wave] = inc;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    if (w < wave) inc += scan[w];
+  int32_t* segs = g.segs + (int64_t)blockIdx.x * kSplitSegs;
+  segs[threadIdx.x] = inc - mine;
+  if (threadIdx.x == kThreads - 1) segs[kSplitSegs - 1] = inc;
+  int32_t at = inc - mine;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    cnt[w][threadIdx.x] = at;
+    at += c[w];
   }
   __syncthreads();
   EmbedPair* out = g.pairs + part0;
 #pragma unroll
   for (int u = 0; u < kGroups; ++u) {
-    int rank;
-    const uint64_t m = same(id[u], rank);
-    if (m != 0) out[cnt[wave][id[u] & 15] + rank] = {id[u], (int32_t)(first + u * kWave + lane)};
+    if (same[u] != 0)
+      out[cnt[wave][id[u] & 255] + __popcll(same[u] & ((1ull << lane) - 1))] = {
+          id[u], (int32_t)(first + u * kWave + lane)};
     // (read by all of its lanes before the first of them moves it on)
     __builtin_amdgcn_wave_barrier();
-    if (m != 0 && rank == 0) atomicAdd(&cnt[wave][id[u] & 15], (int32_t)__popcll(m));
+    if (same[u] != 0 && __builtin_ctzll(same[u]) == lane)
+      atomicAdd(&cnt[wave][id[u] & 255], (int32_t)__popcll(same[u]));
     __builtin_amdgcn_wave_barrier();
   }
 }
 
-// Src: the ids' type, or EmbedPair behind the split.
-template <typename Src>
+namespace {
+
+// The lanes of a mask below this one.
+__device__ __forceinline__ int rank_in(uint64_t m) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+
+// The lanes of `left` whose key (of `bits` bits) is the lane's: most often all of them,
+// else by a ballot for each bit.
+__device__ __forceinline__ uint64_t same_key(int key, uint64_t left, int bits) {
+  const int k0 = __builtin_amdgcn_readlane(key, __builtin_ctzll(left));
+  uint64_t m = left;
+  if ((__ballot(key == k0) & left) == left) return m;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = key >> b & 1;
+    const uint64_t set = __ballot(one);
+    m &= one ? set : ~set;
+  }
+  return m;
+}
+
+// 64 lanes' keys (where `in`) counted in cnt.
+__device__ __forceinline__ void count_keys(int32_t* cnt, int key, bool in, int bits) {
+  const uint64_t left = __ballot(in);
+  if (left == 0) return;
+  const uint64_t same = same_key(key, left, bits);
+  if (in && rank_in(same) == 0) atomicAdd(&cnt[key], (int32_t)__popcll(same));
+}
+
+// 64 lanes' places, written where cnt says that their keys' next ones go.
+__device__ __forceinline__ void put_places(const EmbedGrad& g, int32_t* cnt, int32_t at, int32_t id,
+                                           bool in) {
+  const uint64_t left = __ballot(in);
+  if (left == 0) return;
+  const int key = id >> g.plan.lg;
+  const uint64_t same = same_key(key, left, g.plan.bits);
+  const int rank = rank_in(same);
+  if (in) {
+    const int32_t pos = cnt[key] + rank;
+    g.place[pos] = at;
+    g.sorted[pos] = id;
+  }
+  // (read by all of its lanes before the first of them moves it on)
+  __builtin_amdgcn_wave_barrier();
+  if (in && rank == 0) atomicAdd(&cnt[key], (int32_t)__popcll(same));
+  __builtin_amdgcn_wave_barrier();
+}
+
+// f(the lane's id or -1, its place) for the places that the split put together for a
+// bucket, in the parts of a unit, 64 at a time.
+template <typename F>
+__device__ __forceinline__ void look_at_parts(const EmbedGrad& g, int32_t bucket, int64_t unit, F f) {
+  constexpr int kGroups = 4;
+  const int lane = threadIdx.x % kWave;
+  const int32_t low8 = bucket >> (g.plan.lg - 8);
+  const int64_t first = unit * g.plan.unit;
+  const int64_t last = first + g.plan.unit < g.plan.parts ? first + g.plan.unit : g.plan.parts;
+  for (int64_t q = first; q < last; ++q) {
+    const int from = __builtin_amdgcn_readfirstlane(g.segs[q * kSplitSegs + low8]);
+    const int n = __builtin_amdgcn_readfirstlane(g.segs[q * kSplitSegs + low8 + 1]) - from;
+    const EmbedPair* pairs = g.pairs + q * kSplitPart + from;
+    for (int j0 = 0; j0 < n; j0 += kGroups * kWave) {
+      EmbedPair e[kGroups];
+#pragma unroll
+      for (int u = 0; u < kGroups; ++u) {
+        const int j = j0 + u * kWave + lane;
+        e[u] = {-1, 0};
+        if (j < n) e[u] = pairs[j];
+      }
+#pragma unroll
+      for (int u = 0; u < kGroups; ++u) {
+        if (j0 + u * kWave >= n) break;
+        // (a bucket of more than eight bits shares the low eight with others)
+        if (g.plan.lg > 8 && bucket_of(g.plan, e[u].id) != bucket) e[u].id = -1;
+        f(e[u].id, e[u].at);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+// Workgroup (bucket, y): its four waves are units 4 y .. 4 y + 3, whose places they count
+// id by id.
+__global__ __launch_bounds__(kThreads) void embed_count_kernel(EmbedGrad g) {
+  __shared__ int32_t cnt[kWaves][kSortRange];
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t unit = (int64_t)blockIdx.y * kWaves + wave;
+  const int range = g.plan.range;
+  for (int i = lane; i < range; i += kWave) cnt[wave][i] = 0;
+  __syncthreads();
+  look_at_parts(g, (int32_t)blockIdx.x, unit, [&](int32_t id, int32_t) {
+    count_keys(cnt[wave], id >> g.plan.lg, id >= 0, g.plan.bits);
+  });
+  __syncthreads();
+  if (unit >= g.plan.units) return;
+  int32_t* out = g.counts + unit * g.plan.slots + (int64_t)blockIdx.x * range;
+  for (int i = lane; i < range; i += kWave) out[i] = cnt[wave][i];
+}
+
+// The same workgroups write their places: behind those of the buckets below, the bucket's
+// lower ids, and the units below.
+__global__ __launch_bounds__(kThreads) void embed_place_kernel(EmbedGrad g) {
+  __shared__ int32_t cnt[kWaves][kSortRange], alls[kWaves][kSortRange], lowers[kWaves][kSortRange];
+  __shared__ int32_t scan[kWaves];
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int range = g.plan.range, lg = g.plan.lg;
+  const int32_t bucket = (int32_t)blockIdx.x, low8 = bucket >> (lg - 8);
+  const int64_t unit0 = (int64_t)blockIdx.y * kWaves;
+  // the places of lower low bits, and of the buckets below that share the low eight
+  int32_t under = 0;
+  for (int64_t q = threadIdx.x; q < g.plan.parts; q += kThreads) under += g.segs[q * kSplitSegs + low8];
+  const int64_t slot0 = (int64_t)bucket * range, class0 = (int64_t)(low8 << (lg - 8)) * range;
+  for (int64_t u = 0; u < g.plan.units; ++u)
+    for (int64_t i = class0 + threadIdx.x; i < slot0; i += kThreads) under += g.counts[u * g.plan.slots + i];
+  auto sum_before = [&](int32_t v, int32_t& total) {
+    // exclusive over the workgroup's threads
+    int32_t inc = v;
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) {
+      const int32_t o = __shfl_up(inc, m);
+      if (lane >= m) inc += o;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) scan[wave] = inc;
+    __syncthreads();
+    int32_t before = inc - v;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) before += scan[w];
+      total += scan[w];
+    }
+    return before;
+  };
+  // each wave adds a quarter of the units' counts, all of them and those below unit0, and
+  // looks up its own
+  const int64_t quarter = (g.plan.units + kWaves - 1) / kWaves, u0 = wave * quarter;
+  const int64_t u1 = u0 + quarter < g.plan.units ? u0 + quarter : g.plan.units;
+  const int32_t* counts = g.counts + slot0;
+  for (int i = lane; i < range; i += kWave) {
+    int32_t all = 0, lower = 0;
+#pragma unroll 8
+    for (int64_t u = u0; u < u1; ++u) {
+      const int32_t c = counts[u * g.plan.slots + i];
+      all += c;
+      lower += u < unit0 ? c : 0;
+    }
+    alls[wave][i] = all;
+    lowers[wave][i] = lower;
+    cnt[wave][i] = unit0 + wave < g.plan.units ? counts[(unit0 + wave) * g.plan.slots + i] : 0;
+  }
+  int32_t base;
+  sum_before(under, base);  // (and a barrier)
+  for (int i0 = 0; i0 < range; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    int32_t all = 0, lower = 0;
+    if (i < range) {
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        all += alls[w][i];
+        lower += lowers[w][i];
+      }
+    }
+    int32_t total;
+    const int32_t at = base + sum_before(all, total);
+    if (i < range) {
+      if (blockIdx.y == 0) {
+        g.start[slot0 + i] = at;
+        if (slot0 + i == g.plan.slots - 1) g.start[slot0 + i + 1] = at + all;
+      }
+      int32_t next = at + lower;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const int32_t c = cnt[w][i];
+        cnt[w][i] = next;
+        next += c;
+      }
+    }
+    base += total;
+  }
+  __syncthreads();
+  look_at_parts(g, bucket, unit0 + wave,
+                [&](int32_t id, int32_t at) { put_places(g, cnt[wave], at, id, id >= 0); });
+}
+
+// Few places: one launch, whose workgroups each look at all of them, for one bucket.
+template <typename Id>
 __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedParams p, EmbedGrad g) {
-  constexpr bool kSplit = std::is_same<Src, EmbedPair>::value;
   __shared__ int32_t cnt[kSortWaves][kSortRange];
-  __shared__ int32_t list_at[kSortWaves][kSortList];
-  __shared__ uint16_t list_key[kSortWaves][kSortList];
   __shared__ int32_t below[kSortWaves], scan[kSortWaves];
   const int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int range = g.plan.range, lg = g.plan.lg;
-  const int32_t bucket = (int32_t)blockIdx.x, sixteenth = bucket >> (lg - 4);
+  const int32_t bucket = (int32_t)blockIdx.x;
   for (int i = lane; i < range; i += kWave) cnt[wave][i] = 0;
-  int32_t under = 0, listed = 0;
-  // (the running value of the last id is kept in a register)
-  int last_key = -1, running = 0;
-
-  // f(each lane's id or -1, its place) for the places of the wave, 64 at a time, the
-  // loads of several groups together
+  // f(each lane's id or -1, its place) for the wave's stretch of the places, 64 at a time
   auto look = [&](auto f) {
-    if constexpr (kSplit) {
-      constexpr int kParts = 4;
-      const int64_t each = (g.plan.parts + kSortWaves - 1) / kSortWaves;
-      const int64_t last = (wave + 1) * each < g.plan.parts ? (wave + 1) * each : g.plan.parts;
-      for (int64_t q0 = wave * each; q0 < last; q0 += kParts) {
-        int from[kParts], n[kParts], most = 0;
+    constexpr int kGroups = 4;
+    const int64_t stretch = ((p.N + kSortWaves * kWave - 1) / (kSortWaves * kWave)) * kWave;
+    const int64_t first = wave * stretch;
+    const int64_t last = first + stretch < p.N ? first + stretch : p.N;
+    for (int64_t i0 = first; i0 < last; i0 += kGroups * kWave) {
+      int32_t id[kGroups];
 #pragma unroll
-        for (int k = 0; k < kParts; ++k) {
-          from[k] = n[k] = 0;
-          if (q0 + k < last) {
-            from[k] = g.segs[(q0 + k) * 17 + sixteenth];
-            n[k] = g.segs[(q0 + k) * 17 + sixteenth + 1] - from[k];
-          }
-          most = n[k] > most ? n[k] : most;
-        }
-        constexpr int kGroups = 4;
-        for (int j0 = 0; j0 < most; j0 += kGroups * kWave) {
-          EmbedPair e[kGroups][kParts];
-#pragma unroll
-          for (int u = 0; u < kGroups; ++u)
-#pragma unroll
-            for (int k = 0; k < kParts; ++k) {
-              const int j = j0 + u * kWave + lane;
-              e[u][k] = {-1, 0};
-              if (j < n[k]) e[u][k] = g.pairs[(q0 + k) * kSplitPart + from[k] + j];
-            }
-#pragma unroll
-          for (int u = 0; u < kGroups; ++u)
-#pragma unroll
-            for (int k = 0; k < kParts; ++k)
-              if (j0 + u * kWave < n[k]) f(e[u][k].id, e[u][k].at);
-        }
+      for (int u = 0; u < kGroups; ++u) {
+        const int64_t i = i0 + u * kWave + lane;
+        const int64_t v = i < last ? id_at<Id>(p.ids, i) : -1;
+        id[u] = v >= 0 && v < p.V && v != p.pad ? (int32_t)v : -1;
       }
-    } else {
-      constexpr int kGroups = 8;
-      const int64_t stretch = ((p.N + kSortWaves * kWave - 1) / (kSortWaves * kWave)) * kWave;
-      const int64_t first = wave * stretch;
-      const int64_t last = first + stretch < p.N ? first + stretch : p.N;
-      for (int64_t i0 = first; i0 < last; i0 += kGroups * kWave) {
-        int32_t id[kGroups];
 #pragma unroll
-        for (int u = 0; u < kGroups; ++u) {
-          const int64_t i = i0 + u * kWave + lane;
-          const int64_t v = i < last ? id_at<Src>(p.ids, i) : -1;
-          id[u] = v >= 0 && v < p.V && v != p.pad ? (int32_t)v : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < kGroups; ++u) f(id[u], (int32_t)(i0 + u * kWave) + lane);
-      }
+      for (int u = 0; u < kGroups; ++u) f(id[u], (int32_t)(i0 + u * kWave) + lane);
     }
   };
-
-  if constexpr (kSplit) {
-    // the sixteenths below come first
-    for (int64_t q = threadIdx.x; q < g.plan.parts; q += kSortWaves * kWave)
-      under += g.segs[q * 17 + sixteenth];
-  }
-  look([&](int32_t id, int32_t at) {
+  int32_t under = 0;
+  look([&](int32_t id, int32_t) {
     const int32_t b = bucket_of(g.plan, id);
     under += id >= 0 && b < bucket;
-    const bool in = id >= 0 && b == bucket;
-    uint64_t left = __ballot(in);
-    if (left == 0) return;
-    const int key = id >> lg;
-    if (listed < kSortList) {
-      const int to = listed + __popcll(left & ((1ull << lane) - 1));
-      if (in && to < kSortList) {
-        list_at[wave][to] = at;
-        list_key[wave][to] = (uint16_t)key;
-      }
-    }
-    listed += __popcll(left);
-    while (left != 0) {  // one turn for each id of the bucket among the 64
-      const int lead = __builtin_ctzll(left);
-      const int k = __builtin_amdgcn_readlane(key, lead);
-      const uint64_t those = __ballot(in && key == k);
-      if (k != last_key) {
-        if (lane == 0 && last_key >= 0) cnt[wave][last_key] += running;
-        last_key = k;
-        running = 0;
-      }
-      running += __popcll(those);
-      left &= ~those;
-    }
+    count_keys(cnt[wave], id >> lg, id >= 0 && b == bucket, g.plan.bits);
   });
-  if (lane == 0 && last_key >= 0) cnt[wave][last_key] += running;
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) under += __shfl_xor(under, m);
   if (lane == 0) below[wave] = under;
@@ -397,50 +521,19 @@ __global__ __launch_bounds__(kSortWaves* kWave) void embed_sort_kernel(EmbedPara
     }
   }
   __syncthreads();
-  // each wave's places, from its list or, where that was too short, by another look
-  const int32_t low = low_bits(g.plan, bucket);
-  last_key = -1;
-  auto place = [&](int32_t i, int key, bool in) {
-    uint64_t left = __ballot(in);
-    while (left != 0) {
-      const int lead = __builtin_ctzll(left);
-      const int k = __builtin_amdgcn_readlane(key, lead);
-      const uint64_t those = __ballot(in && key == k);
-      if (k != last_key) {
-        if (lane == 0 && last_key >= 0) cnt[wave][last_key] = running;
-        last_key = k;
-        running = __builtin_amdgcn_readfirstlane(cnt[wave][k]);
-      }
-      if (in && key == k) {
-        const int32_t pos = running + __popcll(those & ((1ull << lane) - 1));
-        g.place[pos] = i;
-        g.sorted[pos] = (k << lg) | low;
-      }
-      running += __popcll(those);
-      left &= ~those;
-    }
-  };
-  if (listed <= kSortList) {
-    for (int j = 0; j < listed; j += kWave) {
-      const bool in = j + lane < listed;
-      place(in ? list_at[wave][j + lane] : 0, in ? list_key[wave][j + lane] : 0, in);
-    }
-  } else {
-    look([&](int32_t id, int32_t at) {
-      place(at, id >> lg, id >= 0 && bucket_of(g.plan, id) == bucket);
-    });
-  }
+  look([&](int32_t id, int32_t at) {
+    put_places(g, cnt[wave], at, id, id >= 0 && bucket_of(g.plan, id) == bucket);
+  });
 }
 
-// Workgroups of four waves: blockIdx.x below `shares` are shares of the sorted places,
-// the ones behind them ids that may be absent; blockIdx.y takes four waves' columns.
+// Workgroups of one wave: blockIdx.x below `shares` are shares of the sorted places, the
+// ones behind them ids that may be absent; blockIdx.y takes a wave's columns.
 // T: the type of dout.
 template <int T>
-__global__ __launch_bounds__(kThreads) void embed_sum_kernel(EmbedParams p, EmbedGrad g) {
+__global__ __launch_bounds__(kWave) void embed_sum_kernel(EmbedParams p, EmbedGrad g) {
   constexpr int EO = T == RP_F32 ? 4 : 2, C = Row16<EO>::kCols;
-  const int lane = threadIdx.x % kWave;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t col = (((int64_t)blockIdx.y * kWaves + wave) * kWave + lane) * C;
+  const int lane = threadIdx.x;
+  const int64_t col = ((int64_t)blockIdx.y * kWave + lane) * C;
   const bool mine = col < p.d;
   float acc[C] = {};
   if ((int64_t)blockIdx.x >= g.plan.shares) {
@@ -599,14 +692,23 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int64_t d, int es_out) {
   while (((V + (1ll << plan.lg) - 1) >> plan.lg) > kSortRange) ++plan.lg;
   plan.range = (int)((V + (1ll << plan.lg) - 1) >> plan.lg);
   plan.slots = (int64_t)plan.range << plan.lg;
+  plan.bits = 0;
+  while ((1 << plan.bits) < plan.range) ++plan.bits;
   // shares as long as leave 4096 waves: each writes up to two rows of `part`
   const int64_t tiles = (d * es_out + 16 * kWave - 1) / (16 * kWave);
   plan.share = 32;
   while (plan.share < 128 && N * tiles >= 4096 * 2 * plan.share) plan.share *= 2;
   plan.shares = (N + plan.share - 1) / plan.share;
-  // (every workgroup looking at all ids takes 15 us for 16384 of them and 88 for 131072;
-  // behind a split of 5 us it takes 14 and 39)
-  plan.parts = N > 32768 ? (N + kSplitPart - 1) / kSplitPart : 0;
+  // (every workgroup looking at all ids takes 5 us for 600 of them, 16 for 16384, 88 for
+  // 131072)
+  plan.parts = N > 4096 ? (N + kSplitPart - 1) / kSplitPart : 0;
+  // units: no more than let all workgroups of 256 buckets be resident, or leave more
+  // counters of a bucket than 2048 (131072 places: 64 units 9 us to count and
+  // 23 to place, 32 units 13 and 17)
+  int64_t units = plan.range < 64 ? 32 : 2048 / plan.range;
+  if (units > plan.parts) units = plan.parts;
+  plan.unit = units > 0 ? (plan.parts + units - 1) / units : 1;
+  plan.units = (plan.parts + plan.unit - 1) / plan.unit;
   return plan;
 }
 
@@ -645,21 +747,25 @@ hipError_t launch_embed_fwd(const EmbedParams& p, hipStream_t st) {
 
 hipError_t launch_embed_bwd(const EmbedParams& p, const EmbedGrad& g, hipStream_t st) {
   if (p.V * p.d == 0) return hipSuccess;
-  if (g.plan.parts > 0)
+  const unsigned buckets = 1u << g.plan.lg;
+  if (g.plan.parts > 0) {
+    const dim3 grid(buckets, (unsigned)((g.plan.units + kWaves - 1) / kWaves));
     hipLaunchKernelGGL((p.ids64 ? embed_split_kernel<int64_t> : embed_split_kernel<int32_t>),
                        dim3((unsigned)g.plan.parts), dim3(kThreads), 0, st, p, g);
-  auto* sort = g.plan.parts > 0 ? embed_sort_kernel<EmbedPair>
-               : p.ids64        ? embed_sort_kernel<int64_t>
-                                : embed_sort_kernel<int32_t>;
-  hipLaunchKernelGGL(sort, dim3(1u << g.plan.lg), dim3(kSortWaves * kWave), 0, st, p, g);
+    hipLaunchKernelGGL(embed_count_kernel, grid, dim3(kThreads), 0, st, g);
+    hipLaunchKernelGGL(embed_place_kernel, grid, dim3(kThreads), 0, st, g);
+  } else {
+    hipLaunchKernelGGL((p.ids64 ? embed_sort_kernel<int64_t> : embed_sort_kernel<int32_t>),
+                       dim3(buckets), dim3(kSortWaves * kWave), 0, st, p, g);
+  }
   const int es = p.es_out;
-  const int64_t wide = 16 * kWave * kWaves;  // bytes of four waves' columns
+  const int64_t wide = 16 * kWave;  // bytes of a wave's columns
   const dim3 sums((unsigned)(g.plan.shares + (p.V + kZeroRows - 1) / kZeroRows),
                   (unsigned)((p.d * es + wide - 1) / wide));
   auto* sum = p.dt_out == RP_F32    ? embed_sum_kernel<RP_F32>
               : p.dt_out == RP_BF16 ? embed_sum_kernel<RP_BF16>
                                     : embed_sum_kernel<RP_F16>;
-  hipLaunchKernelGGL(sum, sums, dim3(kThreads), 0, st, p, g);
+  hipLaunchKernelGGL(sum, sums, dim3(kWave), 0, st, p, g);
   if (g.plan.shares > 1)
     hipLaunchKernelGGL(embed_join_kernel,
                        dim3((unsigned)((g.plan.shares + kSortWaves - 1) / kSortWaves),

@@ -38,13 +38,17 @@ struct EmbedParams {
 // How a backward is laid out.
 struct EmbedPlan {
   int lg;         // ids are sorted in 2^lg buckets by their low bits
-  int range;      // ids of a bucket
+  int range;      // ids of a bucket, and the bits of their numbers in it
+  int bits;
   int share;      // sorted places of a wave of the sums
   int64_t slots;  // 2^lg range
   int64_t shares;
   int64_t parts;  // of the split before the sort, or 0
+  int64_t unit;   // parts of a wave of the count, and the number of such units
+  int64_t units;
 };
 constexpr int64_t kSplitPart = 2048;  // places of a part
+constexpr int kSplitSegs = 257;       // where each value of the low eight bits begins, and the end
 EmbedPlan embed_plan(int64_t N, int64_t V, int64_t d, int es_out);
 
 // A place and its id, as the split leaves them.
@@ -63,7 +67,8 @@ struct EmbedGrad {
   EmbedPair* divided;  // (shares,) workspace: the id that begins in a share and goes on
                        //   behind it, and the number of its pieces (or 0)
   EmbedPair* pairs;  // (parts, 2048) workspace
-  int32_t* segs;     // (parts, 17) workspace: where the sixteen low bits begin in a part
+  int32_t* segs;     // (parts, kSplitSegs) workspace
+  int32_t* counts;   // (units, slots) workspace
   EmbedPlan plan;
 };
 

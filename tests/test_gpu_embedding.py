@@ -58,7 +58,7 @@ def make(N, V, d, tw, tout, seed, skew=True):
 
 @pytest.mark.parametrize("tw,tout", PAIRS)
 @pytest.mark.parametrize("N,V,d", [(1, 1, 1), (5, 3, 7), (31, 40, 64), (32, 40, 100), (33, 7, 257),
-                                   (64, 5, 33), (300, 50, 384), (700, 1000, 1001), (65, 4, 1030), (8193, 70, 6),
+                                   (64, 5, 33), (300, 50, 384), (700, 1000, 1001), (65, 4, 1030), (4097, 70, 6),
                                    (33000, 300, 12)])
 def test_rows_and_gradient(gpu_lib, N, V, d, tw, tout):
     ids, w, dy = make(N, V, d, tw, tout, N * 100 + d)
@@ -84,10 +84,11 @@ def test_borders_of_shares(gpu_lib):
         check(ids, w, 1.0, torch.float32, torch.randn(len(ids), 20, generator=g, device=dev))
 
 
-def test_many_ids(gpu_lib):
-    """More ids than 256 workgroups have counters for, and rows of a wide table."""
+@pytest.mark.parametrize("N", [3000, 50000])
+def test_many_ids(gpu_lib, N):
+    """More ids than 256 buckets have counters for."""
     g = torch.Generator(device=dev).manual_seed(5)
-    V, d, N = 200003, 8, 3000
+    V, d = 200003, 8
     w = torch.randn(V, d, generator=g, device=dev)
     ids = torch.randint(0, V, (N,), generator=g, device=dev)
     ids[::7] = V - 1
@@ -96,7 +97,7 @@ def test_many_ids(gpu_lib):
     (dw,) = torch.autograd.grad(hip_embedding(ids, w), (w,), dy)
     want = torch.zeros(V, d, dtype=torch.float64, device=dev).index_add_(0, ids, dy.double())
     size = torch.zeros(V, d, dtype=torch.float64, device=dev).index_add_(0, ids, dy.double().abs())
-    assert bool(((dw.double() - want).abs() <= 500 * U * size).all())
+    assert bool(((dw.double() - want).abs() <= (N / 7 + 20) * U * size).all())
 
 
 def test_ids_outside_the_table(gpu_lib):

@@ -1828,7 +1828,7 @@ int rp_gated_check(const rp_gated_args* a) {
   if (!known_dtype(a->dtype)) return fail(RP_ERR_INVALID, "gated args: unknown dtype code %d", a->dtype);
   if (a->B == 0 || a->L == 0 || a->D == 0) return RP_OK;
   // (the launches hold a wave for each 64 to 256 channels of a sequence's chunk)
-  if (a->B > ((int64_t)1 << 25) / ((a->D + 63) / 64) || a->L > ((int64_t)1 << 50) / a->D / a->B)
+  if (a->B > ((int64_t)1 << 23) / ((a->D + 63) / 64) || a->L > ((int64_t)1 << 50) / a->D / a->B)
     return fail(RP_ERR_UNSUPPORTED, "gated args: too many channels or elements");
   return RP_OK;
 }

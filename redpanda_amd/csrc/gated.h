@@ -171,8 +171,8 @@ __device__ __forceinline__ void gated_leave(const GatedParams& p, int64_t b, int
 
 hipError_t launch_gated_fold(const GatedParams& p, const float* in, bool backward, hipStream_t st);
 
-// Waves of a workgroup, and where the time axis is split among workgroups.
+// Waves of a workgroup, at most where there are many, and always where the time axis is
+// split among workgroups.
 constexpr int kSplitWaves = 4;
-#define RP_GATED_WAVES(X) X(1) X(2) X(4) X(8)
 
 }  // namespace rp

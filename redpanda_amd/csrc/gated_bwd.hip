@@ -249,10 +249,11 @@ hipError_t run(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
 
 template <int T, int V>
 hipError_t run_waves(const GatedParams& p, const GatedGrad& g, hipStream_t st) {
-#define RP_CASE(NW) \
-  if (p.nw == NW) return run<T, V, NW>(p, g, st);
-  RP_GATED_WAVES(RP_CASE)
-  if constexpr (V == 1) RP_CASE(16)
+#define RP_CASE(NW) if (p.nw == NW) return run<T, V, NW>(p, g, st);
+  RP_CASE(1) RP_CASE(2) RP_CASE(4)
+  if constexpr (V == 1) {
+    RP_CASE(8) RP_CASE(16)
+  }
 #undef RP_CASE
   return hipErrorInvalidValue;
 }

@@ -282,26 +282,30 @@ hipError_t launch_gated_fold(const GatedParams& p, const float* in, bool backwar
   return hipGetLastError();
 }
 
+// Three shapes, by the workgroups that sequences and channels alone give (bf16, both ways,
+// kernels):
+//   256 or more: four waves each, the whole sequence (32 x 2048 x 1024, 256 workgroups: 330
+//     us, split 371; 64 x 2048 x 1024 with eight waves, of which one workgroup is resident a
+//     CU, 519 for 496)
+//   fewer, up to 256 steps: a lane a channel and all steps at once
+//   fewer, more steps: split among about 2048 workgroups (16 x 2048 x 1024, 128 workgroups:
+//     196 us, whole 230; 1 x 131072 x 1024, 8 workgroups: 735)
 int64_t gated_plan(GatedParams* p) {
   const int V = p->v = p->es == 2 && p->D >= 2 ? 2 : 1;
-  int64_t tiles = p->B * ((p->D + kWave * V - 1) / (kWave * V));
-  // waves of a workgroup: until the card is full, or the sequence is
-  int nw = 1;
-  while (nw < 8 && nw * kGatedK < p->L && (tiles * nw < 8192 || nw < 4)) nw *= 2;
+  const int64_t tiles = p->B * ((p->D + kWave * V - 1) / (kWave * V));
   int64_t n = 1;
-  if (tiles * nw < 2048 && p->L <= 16 * kGatedK) {
-    // few channels and few steps: as many waves as there are stretches of 16, and as
-    // many lanes as channels
+  int most = kSplitWaves;
+  if (tiles < 256 && p->L <= 16 * kGatedK) {
     p->v = 1;
-    while (nw < 16 && nw * kGatedK < p->L) nw *= 2;
-  } else if (tiles * nw < 2048) {
-    nw = kSplitWaves;
-    n = (8192 / nw + tiles - 1) / tiles;
-    const int64_t most = (p->L + kGatedK * nw - 1) / (kGatedK * nw);
-    if (n > most) n = most;
+    most = 16;
+  } else if (tiles < 256) {
+    n = (2048 + tiles - 1) / tiles;
+    const int64_t few = (p->L + kGatedK * kSplitWaves - 1) / (kGatedK * kSplitWaves);
+    if (n > few) n = few;
   }
-  const int64_t step = kGatedK * nw, each = (p->L + n - 1) / n;
-  p->nw = nw;
+  p->nw = 1;
+  while (p->nw < most && p->nw * kGatedK < p->L) p->nw *= 2;
+  const int64_t step = kGatedK * p->nw, each = (p->L + n - 1) / n;
   p->chunk = (each + step - 1) / step * step;
   p->nchunk = (int)((p->L + p->chunk - 1) / p->chunk);
   return p->nchunk > 1 ? p->B * p->nchunk * 2 * p->D : 0;
@@ -334,10 +338,11 @@ hipError_t run_few(const GatedParams& p, hipStream_t st) {
 
 template <int T, int V>
 hipError_t run_waves(const GatedParams& p, hipStream_t st) {
-#define RP_CASE(NW) \
-  if (p.nw == NW) return run<T, V, NW>(p, st);
-  RP_GATED_WAVES(RP_CASE)
-  if constexpr (V == 1) RP_CASE(16)
+#define RP_CASE(NW) if (p.nw == NW) return run<T, V, NW>(p, st);
+  RP_CASE(1) RP_CASE(2) RP_CASE(4)
+  if constexpr (V == 1) {
+    RP_CASE(8) RP_CASE(16)
+  }
 #undef RP_CASE
   return hipErrorInvalidValue;
 }

@@ -77,7 +77,13 @@ class _HipCheckpoint8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, fn, x, add, w, eps, out_dtype, *params):
         total, normed, kept, wc, a = norm_forward(x, add, w, eps, out_dtype, True)
-        out = fn(normed)
+        if torch.is_autocast_enabled("cuda"):
+            # (a weight cast here, where nothing is recorded, must not be found in
+            # autocast's cache by a later use that is)
+            with torch.autocast("cuda", dtype=torch.get_autocast_dtype("cuda"), cache_enabled=False):
+                out = fn(normed)
+        else:
+            out = fn(normed)
         ctx.save_for_backward(wc, *kept, *params)
         ctx.fn, ctx.args, ctx.out_dtype = fn, a, out_dtype
         ctx.dtypes = (x.dtype, None if add is None else add.dtype, None if w is None else w.dtype)

@@ -223,3 +223,36 @@ def test_training_step_captured(gpu_lib):
         held = [t.detach().clone() for t in got]
         want = step()
         assert all(rel(a, b) <= 1e-5 for a, b in zip(held, want))
+
+
+def test_weights_used_again_under_autocast(gpu_lib):
+    """A weight that a checkpointed layer has cast for its forward, which records
+    nothing, is cast anew where it is used with a graph, in a second layer or when the
+    backward itself runs under autocast."""
+    d = 64
+    fn = branch(d, 3)
+    g = torch.Generator(device=dev).manual_seed(4)
+    x = torch.randn(70, d, generator=g, device=dev)
+    dy = torch.randn(70, d, generator=g, device=dev).bfloat16()
+    params = list(fn.parameters())
+
+    def own():
+        leaf = x.clone().requires_grad_(True)
+        return hip_checkpoint8(fn, leaf, out_dtype=torch.bfloat16, params=params)
+
+    def cast():
+        return torch.autocast("cuda", dtype=torch.bfloat16)
+
+    with cast():
+        alone = own()
+    want = torch.autograd.grad(alone, params, dy)
+    with cast():
+        plain = fn(x)
+    want_plain = torch.autograd.grad(plain, params, dy)
+    with cast():
+        first, second = own(), fn(x)
+        assert second.requires_grad
+        got = torch.autograd.grad(first, params, dy)
+        got_plain = torch.autograd.grad(second, params, dy)
+    for a, b in zip((*got, *got_plain), (*want, *want_plain)):
+        assert torch.equal(a, b)

@@ -125,7 +125,7 @@ def hip_checkpoint8(fn, x, weight=None, eps=1e-5, add=None, out_dtype=None, para
     parameters().  The results are those of the plain layer; its gradients are the exact
     ones at the kept values.  Differentiable once and in reverse mode."""
     eps, out_dtype, grad = check_norm(x, weight, eps, add, out_dtype, "checkpoint8")
-    params = tuple(params)
+    params = tuple(dict.fromkeys(params))  # (one given twice has its gradient once)
     if recorded(grad or any(p.requires_grad for p in params)):
         return _HipCheckpoint8.apply(fn, x, add, weight, eps, out_dtype, *params)
     total, normed, _, _, _ = norm_forward(x, add, weight, eps, out_dtype, False)

@@ -214,7 +214,7 @@ def test_training_step_captured(gpu_lib):
     torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        got = step()
+        got = [t.detach() for t in step()]
     for k in range(3):
         ids.copy_(torch.randint(0, 200, (4, 24), device=dev))
         dy.copy_(torch.randn(4, 24, 96, device=dev))
@@ -256,3 +256,13 @@ def test_weights_used_again_under_autocast(gpu_lib):
         got_plain = torch.autograd.grad(second, params, dy)
     for a, b in zip((*got, *got_plain), (*want, *want_plain)):
         assert torch.equal(a, b)
+
+
+def test_a_parameter_given_twice(gpu_lib):
+    fn = branch(32, 5)
+    x = torch.randn(9, 32, device=dev, requires_grad=True)
+    params = list(fn.parameters())
+    dy = torch.randn(9, 32, device=dev)
+    want = torch.autograd.grad(hip_checkpoint8(fn, x, params=params), (x, *params), dy)
+    got = torch.autograd.grad(hip_checkpoint8(fn, x, params=params + params[:2]), (x, *params), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

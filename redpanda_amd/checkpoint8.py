@@ -72,6 +72,11 @@ def hip_unpack8(packed, dtype=None):
     return out
 
 
+def _one_tensor(out):
+    if not isinstance(out, torch.Tensor):
+        raise TypeError(f"redpanda_amd checkpoint8: fn must give one tensor, got {type(out).__name__}")
+
+
 class _HipCheckpoint8(torch.autograd.Function):
 
     @staticmethod
@@ -84,6 +89,7 @@ class _HipCheckpoint8(torch.autograd.Function):
                 out = fn(normed)
         else:
             out = fn(normed)
+        _one_tensor(out)
         ctx.save_for_backward(wc, *kept, *params)
         ctx.fn, ctx.args, ctx.out_dtype = fn, a, out_dtype
         ctx.dtypes = (x.dtype, None if add is None else add.dtype, None if w is None else w.dtype)
@@ -129,4 +135,6 @@ def hip_checkpoint8(fn, x, weight=None, eps=1e-5, add=None, out_dtype=None, para
     if recorded(grad or any(p.requires_grad for p in params)):
         return _HipCheckpoint8.apply(fn, x, add, weight, eps, out_dtype, *params)
     total, normed, _, _, _ = norm_forward(x, add, weight, eps, out_dtype, False)
-    return fn(normed) if add is None else (total, fn(normed))
+    out = fn(normed)
+    _one_tensor(out)
+    return out if add is None else (total, out)

@@ -266,3 +266,10 @@ def test_a_parameter_given_twice(gpu_lib):
     want = torch.autograd.grad(hip_checkpoint8(fn, x, params=params), (x, *params), dy)
     got = torch.autograd.grad(hip_checkpoint8(fn, x, params=params + params[:2]), (x, *params), dy)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_function_of_several_results_is_refused(gpu_lib):
+    x = torch.randn(9, 32, device=dev)
+    for leaf in (x, x.clone().requires_grad_(True)):
+        with pytest.raises(TypeError, match="one tensor"):
+            hip_checkpoint8(lambda n: (n, n * 2), leaf)

@@ -392,6 +392,8 @@ class Mamba(nn.Module):
         dtype that in_proj reads it in.  keep8 (fused too): each layer is checkpointed
         with its input in 8 bits (hip_checkpoint8), whatever grad_checkpoint says: the
         output is the same, the gradients are those at the kept values."""
+        if embed_scale != 1.0 and input_embeds is not None:
+            raise ValueError("Mamba.forward: embed_scale scales the embedding of input_ids, not input_embeds")
         if fused or keep8:
             return self._forward_fused(input_ids, input_embeds, dropout, seed, embed_scale, keep8)
         if embed_scale != 1.0:

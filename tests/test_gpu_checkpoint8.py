@@ -273,3 +273,11 @@ def test_a_function_of_several_results_is_refused(gpu_lib):
     for leaf in (x, x.clone().requires_grad_(True)):
         with pytest.raises(TypeError, match="one tensor"):
             hip_checkpoint8(lambda n: (n, n * 2), leaf)
+
+
+def test_embed_scale_of_given_embeddings_is_refused(gpu_lib):
+    m = make_model(6)
+    x = torch.randn(2, 15, 96, device=dev)
+    for kw in ({}, {"fused": True}, {"keep8": True}):
+        with pytest.raises(ValueError, match="embed_scale"):
+            m(None, input_embeds=x, embed_scale=2.0, **kw)

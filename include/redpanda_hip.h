@@ -621,7 +621,8 @@ int rp_addnorm_bwd(const rp_addnorm_args* a, const rp_addnorm_grad* g, void* str
  * Gated linear recurrence along a sequence, each channel by itself:
  *     a_t = 1 / (1 + exp(-gate_t)),   h_t = a_t h_{t-1} + (1 - a_t) x_t,   y_t = h_t
  * from h_{-1} = h0 (NULL: 0).  Where starts is not 0 a sequence begins anew: h_{t-1}
- * counts as 0 (1 - a_t stays).  A gate of +inf keeps the state, -inf takes x_t.
+ * counts as 0 (1 - a_t stays).  A gate of +inf keeps the state (x_t finite), -inf
+ * takes x_t (the state finite).
  * x, gate: (B, L, D) in dtype with strides *_sb and *_sl and unit stride along D;
  * h0: (B, D) fp32; starts: NULL or (B, L) bytes with batch stride starts_sb and unit
  * stride along L; y: (B, L, D) contiguous in dtype; h_last: NULL or (B, D) fp32;

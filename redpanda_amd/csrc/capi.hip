@@ -1502,7 +1502,7 @@ rp::EmbedParams embed_params(const rp_embedding_args* a) {
 }
 
 struct EmbedWork {
-  int64_t start, place, sorted, part, divided, pairs, segs, counts, bytes;
+  int64_t start, place, sorted, part, divided, pairs, segs, counts, totals, bytes;
 };
 
 EmbedWork embed_work(const rp_embedding_args* a, const rp::EmbedPlan& plan) {
@@ -1515,7 +1515,8 @@ EmbedWork embed_work(const rp_embedding_args* a, const rp::EmbedPlan& plan) {
   w.pairs = w.divided + round_up(plan.shares * (int64_t)sizeof(rp::EmbedPair), 256);
   w.segs = w.pairs + round_up(plan.parts * rp::kSplitPart * (int64_t)sizeof(rp::EmbedPair), 256);
   w.counts = w.segs + round_up(plan.parts * rp::kSplitSegs * 4, 256);
-  w.bytes = w.counts + round_up(plan.units * plan.slots * 4, 256);
+  w.totals = w.counts + round_up(plan.units * plan.slots * 4, 256);
+  w.bytes = w.totals + (plan.lg > 8 ? round_up((plan.units << plan.lg) * 4, 256) : 0);
   return w;
 }
 
@@ -1580,6 +1581,7 @@ int rp_embedding_bwd(const rp_embedding_args* a, const rp_embedding_grad* g, voi
   eg.pairs = reinterpret_cast<rp::EmbedPair*>(work + at.pairs);
   eg.segs = reinterpret_cast<int32_t*>(work + at.segs);
   eg.counts = reinterpret_cast<int32_t*>(work + at.counts);
+  eg.totals = reinterpret_cast<int32_t*>(work + at.totals);
   hipError_t e = rp::launch_embed_bwd(embed_params(a), eg, (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "embedding bwd launch");
   return RP_OK;

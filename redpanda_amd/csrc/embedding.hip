@@ -363,7 +363,12 @@ __global__ __launch_bounds__(kThreads) void embed_count_kernel(EmbedGrad g) {
   __syncthreads();
   if (unit >= g.plan.units) return;
   int32_t* out = g.counts + unit * g.plan.slots + (int64_t)blockIdx.x * range;
-  for (int i = lane; i < range; i += kWave) out[i] = cnt[wave][i];
+  int32_t total = 0;
+  for (int i = lane; i < range; i += kWave) total += out[i] = cnt[wave][i];
+  if (g.plan.lg == 8) return;
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m);
+  if (lane == 0) g.totals[(unit << g.plan.lg) + blockIdx.x] = total;
 }
 
 // The same workgroups write their places: behind those of the buckets below, the bucket's
@@ -379,9 +384,11 @@ __global__ __launch_bounds__(kThreads) void embed_place_kernel(EmbedGrad g) {
   // the places of lower low bits, and of the buckets below that share the low eight
   int32_t under = 0;
   for (int64_t q = threadIdx.x; q < g.plan.parts; q += kThreads) under += g.segs[q * kSplitSegs + low8];
-  const int64_t slot0 = (int64_t)bucket * range, class0 = (int64_t)(low8 << (lg - 8)) * range;
-  for (int64_t u = 0; u < g.plan.units; ++u)
-    for (int64_t i = class0 + threadIdx.x; i < slot0; i += kThreads) under += g.counts[u * g.plan.slots + i];
+  const int64_t slot0 = (int64_t)bucket * range;
+  if (lg > 8)
+    for (int64_t u = 0; u < g.plan.units; ++u)
+      for (int32_t b = (low8 << (lg - 8)) + (int32_t)threadIdx.x; b < bucket; b += kThreads)
+        under += g.totals[(u << lg) + b];
   auto sum_before = [&](int32_t v, int32_t& total) {
     // exclusive over the workgroup's threads
     int32_t inc = v;

@@ -69,6 +69,7 @@ struct EmbedGrad {
   EmbedPair* pairs;  // (parts, 2048) workspace
   int32_t* segs;     // (parts, kSplitSegs) workspace
   int32_t* counts;   // (units, slots) workspace
+  int32_t* totals;   // (units, buckets) workspace, where buckets are of more than eight bits
   EmbedPlan plan;
 };
 

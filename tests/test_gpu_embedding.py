@@ -199,3 +199,21 @@ def test_refusals(gpu_lib):
         dual = torch.autograd.forward_ad.make_dual(w, torch.ones_like(w))
         with pytest.raises((RuntimeError, NotImplementedError)):
             hip_embedding(ids, dual)
+
+
+@pytest.mark.parametrize("V", [2 ** 22 + 3, 2 ** 27])
+@pytest.mark.parametrize("N", [3000, 40000])
+def test_tables_of_millions_of_rows(gpu_lib, V, N):
+    """Buckets of up to 19 bits, of which many share the low eight."""
+    g = torch.Generator(device=dev).manual_seed(8)
+    d = 1
+    w = torch.randn(V, d, generator=g, device=dev).bfloat16().requires_grad_(True)
+    ids = torch.randint(0, V, (N,), generator=g, device=dev)
+    ids[::5] = V - 1 - 256 * torch.randint(0, 40, (len(ids[::5]),), generator=g, device=dev)
+    dy = torch.randint(-8, 9, (N, d), generator=g, device=dev).bfloat16()
+    y = hip_embedding(ids, w)
+    assert torch.equal(y, w[ids])
+    (dw,) = torch.autograd.grad(y, (w,), dy)
+    # (sums of small integers: exact in fp32, and rounded to bf16 once)
+    want = torch.zeros(V, d, device=dev).index_add_(0, ids, dy.float()).bfloat16()
+    assert torch.equal(dw, want)

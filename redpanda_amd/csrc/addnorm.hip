@@ -8,6 +8,9 @@
 // (rp_pack8.h), which the forward writes beside the rest and the backward takes in
 // its place: the gradient is then exact for the values that were kept.  All sums in
 // fp32 or wider.
+//
+// Rows of up to 16384 columns are held in registers (addnorm_rows.h); longer ones are
+// read again for each use, here.
 
 #include "addnorm_rows.h"
 

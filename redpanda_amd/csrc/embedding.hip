@@ -21,6 +21,10 @@
 //          written to dw, what may go on in the next share, or began in one before, to
 //          `part`.  Ids that do not occur get zeros.
 //   join   the share in which a divided id begins adds its pieces in order.
+// HBM bounds the rows and the sums, the sums by reads in the order of the ids.  131072
+// places of 8192 x 1024 bf16: rows 57 us, sort 35, sums 87 (at 3.1 TB/s), join 16; adding
+// in the order of the places would read at 4.3, by atomics.  16384 of 8192 x 768 fp32: 15,
+// 17, 15, 5.
 
 #include "rp_rows.h"
 #include "rp_train.h"

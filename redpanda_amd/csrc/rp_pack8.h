@@ -55,7 +55,6 @@ __device__ __forceinline__ void unpack_block(const uint32_t (&q)[2], uint32_t e,
   for (int i = 0; i < 8; ++i) v[i] = (float)(int8_t)(q[i / 4] >> (8 * (i & 3))) * up;
 }
 
-
 // The bytes at `col` .. col + 7 of a row of d (zeros at and past d).
 __device__ __forceinline__ void load_q8(const int8_t* row, int64_t col, int64_t d, uint32_t (&q)[2]) {
   q[0] = q[1] = 0;

@@ -72,6 +72,10 @@ def hip_unpack8(packed, dtype=None):
     return out
 
 
+def _versions(params):
+    return [None if p.is_inference() else p._version for p in params]
+
+
 def _one_tensor(out):
     if not isinstance(out, torch.Tensor):
         raise TypeError(f"redpanda_amd checkpoint8: fn must give one tensor, got {type(out).__name__}")
@@ -90,7 +94,10 @@ class _HipCheckpoint8(torch.autograd.Function):
         else:
             out = fn(normed)
         _one_tensor(out)
-        ctx.save_for_backward(wc, *kept, *params)
+        ctx.save_for_backward(wc, *kept)
+        # (not saved: their gradients are asked for by identity, and hooks on saved tensors,
+        # such as another checkpoint's around this one, give others back)
+        ctx.params, ctx.versions = params, _versions(params)
         ctx.fn, ctx.args, ctx.out_dtype = fn, a, out_dtype
         ctx.dtypes = (x.dtype, None if add is None else add.dtype, None if w is None else w.dtype)
         ctx.autocast = (torch.is_autocast_enabled("cuda"), torch.get_autocast_dtype("cuda"),
@@ -102,9 +109,12 @@ class _HipCheckpoint8(torch.autograd.Function):
     @once
     def backward(ctx, *grads):
         dsum, dout = grads if len(grads) == 2 else (None, grads[0])
-        w, q, e, *params = ctx.saved_tensors
+        w, q, e = ctx.saved_tensors
+        if _versions(ctx.params) != ctx.versions:
+            raise RuntimeError("redpanda_amd checkpoint8: one of the params has been modified by an "
+                               "inplace operation since the forward")
         need = ctx.needs_input_grad
-        wanted = [p for p, n in zip(params, need[6:]) if n]
+        wanted = [p for p, n in zip(ctx.params, need[6:]) if n]
         got = [None] * len(wanted)
         dnorm = None
         if dout is not None:

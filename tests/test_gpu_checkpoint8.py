@@ -6,6 +6,7 @@ other bytes but do the same arithmetic."""
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from redpanda_amd.checkpoint8 import hip_checkpoint8, hip_pack8, hip_unpack8
 from redpanda_amd.mamba import Mamba, MambaConfig
@@ -281,3 +282,24 @@ def test_embed_scale_of_given_embeddings_is_refused(gpu_lib):
     for kw in ({}, {"fused": True}, {"keep8": True}):
         with pytest.raises(ValueError, match="embed_scale"):
             m(None, input_embeds=x, embed_scale=2.0, **kw)
+
+
+def test_hooks_on_saved_tensors(gpu_lib):
+    """Another checkpoint around it, or saved tensors kept on the host: the parameters'
+    gradients are still found."""
+    fn = branch(32, 7)
+    x = torch.randn(9, 32, device=dev, requires_grad=True)
+    params = list(fn.parameters())
+    dy = torch.randn(9, 32, device=dev)
+
+    def own(x):
+        return hip_checkpoint8(fn, x, params=params)
+
+    want = torch.autograd.grad(own(x), (x, *params), dy)
+    y = torch.utils.checkpoint.checkpoint(own, x, use_reentrant=False)
+    got = torch.autograd.grad(y, (x, *params), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.autograd.graph.save_on_cpu():
+        y = own(x)
+    got = torch.autograd.grad(y, (x, *params), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

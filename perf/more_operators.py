@@ -240,7 +240,7 @@ def _plain_gated(s):
     if not case["train"]:
         return [y, last]
     g = s["dy"].float()
-    g = torch.cat((g[:, :-1], g[:, -1:] + s["dh"][:, None]), dim=1)
+    g[:, -1] += s["dh"]
     after = torch.cat((a[:, 1:], torch.zeros_like(a[:, :1])), dim=1)
     adj = _along(after.flip(1), g.flip(1)).flip(1)
     before = torch.cat((h0[:, None], h[:, :-1]), dim=1)

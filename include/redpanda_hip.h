@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define RP_ABI_VERSION 16
+#define RP_ABI_VERSION 17
 
 /* element type codes of the streamed scan inputs (delta, u, Bc, Cc); each
  * tensor carries its own code, as autocast hands over mixed dtypes */
@@ -549,13 +549,15 @@ int rp_embedding_bwd(const rp_embedding_args* a, const rp_embedding_grad* g, voi
  * shares a power of two, the least 2^E >= 2^-126 that takes the block's largest
  * magnitude to an integer of at most 127: q = round(x 2^-E), to nearest even, and
  * e = E + 127.  What is held, q 2^E, is off by half of 2^E at most.  A block with an
- * infinity or a NaN has e = 255 and comes back as NaN.
+ * infinity or a NaN has e = 255 and comes back as NaN.  Finite values of dtype_held
+ * (rp_unpack: the type that was packed) come back finite: q 2^E beyond its largest
+ * value is that value, and then rounded to dtype.
  * x: (rows, d) in dtype with row stride x_sr (contiguous for rp_unpack, which
  * writes it); q: (rows, d) int8 contiguous; e: (rows, ceil(d / 32)) contiguous.
  */
 typedef struct rp_pack_args {
   int64_t rows, d;
-  int32_t dtype, reserved;
+  int32_t dtype, dtype_held;
   void* x;  int64_t x_sr;
   int8_t* q;
   uint8_t* e;
@@ -574,8 +576,8 @@ int rp_unpack(const rp_pack_args* a, void* stream);
  * w: (d,) fp32 or NULL (1); sum: (rows, d) contiguous in dtype_sum (NULL without
  * add); out: (rows, d) contiguous in dtype_out, or NULL; q, e: NULL, or s in 8 bits
  * (as rp_pack writes it) beside the rest.
- * With x NULL the rows are those that q and e hold (dtype_sum names no buffer then,
- * add and sum are NULL): a checkpointed layer's norm, computed again.
+ * With x NULL the rows are those that q and e hold (of values of dtype_sum, which names
+ * no buffer then; add and sum are NULL): a checkpointed layer's norm, computed again.
  * All arithmetic in fp32.
  */
 typedef struct rp_addnorm_args {

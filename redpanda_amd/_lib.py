@@ -13,7 +13,7 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libredpanda_hip.so")
 
-ABI_VERSION = 16
+ABI_VERSION = 17
 RP_F32, RP_BF16, RP_F16 = 0, 1, 2
 DTYPE_CODES = {torch.float32: RP_F32, torch.bfloat16: RP_BF16, torch.float16: RP_F16}
 MAX_STATE = 128
@@ -187,7 +187,7 @@ class EmbeddingGrad(ctypes.Structure):
 
 class PackArgs(ctypes.Structure):
     _fields_ = [
-        ("rows", _i64), ("d", _i64), ("dtype", _i32), ("reserved", _i32),
+        ("rows", _i64), ("d", _i64), ("dtype", _i32), ("dtype_held", _i32),
         ("x", _vp), ("x_sr", _i64), ("q", _vp), ("e", _vp),
     ]
 

@@ -18,8 +18,8 @@ from redpanda_amd.norm import (check_norm, norm_again, norm_backward, norm_forwa
 
 class Packed8:
     """A tensor in 8 bits: q (int8, its shape), e (uint8, an exponent for each 32
-    columns) and the dtype it had.  Its values are q * 2^(e - 127); NaN where e is
-    255."""
+    columns) and the dtype it had.  Its values are q * 2^(e - 127), cut to the dtype's
+    finite range; NaN where e is 255."""
 
     __slots__ = ("q", "e", "dtype")
 
@@ -36,8 +36,9 @@ def hip_pack8(x):
 
     Each 32 columns of a row (the last ones what is left) share the least power of two
     (2^-126 or more) that takes the largest of them to at most 127; values are rounded to
-    nearest, ties to even.  32 columns with an infinity or a NaN come back as NaN.  Not
-    differentiable."""
+    nearest, ties to even.  Finite values come back finite (those nearest to the end of
+    x's type as its largest value); 32 columns with an infinity or a NaN come back as NaN.
+    Not differentiable."""
     if not x.is_cuda:
         raise RuntimeError("redpanda_amd pack8: inputs must be ROCm device tensors")
     if x.dim() == 0:
@@ -47,18 +48,18 @@ def hip_pack8(x):
     q, e = pack_buffers(x)
     if q.numel() > 0:
         xr, rows, sr = rows_of(x, d)
-        a = _lib.PackArgs(rows, d, code, 0, xr.data_ptr(), sr, q.data_ptr(), e.data_ptr())
+        a = _lib.PackArgs(rows, d, code, code, xr.data_ptr(), sr, q.data_ptr(), e.data_ptr())
         _lib.call(_lib.load().rp_pack, x.device, ctypes.byref(a))
     return Packed8(q, e, x.dtype)
 
 
 def hip_unpack8(packed, dtype=None):
-    """The tensor that a Packed8 holds, in its own dtype or another."""
+    """The tensor that a Packed8 holds, in its own dtype or rounded to another."""
     q, e = packed.q, packed.e
     if not q.is_cuda:
         raise RuntimeError("redpanda_amd unpack8: inputs must be ROCm device tensors")
     dtype = packed.dtype if dtype is None else dtype
-    code = dtype_code(dtype, "unpack8")
+    code, held = dtype_code(dtype, "unpack8"), dtype_code(packed.dtype, "unpack8")
     d = q.shape[-1]
     if (q.dtype is not torch.int8 or e.dtype is not torch.uint8 or e.device != q.device or
             e.shape != (*q.shape[:-1], (d + 31) // 32)):
@@ -67,7 +68,7 @@ def hip_unpack8(packed, dtype=None):
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
     if out.numel() > 0:
         q, e = q.contiguous(), e.contiguous()
-        a = _lib.PackArgs(out.numel() // d, d, code, 0, out.data_ptr(), d, q.data_ptr(), e.data_ptr())
+        a = _lib.PackArgs(out.numel() // d, d, code, held, out.data_ptr(), d, q.data_ptr(), e.data_ptr())
         _lib.call(_lib.load().rp_unpack, out.device, ctypes.byref(a))
     return out
 

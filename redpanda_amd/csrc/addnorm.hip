@@ -47,7 +47,7 @@ __device__ __forceinline__ void load_s(const AddNormParams& p, int64_t row, int6
   } else {
     uint32_t q[2];
     load_q8(p.q8 + row * p.d, col, p.d, q);
-    unpack_block(q, p.e8[row * ((p.d + kPackBlock - 1) / kPackBlock) + col / kPackBlock], v);
+    unpack_block(q, p.e8[row * ((p.d + kPackBlock - 1) / kPackBlock) + col / kPackBlock], p.dt_sum, v);
   }
 }
 

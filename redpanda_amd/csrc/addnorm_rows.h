@@ -28,7 +28,9 @@ struct AnyRow {
 template <>
 struct AnyRow<1> {
   uint32_t q[2], e;
-  __device__ __forceinline__ void floats(int, float (&v)[8]) const { unpack_block(q, e, v); }
+  __device__ __forceinline__ void floats(int dtype, float (&v)[8]) const {
+    unpack_block(q, e, dtype, v);
+  }
 };
 
 template <int ES, int G, int NB>
@@ -89,7 +91,7 @@ __global__ __launch_bounds__(norm_threads(G)) void addnorm_fwd_rows_kernel(AddNo
   for (int it = 0; at.row < p.rows; at.row += at.step, it ^= 1) {
     float v[NB][8];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) rx[j].floats(p.dt_x, v[j]);
+    for (int j = 0; j < NB; ++j) rx[j].floats(ES == 1 ? p.dt_sum : p.dt_x, v[j]);
     if constexpr (ES != 1) {
       if (p.add != nullptr) {
 #pragma unroll

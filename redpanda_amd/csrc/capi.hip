@@ -1611,6 +1611,7 @@ rp::Pack8Params pack_params(const rp_pack_args* a) {
   p.d = a->d;
   p.dt = a->dtype;
   p.es = (int)elem_size(a->dtype);
+  p.dt_held = a->dtype_held;
   p.x = a->x;
   p.xsr = a->x_sr;
   p.q8 = a->q;
@@ -1631,6 +1632,8 @@ int rp_unpack(const rp_pack_args* a, void* stream) {
   int st = rp_pack_check(a);
   if (st != RP_OK) return st;
   if (a->x_sr != a->d) return fail(RP_ERR_INVALID, "unpack args: x must be contiguous");
+  if (!known_dtype(a->dtype_held))
+    return fail(RP_ERR_INVALID, "unpack args: unknown dtype code %d of what was packed", a->dtype_held);
   hipError_t e = rp::launch_unpack8(pack_params(a), (hipStream_t)stream);
   if (e != hipSuccess) return fail_hip(e, "unpack launch");
   return RP_OK;

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kThreads) void unpack8_kernel(Pack8Params p) {
     uint32_t q[2];
     float v[8];
     load_q8(p.q8 + row * p.d, col, p.d, q);
-    unpack_block(q, p.e8[(row * lanes + at) / 4], v);
+    unpack_block(q, p.e8[(row * lanes + at) / 4], p.dt_held, v);
     store8(static_cast<char*>(p.x) + row * p.xsr * p.es, col, p.d, p.dt, v);
   }
 }

@@ -6,6 +6,11 @@
 // error, so every part of the library and of a test finds the same bits.  A scale of
 // largest / 127 would leave 0.7 of the error on average, at a division a block and
 // results that turn on its rounding.
+//
+// In a block that reaches to the top of its type's range the largest value is 64 steps,
+// and 64 of them may be the power of two behind the type's largest (fp16: 65280 on, held
+// as 64 * 1024).  What was finite is read back finite: cut to the type's largest value,
+// which is nearer to what was packed than the 64 steps are.
 #pragma once
 
 #include "rp_rows.h"
@@ -48,11 +53,18 @@ __device__ __forceinline__ uint32_t pack_block(const float (&v)[8], uint32_t (&q
   return fine ? (uint32_t)e : 255u;
 }
 
-// What they hold (255: infinity times q = 0, a NaN).
-__device__ __forceinline__ void unpack_block(const uint32_t (&q)[2], uint32_t e, float (&v)[8]) {
+// What they hold of values of a type (255: infinity times q = 0, a NaN).
+__device__ __forceinline__ void unpack_block(const uint32_t (&q)[2], uint32_t e, int dtype,
+                                             float (&v)[8]) {
   const float up = __uint_as_float(e << 23);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = (float)(int8_t)(q[i / 4] >> (8 * (i & 3))) * up;
+  // (the least step of which 127 pass the type's largest value)
+  if (e >= (dtype == RP_F16 ? 137u : 249u)) {
+    const float top = dtype == RP_F16 ? 65504.f : __uint_as_float(dtype == RP_BF16 ? 0x7f7f0000u : 0x7f7fffffu);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = v[i] > top ? top : v[i] < -top ? -top : v[i];  // (a NaN stays)
+  }
 }
 
 // The bytes at `col` .. col + 7 of a row of d (zeros at and past d).

@@ -114,6 +114,7 @@ hipError_t launch_addnorm_bwd(const AddNormParams& p, const AddNormGrad& g, hipS
 struct Pack8Params {
   int64_t rows, d;
   int dt, es;
+  int dt_held;   // (unpack) the type that was packed
   void* x;       // (rows, d), row stride xsr; read by the pack, written by the unpack
   int64_t xsr;
   int8_t* q8;    // (rows, d) contiguous

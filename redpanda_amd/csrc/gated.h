@@ -124,14 +124,33 @@ struct GatedAt {
 
 // The (product of the gates, end from 0) of a stretch, applied to what enters it.  A
 // stretch in which a sequence begins has the product -0 and passes nothing on, not even
-// an infinity.
+// an infinity.  Else the product is 0 where a gate is, and only there: one that underflows
+// is held at kGatedLeast, so that an infinity goes through any number of gates above 0 as
+// it does step by step, where 0 times it would be NaN.  (Of a finite state 2^-149 of it
+// comes through then, 5e-7 at most.)
+constexpr float kGatedLeast = 0x1p-149f;
 __device__ __forceinline__ float gated_join(float prod, float end, float in) {
   return __float_as_uint(prod) == 0x80000000u ? end : ffma(prod, in, end);
 }
 // And of two stretches, one behind the other.
 __device__ __forceinline__ float gated_product(float first, float second) {
-  const float p = first * second;
+  float p = first * second;
+  if (p == 0.f && first != 0.f && second != 0.f) p = kGatedLeast;
   return __float_as_uint(first) == 0x80000000u || __float_as_uint(second) == 0x80000000u ? -0.f : p;
+}
+// The products of n steps' gates (up to K) that have come out as 0: held above it unless
+// one of the gates, gate(step, channel), is 0 itself.
+template <int K, int V, typename F>
+__device__ __forceinline__ void gated_above_0(float (&prod)[V], int n, F gate) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (__float_as_uint(prod[i]) != 0u) continue;
+    float low = 1.f;
+#pragma unroll
+    for (int u = 0; u < K; ++u)
+      if (u < n) low = fminf(low, gate(u, i));
+    prod[i] = low > 0.f ? kGatedLeast : 0.f;
+  }
 }
 
 // What the waves of a workgroup know of their stretches.

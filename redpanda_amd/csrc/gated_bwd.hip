@@ -110,6 +110,7 @@ __attribute__((amdgpu_waves_per_eu(3))) void gated_bwd_kernel(GatedParams p, Gat
     else
       there(std::false_type{});
     if constexpr (NW > 1) {
+      gated_above_0<K>(prod, n, [&](int u, int i) { return a[u][i]; });
       gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.prod[turn][wave]), lane * V * 4, prod);
       gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.end[turn][wave]), lane * V * 4, end);
       __syncthreads();
@@ -209,6 +210,9 @@ __global__ __launch_bounds__(kWave* NW) void gated_bwd_sum_kernel(GatedParams p,
       cd[u] = rd[u];
     }
     if (t - K >= first) load(t - K);
+    float part[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[i] = 1.f;
     auto walk = [&](auto whole) {
 #pragma unroll
       for (int u = K - 1; u >= 0; --u) {
@@ -220,7 +224,7 @@ __global__ __launch_bounds__(kWave* NW) void gated_bwd_sum_kernel(GatedParams p,
             gate_of(gated_value<T>(cg[u], i), a, na);
             const float s = gated_value<T>(cd[u], i) + end[i];
             end[i] = begin ? 0.f : a * s;
-            prod[i] = begin ? -0.f : prod[i] * a;
+            part[i] = begin ? -0.f : part[i] * a;
           }
         }
       }
@@ -229,6 +233,13 @@ __global__ __launch_bounds__(kWave* NW) void gated_bwd_sum_kernel(GatedParams p,
       walk(std::true_type{});
     else
       walk(std::false_type{});
+    gated_above_0<K>(part, m, [&](int u, int i) {
+      float a, na;
+      gate_of(gated_value<T>(cg[u], i), a, na);
+      return a;
+    });
+#pragma unroll
+    for (int i = 0; i < V; ++i) prod[i] = gated_product(prod[i], part[i]);
   }
   gated_leave<V, NW>(p, at.b, at.c, at.ch, lane, wave, true, prod, end, share);
 }

@@ -82,6 +82,7 @@ __global__ __launch_bounds__(kWave* NW) void gated_fwd_kernel(GatedParams p) {
       there(std::false_type{});
     float from[V];
     if constexpr (NW > 1) {
+      gated_above_0<K>(prod, n, [&](int u, int i) { return a[u][i]; });
       gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.prod[turn][wave]), lane * V * 4, prod);
       gated_store<RP_F32, V>(reinterpret_cast<char*>(&share.end[turn][wave]), lane * V * 4, end);
       // (the next turn's stores go to the other half, and the one behind that waits for
@@ -102,10 +103,7 @@ __global__ __launch_bounds__(kWave* NW) void gated_fwd_kernel(GatedParams p) {
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        from[i] = h[i];
-        h[i] = gated_join(prod[i], end[i], h[i]);
-      }
+      for (int i = 0; i < V; ++i) from[i] = h[i];
     }
     if (n > 0 && p.ckpt != nullptr) {
       float* to = p.ckpt + (at.b * ((p.L + K - 1) / K) + t / K) * p.D;
@@ -126,6 +124,10 @@ __global__ __launch_bounds__(kWave* NW) void gated_fwd_kernel(GatedParams p) {
       again(std::true_type{});
     else
       again(std::false_type{});
+    if constexpr (NW == 1) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) h[i] = from[i];
+    }
     // the wave with the last step has the last state, as its own steps give it
     if (p.h_last != nullptr && t < p.L && t + n == p.L)
       gated_store<RP_F32, V>(reinterpret_cast<char*>(p.h_last + at.b * p.D), at.ch * 4, from);
@@ -172,6 +174,9 @@ __global__ __launch_bounds__(kWave* NW) void gated_fwd_sum_kernel(GatedParams p)
       cg[u] = rg[u];
     }
     if (t + K < last) load(t + K);
+    float part[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[i] = 1.f;
     auto walk = [&](auto whole) {
 #pragma unroll
       for (int u = 0; u < K; ++u) {
@@ -180,7 +185,7 @@ __global__ __launch_bounds__(kWave* NW) void gated_fwd_sum_kernel(GatedParams p)
         for (int i = 0; i < V; ++i) {
           float a, na;
           gate_of(gated_value<T>(cg[u], i), a, na);
-          prod[i] = begin ? -0.f : prod[i] * a;
+          part[i] = begin ? -0.f : part[i] * a;
           end[i] = ffma(a, begin ? 0.f : end[i], na * gated_value<T>(cx[u], i));
         }
       }
@@ -189,6 +194,13 @@ __global__ __launch_bounds__(kWave* NW) void gated_fwd_sum_kernel(GatedParams p)
       walk(std::true_type{});
     else
       walk(std::false_type{});
+    gated_above_0<K>(part, K, [&](int u, int i) {
+      float a, na;
+      gate_of(gated_value<T>(cg[u], i), a, na);
+      return a;
+    });
+#pragma unroll
+    for (int i = 0; i < V; ++i) prod[i] = gated_product(prod[i], part[i]);
   }
   gated_leave<V, NW>(p, at.b, at.c, at.ch, lane, wave, false, prod, end, share);
 }

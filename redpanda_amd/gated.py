@@ -113,9 +113,10 @@ def hip_gated_scan(x, gate, h0=None, starts=None):
     halves of one projection are read in place); h0: (B, D) fp32 or None (0).  starts:
     None, or (B, L) bool: where it is True a sequence begins anew, h_{t-1} counting as 0
     (packed sequences).  A gate of +inf keeps the state as it is where x_t is
-    finite (padding behind a sequence's end), of -inf takes x_t where the state is finite:
-    0 times an infinity or a NaN is NaN, as in the formula.  y: (B, L, D) in x's dtype; h_last: (B, D) fp32, the
-    last state (h0 where L is 0).  The state is fp32 throughout.  Differentiable in x,
+    finite (padding behind a sequence's end), of -inf takes x_t where the state is finite
+    (and so beyond about +-87, where fp32's exp is 0): 0 times an infinity or a NaN is NaN,
+    as in the formula; an infinite state stays one through all other gates.  y: (B, L, D)
+    in x's dtype; h_last: (B, D) fp32, the last state (h0 where L is 0).  The state is fp32 throughout.  Differentiable in x,
     gate and h0, once and in reverse mode (a tangent is refused)."""
     if not x.is_cuda:
         raise RuntimeError("redpanda_amd gated_scan: inputs must be ROCm device tensors")

@@ -22,9 +22,11 @@ def _args(ids, V, d, wt, out_dtype, scale, padding):
 def _forward(ids, w, scale, padding, out_dtype):
     lib = _lib.load()
     V, d = w.shape
+    out = torch.empty((*ids.shape, d), dtype=out_dtype, device=w.device)
+    if out.numel() == 0:
+        return out
     ids = ids.contiguous()
     wr, _, wsr = rows_of(w, d)
-    out = torch.empty((*ids.shape, d), dtype=out_dtype, device=w.device)
     a = _args(ids, V, d, w.dtype, out_dtype, scale, padding)
     a.w, a.w_sr, a.out = wr.data_ptr(), wsr, out.data_ptr()
     _lib.call(lib.rp_embedding_fwd, out.device, ctypes.byref(a))
@@ -45,10 +47,12 @@ class _HipEmbedding(torch.autograd.Function):
         lib = _lib.load()
         (ids,) = ctx.saved_tensors
         (V, d), wt, scale, padding, out_dtype = ctx.args
+        dw = torch.empty((V, d), dtype=wt, device=dout.device)
+        if d == 0:
+            return None, dw, None, None, None
         ids = ids.contiguous()
         a = _args(ids, V, d, wt, out_dtype, scale, padding)
         dr, _, dsr = rows_of(dout, d)
-        dw = torch.empty((V, d), dtype=wt, device=dout.device)
         nbytes = lib.rp_embedding_work_bytes(ctypes.byref(a))
         work = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dout.device)
         g = _lib.EmbeddingGrad(dr.data_ptr(), dsr, dw.data_ptr(), work.data_ptr(), nbytes)

@@ -50,6 +50,9 @@ def _work(lib, a, device):
 def _forward(x, gate, h0, starts, keep):
     lib = _lib.load()
     B, L, D = x.shape
+    if x.numel() == 0:  # the last state is the first
+        last = torch.zeros((B, D), dtype=torch.float32, device=x.device)
+        return torch.empty((B, L, D), dtype=x.dtype, device=x.device), last if h0 is None else last.copy_(h0), None
     a, hold = _args(x, gate, starts)
     y = torch.empty((B, L, D), dtype=x.dtype, device=x.device)
     last = torch.empty((B, D), dtype=torch.float32, device=x.device)
@@ -84,6 +87,10 @@ class _HipGatedScan(torch.autograd.Function):
         lib = _lib.load()
         x, gate, starts, ckpt = ctx.saved_tensors
         B, L, D = x.shape
+        need = ctx.needs_input_grad
+        if x.numel() == 0:
+            return (torch.zeros_like(x) if need[0] else None, torch.zeros_like(gate) if need[1] else None,
+                    dlast if need[2] else None, None)
         a, hold = _args(x, gate, starts)
         a.ckpt = ckpt.data_ptr()
         work = _work(lib, a, x.device)  # noqa: F841  (held until the launch)
@@ -97,11 +104,10 @@ class _HipGatedScan(torch.autograd.Function):
             dlast = dlast.contiguous()
             g.dh_last = dlast.data_ptr()
         dh0 = None
-        if ctx.needs_input_grad[2]:
+        if need[2]:
             dh0 = torch.empty((B, D), dtype=torch.float32, device=x.device)
             g.dh0 = dh0.data_ptr()
         _lib.call(lib.rp_gated_bwd, x.device, ctypes.byref(a), ctypes.byref(g))
-        need = ctx.needs_input_grad
         return dx if need[0] else None, dgate if need[1] else None, dh0, None
 
 
@@ -145,9 +151,6 @@ def hip_gated_scan(x, gate, h0=None, starts=None):
         if starts.dtype is not torch.bool:
             raise TypeError(f"redpanda_amd gated_scan: starts must be bool, got {starts.dtype}")
         starts = starts.contiguous()
-    if x.numel() == 0:
-        last = torch.zeros((B, D), dtype=torch.float32, device=dev) if h0 is None else h0.clone()
-        return x.new_empty((B, L, D)), last
     if recorded(grad):
         return _HipGatedScan.apply(x, gate, h0, starts)
     return _forward(x, gate, h0, starts, False)[:2]

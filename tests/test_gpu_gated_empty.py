@@ -22,7 +22,7 @@ def test_an_empty_batch_trains(gpu_lib, B, L, D, state, t):
     assert y.requires_grad and last.requires_grad
     assert torch.equal(last, torch.zeros(B, D, device=dev) if h0 is None else h0)
     dh = torch.randn(B, D, device=dev)
-    grads = torch.autograd.grad((y, last), leaves, (torch.zeros_like(y), dh))
+    grads = torch.autograd.grad((y, last), leaves, (torch.zeros_like(y), dh), retain_graph=True)
     assert all(g.shape == v.shape and g.dtype == v.dtype for g, v in zip(grads, leaves))
     if state and L == 0:
         assert torch.equal(grads[2], dh)

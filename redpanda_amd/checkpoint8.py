@@ -87,13 +87,14 @@ class _HipCheckpoint8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, fn, x, add, w, eps, out_dtype, *params):
         total, normed, kept, wc, a = norm_forward(x, add, w, eps, out_dtype, True)
-        if torch.is_autocast_enabled("cuda"):
-            # (a weight cast here, where nothing is recorded, must not be found in
-            # autocast's cache by a later use that is)
-            with torch.autocast("cuda", dtype=torch.get_autocast_dtype("cuda"), cache_enabled=False):
-                out = fn(normed)
-        else:
+        try:
             out = fn(normed)
+        finally:
+            # (a weight cast here, where nothing is recorded, must not be found in
+            # autocast's cache by a later use that is; fn may turn the cache on itself, so
+            # that it is emptied, not kept off)
+            if torch.is_autocast_enabled("cuda"):
+                torch.clear_autocast_cache()
         _one_tensor(out)
         ctx.save_for_backward(wc, *kept)
         # (not saved: their gradients are asked for by identity, and hooks on saved tensors,

@@ -93,6 +93,22 @@ class RMSNorm(nn.Module):
         return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + self.eps) * self.weight
 
 
+_RMS_FORWARD = RMSNorm.forward
+_EMBEDDING_FORWARD = nn.Embedding.forward
+
+
+def _need_own(module, forward, what):
+    """ValueError unless a call of `module` is `forward` and nothing besides: the fused
+    path computes it from its weight."""
+    if getattr(type(module), "forward", None) is not forward or "forward" in module.__dict__:
+        raise ValueError(f"Mamba.forward: fused and keep8 compute {what} themselves, but a "
+                         f"{type(module).__name__} with a forward of its own stands there")
+    if (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or
+            module._backward_pre_hooks):
+        raise ValueError(f"Mamba.forward: fused and keep8 do not call {what} as a module, which "
+                         "would leave out the hooks on it")
+
+
 def _gate_out_dtype():
     """The dtype out_proj will read the gate's output in: autocast's when it
     is on for the device, so the gate writes it directly (the same rounding
@@ -391,7 +407,11 @@ class Mamba(nn.Module):
         each way, where torch takes one for each operation; the norm's result is in the
         dtype that in_proj reads it in.  keep8 (fused too): each layer is checkpointed
         with its input in 8 bits (hip_checkpoint8), whatever grad_checkpoint says: the
-        output is the same, the gradients are those at the kept values."""
+        output is the same, the gradients are those at the kept values.
+        On the fused path the norms and the embedding are computed from their weights, not
+        called as modules: ones with a forward or hooks of their own are refused, as are an
+        embedding's max_norm, scale_grad_by_freq and sparse; hooks for all modules do not see
+        them.  An id outside the vocabulary is padding there (a row of zeros, no gradient)."""
         if embed_scale != 1.0 and input_embeds is not None:
             raise ValueError("Mamba.forward: embed_scale scales the embedding of input_ids, not input_embeds")
         if fused or keep8:
@@ -418,9 +438,17 @@ class Mamba(nn.Module):
         return self.norm_f(x)
 
     def _forward_fused(self, input_ids, input_embeds, dropout, seed, embed_scale, keep8):
+        for layer in self.layers:
+            _need_own(layer["norm"], _RMS_FORWARD, "a layer's norm")
+        _need_own(self.norm_f, _RMS_FORWARD, "norm_f")
         x = input_embeds
         if x is None:
-            x = hip_embedding(input_ids, self.embedding.weight, scale=embed_scale)
+            emb = self.embedding
+            _need_own(emb, _EMBEDDING_FORWARD, "the embedding")
+            if emb.max_norm is not None or emb.scale_grad_by_freq or emb.sparse:
+                raise ValueError("Mamba.forward: fused and keep8 have no max_norm, scale_grad_by_freq "
+                                 "or sparse gradient for the embedding")
+            x = hip_embedding(input_ids, emb.weight, scale=embed_scale, padding_idx=emb.padding_idx)
         branch, dtype = None, _gate_out_dtype()
         for i, layer in enumerate(self.layers):
             mixer, norm = layer["mixer"], layer["norm"]

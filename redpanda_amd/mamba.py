@@ -467,7 +467,14 @@ class Mamba(nn.Module):
                 x, branch = hip_dropout(out, dropout, seed, residual=x, stream=i), None
             else:
                 branch = out  # added with the next norm
-        got = hip_rmsnorm(x, self.norm_f.weight, self.norm_f.eps, add=branch)
+        # (the type that the plain norm's products have: autocast takes its powers in fp32)
+        w, out_dtype = self.norm_f.weight, x.dtype
+        for other in (w, branch):
+            if other is not None:
+                out_dtype = torch.promote_types(out_dtype, other.dtype)
+        if torch.is_autocast_enabled("cuda"):
+            out_dtype = torch.float32
+        got = hip_rmsnorm(x, w, self.norm_f.eps, add=branch, out_dtype=out_dtype)
         return got if branch is None else got[1]
 
     def init_cache(self, batch_size, device):

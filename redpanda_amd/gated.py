@@ -61,8 +61,10 @@ def _forward(x, gate, h0, starts, keep):
         a.h0 = h0.data_ptr()
     ckpt = None
     if keep:
-        ckpt = torch.empty(lib.rp_gated_ckpt_bytes(ctypes.byref(a)) // 4, dtype=torch.float32,
-                           device=x.device)
+        nbytes = lib.rp_gated_ckpt_bytes(ctypes.byref(a))
+        if nbytes < 0:
+            _lib.check(lib.rp_gated_check(ctypes.byref(a)), lib)
+        ckpt = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
         a.ckpt = ckpt.data_ptr()
     work = _work(lib, a, x.device)  # noqa: F841  (held until the launch)
     a.y, a.h_last = y.data_ptr(), last.data_ptr()

@@ -527,7 +527,9 @@ typedef struct rp_embedding_args {
  * with ids[i] = v, in fp32 and in a fixed order (the places are sorted by their
  * ids), rounded once; zeros for ids that do not occur.  dout: (N, d) in dtype_out
  * with row stride dout_sr; dw: (V, d) contiguous in dtype_w.  The forward's w and
- * out are not read.  work: rp_embedding_work_bytes() of scratch, 256-byte aligned.
+ * out are not read.  work: rp_embedding_work_bytes() of scratch, 256-byte aligned: 17
+ * bytes an id, 8 d a share of 32 to 128 ids, and for the counters a few megabytes, or
+ * where the table has millions of rows up to 36 bytes a row (4 for up to 4096 ids).
  */
 typedef struct rp_embedding_grad {
   const void* dout; int64_t dout_sr;
@@ -602,7 +604,8 @@ typedef struct rp_addnorm_args {
  * dtype_out; dsum: NULL or (rows, d) in dtype_sum; dx, dadd: NULL or (rows, d)
  * contiguous, ds in dtype_x and in dtype_add; dw: NULL or (d,) fp32, summed in a
  * fixed order.  The forward's add, sum and out are not read.  work:
- * rp_addnorm_work_bytes() of scratch, 256-byte aligned (unused without dw).
+ * rp_addnorm_work_bytes() of scratch, 256-byte aligned (without dw used for rows of
+ * more than 16384 columns only, whose r it holds).
  */
 typedef struct rp_addnorm_grad {
   const void* dout; int64_t dout_sr;

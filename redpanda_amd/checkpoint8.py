@@ -138,7 +138,8 @@ def hip_checkpoint8(fn, x, weight=None, eps=1e-5, add=None, out_dtype=None, para
 
     x, add, weight, eps, out_dtype: as in hip_rmsnorm.  fn: a function of the normed rows
     that gives one tensor; it runs again in the backward, on the norm of the values that
-    8 bits hold, and must then do the same (no random numbers but from seeds of its own).
+    8 bits hold, and must then do the same (no random numbers but from seeds of its own);
+    its argument may not be changed in place.
     params: the tensors it reads whose gradients are wanted, as a module's
     parameters().  The results are those of the plain layer; its gradients are the exact
     ones at the kept values.  Differentiable once and in reverse mode."""

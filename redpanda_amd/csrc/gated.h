@@ -88,8 +88,10 @@ __device__ __forceinline__ void gated_store(char* row, uint32_t at, const float 
   }
 }
 
-// a = 1 / (1 + exp(-z)) and 1 - a, both to full relative accuracy: of exp(-|z|) / (1 +
-// exp(-|z|)) and 1 / (1 + exp(-|z|)) each is the one or the other.
+// a = 1 / (1 + exp(-z)) and 1 - a, neither from the other by a subtraction: of exp(-|z|) /
+// (1 + exp(-|z|)) and 1 / (1 + exp(-|z|)) each is the one or the other.  The exponent |z|
+// log2 e is rounded, so each is off by up to (2 |z| + 6) 2^-24 of itself; the smaller is 0
+// beyond |z| = 87.3, where fp32's normal numbers end.
 __device__ __forceinline__ void gate_of(float z, float& a, float& na) {
   const float e = exp2_hw(fabsf(z) * -kLog2e);
   const float big = __builtin_amdgcn_rcpf(1.f + e), small = e * big;

@@ -7,9 +7,14 @@
 // forward the waves of a workgroup stand one behind the other in time, and the time
 // axis is split among workgroups where there are few.
 //
-// Registers bound it: 16 steps of gates, complements and factors are a wave's, and three
-// waves a SIMD fit (256 x 64 x 1536 bf16: 63 us, 50 at the rate of a large copy; 64 x 2048
-// x 1024 319 for 267; 1 x 131072 x 1024: sums 143, join 8, main 290 for 261).
+// Registers bound it: 16 steps of gates, complements and factors are a wave's; two channels
+// a lane take 168 and three waves a SIMD, one channel 120 and four.  The rows' scalar
+// addresses, of 16 steps and up to five arrays in two unrolled bodies, do not fit the scalar
+// registers: 360 to 440 of them are kept in lanes of vector registers, and with two channels
+// 12 bytes a lane are in scratch, 232 in the kernel of up to 16 steps.  (256 x 64 x 1536
+// bf16: 64 us, 50 at the rate of a large copy; 64 x 2048 x 1024 300 for 267; 1 x 131072 x
+// 1024: sums 144, join 9, main 293 for 261; 4096 x 1 x 1024 93 for 18, 4096 x 12 x 1024 251
+// for 108.)
 
 #include "gated.h"
 

@@ -13,7 +13,7 @@
 // then.
 //
 // HBM bounds it where the card is full (256 x 64 x 1536 bf16: 33 us, 31 at the rate of a
-// large copy; 64 x 2048 x 1024 177 for 163; 1 x 131072 x 1024: sums 125, join 8, main 161
+// large copy; 64 x 2048 x 1024 174 for 163; 1 x 131072 x 1024: sums 129, join 9, main 160
 // for 157).  A wave that walked its whole stretch with eight steps loaded ahead took 45
 // us for the first and 422 for the last.
 

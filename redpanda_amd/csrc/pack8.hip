@@ -1,6 +1,6 @@
 // Rows to 8 bits and back (the format is described in rp_pack8.h): one thread per
 // eight columns, four adjacent threads a block of 32.  HBM bounds both (131072 x 1024
-// bf16: 85 us there and 77 back, 79 each at the rate of a large copy; 16384 x 768 fp32 11
+// bf16: 88 us there and 83 back, 79 each at the rate of a large copy; 16384 x 768 fp32 11
 // and 13).
 
 #include "rp_pack8.h"
